@@ -8,9 +8,10 @@ call does, and it raises if the library is missing (there is no fallback path).
 """
 from .action_selection import (GumbelMuZeroExtraData, gumbel_muzero_interior_action_selection,
                                gumbel_muzero_root_action_selection, muzero_action_selection,
-                               sampled_muzero_action_selection)
+                               sample_actions, sampled_muzero_action_selection)
 from .base import (ChanceRecurrentFnOutput, DecisionRecurrentFnOutput, PolicyOutput, RecurrentFnOutput,
                    RootFnOutput, StochasticRecurrentState)
+from .layers import dense, layer_norm
 from .networks import FusedModel, FusedRecurrentFn, init_mlp
 from .policies import (actor_post, gumbel_muzero_policy, muzero_policy, sampled_muzero_policy,
                        stochastic_muzero_policy)
@@ -35,5 +36,5 @@ __all__ = [
     "qtransform_by_parent_and_siblings", "qtransform_completed_by_mix_value",
     "sampled_muzero_action_selection", "sampled_muzero_policy", "search",
     "ChanceRecurrentFnOutput", "DecisionRecurrentFnOutput", "StochasticRecurrentState",
-    "stochastic_muzero_policy", "minatar",
+    "stochastic_muzero_policy", "minatar", "dense", "layer_norm", "sample_actions",
 ]

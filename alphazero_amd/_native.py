@@ -84,11 +84,21 @@ class ReplayState(C.Structure):
                 ("sample_position", C.c_int32)]
 
 
+class SampleDesc(C.Structure):
+    """az_sample_desc (include/az_layers.h)."""
+    _fields_ = [("dtype", C.c_int32), ("rows", C.c_int32), ("actions", C.c_int32), ("top_k", C.c_int32),
+                ("temperature", C.c_double), ("top_p", C.c_double), ("min_p", C.c_double)] + \
+        [(n, C.c_void_p) for n in ("logits", "uniform", "invalid", "temperature_rows", "top_k_rows",
+                                   "top_p_rows", "min_p_rows")]
+
+
 _P = C.c_void_p
 _I = C.c_int32
 _F = C.c_float
 _K2 = C.POINTER(C.c_uint32 * 2)
 
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2                       # include/az_layers.h
+ACT_NONE, ACT_RELU, ACT_SWISH, ACT_GELU = 0, 1, 2, 3
 BREAKOUT_WORDS, BREAKOUT_OBS, BREAKOUT_ACTIONS = 20, 400, 3   # include/az_minatar.h
 
 # name -> (restype, argtypes); every symbol declared in include/az_mcts.h, az_replay.h, az_minatar.h
@@ -148,6 +158,17 @@ SIGNATURES = {
     "az_threefry": (C.c_int, [_I, _P, _P, _P, _P]),
 }
 
+# the same for include/az_layers.h
+LAYER_SIGNATURES = {
+    "az_dense_workspace_bytes": (C.c_int64, [_I, _I, _I, _I, _I]),
+    "az_dense_forward": (C.c_int, [_I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "az_dense_backward": (C.c_int, [_I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "az_layer_norm_workspace_bytes": (C.c_int64, [_I, _I]),
+    "az_layer_norm_forward": (C.c_int, [_I, _I, _I, _I, _P, _P, _P, _F, _P, _P, _P, _P]),
+    "az_layer_norm_backward": (C.c_int, [_I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P, C.c_int64, _P]),
+    "az_sample_actions": (C.c_int, [C.POINTER(SampleDesc), _P, _P, _P]),
+}
+
 _lib = None
 
 
@@ -163,7 +184,7 @@ def lib():
             handle = C.CDLL(LIB_PATH)
         except OSError as e:  # pragma: no cover - depends on the machine
             raise NativeLibraryError(f"cannot load {LIB_PATH}: {e}") from e
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in {**SIGNATURES, **LAYER_SIGNATURES}.items():
             try:
                 fn = getattr(handle, name)
             except AttributeError as e:

@@ -4,8 +4,12 @@ The four selection rules run inside the HIP search kernels.  As in the
 reference, `search()` receives them as ``functools.partial`` objects binding
 their keyword options; here the functions are markers that identify the rule
 and carry those options to the kernels.
+
+`sample_actions` selects without a search: a draw from (truncated) policy logits.
 """
+import ctypes as C
 import dataclasses
+import math
 from typing import Any
 
 from . import _native as nat
@@ -105,3 +109,59 @@ def resolve(root_fn, interior_fn, desc, num_simulations):
         raise NotImplementedError("root and interior selection must use the same qtransform")
     qt.apply_to_desc(q_int, desc)
     return desc
+
+
+def sample_actions(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, invalid_actions=None):
+    """Draws one action a row from truncated policy logits: (action int32 [B], log_prob float32 [B]).
+
+    logits [B, A] float32 / bfloat16 / float16; uniform [B] float32, the row's random number in [0, 1);
+    invalid_actions [B, A], nonzero where an action is illegal.  Of the legal actions in descending order of their
+    logits (equal ones by index) the first `top_k` are kept (0: all), of these the fewest that hold
+    `top_p` of their probability, of these the ones with at least `min_p` of the largest one's probability (and
+    never one with less than 2^-40 of it).  The action is the first, in index order, whose cumulative
+    probability among the kept ones exceeds `uniform`; log_prob is its log probability among them.  temperature
+    divides the logits; 0 takes the largest one.  The four parameters are numbers or [B] tensors (in which a
+    negative or NaN temperature counts as 0, top_k <= 0 as all, and top_p, min_p beyond [0, 1] as the nearer end).
+    -inf and NaN logits are illegal; a row without a legal action gives action 0 and log_prob -inf.
+    """
+    import torch
+    from . import layers
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"sample_actions: logits {tuple(logits.shape)} must be [B, A] with A >= 1")
+    B, A = logits.shape
+    if logits.dtype not in layers.DTYPES:
+        raise TypeError(f"sample_actions: float32, bfloat16 or float16 logits, got {logits.dtype}")
+    if tuple(uniform.shape) != (B,) or uniform.dtype != torch.float32:
+        raise ValueError(f"sample_actions: uniform must be float32 [{B}], got {uniform.dtype} {tuple(uniform.shape)}")
+    if invalid_actions is not None and tuple(invalid_actions.shape) != (B, A):
+        raise ValueError(f"sample_actions: invalid_actions {tuple(invalid_actions.shape)} must be {(B, A)}")
+    d = nat.SampleDesc(dtype=layers.DTYPES[logits.dtype], rows=B, actions=A)
+    keep = []
+    for name, value, dtype, ok in (
+            ("temperature", temperature, torch.float32, lambda v: 0.0 <= v < math.inf),
+            ("top_k", top_k, torch.int32, lambda v: 0 <= v < 2 ** 31 and v == int(v)),
+            ("top_p", top_p, torch.float32, lambda v: 0.0 <= v <= 1.0),
+            ("min_p", min_p, torch.float32, lambda v: 0.0 <= v <= 1.0)):
+        if torch.is_tensor(value) and value.dim() > 0:
+            if tuple(value.shape) != (B,):
+                raise ValueError(f"sample_actions: {name} {tuple(value.shape)} must be a number or [{B}]")
+            if value.device != logits.device:
+                raise ValueError(f"sample_actions: {name} is on {value.device}, logits on {logits.device}")
+            keep.append(value.to(dtype).contiguous())
+            setattr(d, name + "_rows", keep[-1].data_ptr())
+        else:
+            if not ok(value):
+                raise ValueError(f"sample_actions: {name}={value}")
+            setattr(d, name, int(value) if name == "top_k" else float(value))
+    layers._checked("sample_actions", logits, (("uniform", uniform), ("invalid_actions", invalid_actions)))
+    logits, uniform = logits.detach().contiguous(), uniform.contiguous()
+    d.logits, d.uniform = logits.data_ptr(), uniform.data_ptr()
+    if invalid_actions is not None:
+        if invalid_actions.dtype not in (torch.bool, torch.uint8, torch.int8):
+            invalid_actions = invalid_actions != 0
+        keep.append(invalid_actions.contiguous())
+        d.invalid = keep[-1].data_ptr()
+    action = torch.empty((B,), dtype=torch.int32, device=logits.device)
+    log_prob = torch.empty((B,), dtype=torch.float32, device=logits.device)
+    layers._native(logits.device, nat.lib().az_sample_actions, C.byref(d), nat.ptr(action), nat.ptr(log_prob))
+    return action, log_prob

@@ -1,0 +1,383 @@
+// az_norm.hip -- layer norm over the last axis and its backward pass (include/az_layers.h).
+// Part of libaz_mcts.so (gfx950 only).
+//
+// Bound by memory: the forward pass reads x and writes y once, the backward pass reads x and dy and writes dx once.
+// A row stays in the registers of NT threads between its sums and its outputs, so the variance is taken from the
+// differences to the mean (no cancellation), and the backward pass adds its row's share of the scale's and bias'
+// gradients to registers that a thread keeps for its columns over all rows of its workgroup.
+#include <hip/hip_runtime.h>
+
+#include "az_host.h"
+#include "az_types.h"
+
+namespace {
+
+struct Norm {
+  const void* x;
+  const void* scale;
+  const void* bias;
+  const void* dy;
+  void* out;            // y or dx
+  float* mean;
+  float* rstd;
+  float* partial;       // [blocks][2][width]: scale's, bias' gradient
+  float eps;
+  int rows, width;
+};
+
+// V elements of a row from column c; 0 beyond its end.
+template <typename T, int V>
+__device__ __forceinline__ void load_row(const T* row, int c, int width, float* v) {
+  if (c + V <= width) {
+    const AzVec<T, V> r = az_loadu<T, V>(row + c);
+    for (int i = 0; i < V; ++i) v[i] = (float)r.v[i];
+  } else {
+    for (int i = 0; i < V; ++i) v[i] = c + i < width ? (float)row[c + i] : 0.0f;
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_row(T* row, int c, int width, const float* v) {
+  if (c + V <= width) {
+    AzVec<T, V> r;
+    for (int i = 0; i < V; ++i) r.v[i] = (T)v[i];
+    az_storeu<T, V>(row + c, r);
+  } else {
+    for (int i = 0; i < V; ++i)
+      if (c + i < width) row[c + i] = (T)v[i];
+  }
+}
+
+// Sum over the NT threads of a row, the same in each of them.  `scratch` holds NT / 64 floats and may be used again
+// after the next barrier.
+template <int NT>
+__device__ __forceinline__ float row_sum(float s, float* scratch) {
+  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
+  if constexpr (NT > 64) {
+    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = 0.0f;
+    for (int i = 0; i < NT / 64; ++i) s += scratch[i];
+  }
+  return s;
+}
+
+template <typename T>
+constexpr int vec_of() {
+  return 16 / sizeof(T);
+}
+
+// NT threads a row, R 16-byte loads a thread; workgroups of max(NT, 256) threads.
+template <typename T, typename P, int NT, int R>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm_forward(Norm p) {
+  constexpr int V = vec_of<T>(), ROWS = NT < 256 ? 256 / NT : 1;
+  __shared__ float scratch[2][NT / 64];
+  const int t = threadIdx.x % NT;
+  const int m = blockIdx.x * ROWS + threadIdx.x / NT;
+  if (m >= p.rows) return;   // (whole waves; with NT > 64 a workgroup has one row)
+  const T* x = (const T*)p.x + (int64_t)m * p.width;
+  float v[R][V];
+  float s = 0.0f;
+  for (int r = 0; r < R; ++r) {
+    load_row<T, V>(x, (r * NT + t) * V, p.width, v[r]);
+    for (int i = 0; i < V; ++i) s += v[r][i];
+  }
+  const float mean = row_sum<NT>(s, scratch[0]) / p.width;
+  s = 0.0f;
+  for (int r = 0; r < R; ++r)
+    for (int i = 0; i < V; ++i) {
+      v[r][i] -= mean;
+      if ((r * NT + t) * V + i < p.width) s += v[r][i] * v[r][i];
+    }
+  const float rstd = 1.0f / sqrtf(row_sum<NT>(s, scratch[1]) / p.width + p.eps);
+  T* y = (T*)p.out + (int64_t)m * p.width;
+  for (int r = 0; r < R; ++r) {
+    const int c = (r * NT + t) * V;
+    float g[V], b[V];
+    if (p.scale) load_row<P, V>((const P*)p.scale, c, p.width, g);
+    if (p.bias) load_row<P, V>((const P*)p.bias, c, p.width, b);
+    for (int i = 0; i < V; ++i) {
+      float o = v[r][i] * rstd;
+      if (p.scale) o *= g[i];
+      if (p.bias) o += b[i];
+      v[r][i] = o;
+    }
+    store_row<T, V>(y, c, p.width, v[r]);
+  }
+  if (t == 0 && p.mean) p.mean[m] = mean, p.rstd[m] = rstd;
+}
+
+template <typename T, typename P, int NT, int R>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm_backward(Norm p) {
+  constexpr int V = vec_of<T>(), ROWS = NT < 256 ? 256 / NT : 1, W = NT * V * R;
+  __shared__ float scratch[4][NT / 64];
+  __shared__ float joined[ROWS > 1 ? 2 * W : 1];
+  const int t = threadIdx.x % NT, g = threadIdx.x / NT;
+  float ds[R][V] = {}, db[R][V] = {}, gain[R][V];
+  for (int r = 0; r < R; ++r) {
+    if (p.scale)
+      load_row<P, V>((const P*)p.scale, (r * NT + t) * V, p.width, gain[r]);
+    else
+      for (int i = 0; i < V; ++i) gain[r][i] = 1.0f;
+  }
+  int phase = 0;
+  for (int m = blockIdx.x * ROWS + g; m < p.rows; m += gridDim.x * ROWS, phase ^= 2) {
+    const int64_t at = (int64_t)m * p.width;
+    const float mean = p.mean[m], rstd = p.rstd[m];
+    float x[R][V], h[R][V], s1 = 0.0f, s2 = 0.0f;
+    for (int r = 0; r < R; ++r) {
+      load_row<T, V>((const T*)p.x + at, (r * NT + t) * V, p.width, x[r]);
+      load_row<T, V>((const T*)p.dy + at, (r * NT + t) * V, p.width, h[r]);
+    }
+    for (int r = 0; r < R; ++r)
+      for (int i = 0; i < V; ++i) {
+        x[r][i] = (x[r][i] - mean) * rstd;
+        ds[r][i] += h[r][i] * x[r][i];
+        db[r][i] += h[r][i];
+        h[r][i] *= gain[r][i];
+        s1 += h[r][i];          // (beyond the row's end h is 0)
+        s2 += h[r][i] * x[r][i];
+      }
+    if (!p.out) continue;
+    // (two sets of scratch in turn: a set is written again only behind the other set's barrier)
+    s1 = row_sum<NT>(s1, scratch[phase]) / p.width;
+    s2 = row_sum<NT>(s2, scratch[phase + 1]) / p.width;
+    for (int r = 0; r < R; ++r) {
+      for (int i = 0; i < V; ++i) h[r][i] = rstd * (h[r][i] - s1 - x[r][i] * s2);
+      store_row<T, V>((T*)p.out + at, (r * NT + t) * V, p.width, h[r]);
+    }
+  }
+  if (!p.partial) return;
+  if constexpr (ROWS > 1) {   // the workgroup's rows, in their order
+    for (int k = 0; k < ROWS; ++k) {
+      if (g == k)
+        for (int r = 0; r < R; ++r)
+          for (int i = 0; i < V; ++i) {
+            const int c = (r * NT + t) * V + i;
+            joined[c] = k ? joined[c] + ds[r][i] : ds[r][i];
+            joined[W + c] = k ? joined[W + c] + db[r][i] : db[r][i];
+          }
+      __syncthreads();
+    }
+    float* out = p.partial + (int64_t)blockIdx.x * 2 * p.width;
+    for (int c = threadIdx.x; c < p.width; c += ROWS * NT) out[c] = joined[c], out[p.width + c] = joined[W + c];
+  } else {
+    float* out = p.partial + (int64_t)blockIdx.x * 2 * p.width;
+    for (int r = 0; r < R; ++r) {
+      store_row<float, V>(out, (r * NT + t) * V, p.width, ds[r]);
+      store_row<float, V>(out + p.width, (r * NT + t) * V, p.width, db[r]);
+    }
+  }
+}
+
+// Rows too wide for the registers: a workgroup a row, which it reads again from L2 for each sum.
+template <typename T, typename P>
+__global__ __launch_bounds__(1024) void k_norm_forward_wide(Norm p) {
+  __shared__ float scratch[2][16];
+  const int64_t at = (int64_t)blockIdx.x * p.width;
+  const T* x = (const T*)p.x + at;
+  float s = 0.0f;
+  for (int c = threadIdx.x; c < p.width; c += 1024) s += (float)x[c];
+  const float mean = row_sum<1024>(s, scratch[0]) / p.width;
+  s = 0.0f;
+  for (int c = threadIdx.x; c < p.width; c += 1024) {
+    const float d = (float)x[c] - mean;
+    s += d * d;
+  }
+  const float rstd = 1.0f / sqrtf(row_sum<1024>(s, scratch[1]) / p.width + p.eps);
+  for (int c = threadIdx.x; c < p.width; c += 1024) {
+    float o = ((float)x[c] - mean) * rstd;
+    if (p.scale) o *= (float)((const P*)p.scale)[c];
+    if (p.bias) o += (float)((const P*)p.bias)[c];
+    ((T*)p.out)[at + c] = (T)o;
+  }
+  if (threadIdx.x == 0 && p.mean) p.mean[blockIdx.x] = mean, p.rstd[blockIdx.x] = rstd;
+}
+
+template <typename T, typename P>
+__global__ __launch_bounds__(1024) void k_norm_backward_wide(Norm p) {
+  __shared__ float scratch[2][16];
+  const int64_t at = (int64_t)blockIdx.x * p.width;
+  const float mean = p.mean[blockIdx.x], rstd = p.rstd[blockIdx.x];
+  auto h_of = [&](int c) {
+    const float d = (float)((const T*)p.dy)[at + c];
+    return p.scale ? d * (float)((const P*)p.scale)[c] : d;
+  };
+  auto x_of = [&](int c) { return ((float)((const T*)p.x)[at + c] - mean) * rstd; };
+  float s1 = 0.0f, s2 = 0.0f;
+  for (int c = threadIdx.x; c < p.width; c += 1024) {
+    const float h = h_of(c);
+    s1 += h;
+    s2 += h * x_of(c);
+  }
+  s1 = row_sum<1024>(s1, scratch[0]) / p.width;
+  s2 = row_sum<1024>(s2, scratch[1]) / p.width;
+  for (int c = threadIdx.x; c < p.width; c += 1024)
+    ((T*)p.out)[at + c] = (T)(rstd * (h_of(c) - s1 - x_of(c) * s2));
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_norm_columns_wide(Norm p) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= p.width) return;
+  float ds = 0.0f, db = 0.0f;
+  for (int m = blockIdx.y; m < p.rows; m += gridDim.y) {
+    const int64_t at = (int64_t)m * p.width + c;
+    const float d = (float)((const T*)p.dy)[at];
+    ds += d * (((float)((const T*)p.x)[at] - p.mean[m]) * p.rstd[m]);
+    db += d;
+  }
+  p.partial[(int64_t)blockIdx.y * 2 * p.width + c] = ds;
+  p.partial[(int64_t)blockIdx.y * 2 * p.width + p.width + c] = db;
+}
+
+// Column sums of the workgroups' partial gradients, in their order: 64 columns a workgroup, 16 threads a column.
+template <typename P>
+__global__ __launch_bounds__(1024) void k_norm_join(const float* partial, int blocks, int width, P* dscale, P* dbias) {
+  __shared__ float sums[16][64];
+  const int which = blockIdx.y, g = threadIdx.x & 63, w = threadIdx.x >> 6;
+  P* out = which ? dbias : dscale;
+  if (!out) return;
+  const int c = blockIdx.x * 64 + g;
+  float s = 0.0f;
+  if (c < width) {
+#pragma unroll 8
+    for (int i = w; i < blocks; i += 16) s += partial[((int64_t)i * 2 + which) * width + c];
+  }
+  sums[w][g] = s;
+  __syncthreads();
+  if (w != 0 || c >= width) return;
+  s = 0.0f;
+  for (int i = 0; i < 16; ++i) s += sums[i][g];
+  out[c] = (P)s;
+}
+
+template <typename P>
+__global__ void k_norm_zero(P* a, P* b, int n) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  if (a) a[i] = (P)0.0f;
+  if (b) b[i] = (P)0.0f;
+}
+
+// ---------------------------------------------------------------------------
+constexpr int IN_REGISTERS = 16384;   // widest row of the register form: 1024 threads x 16 elements
+
+int threads_of(int width) { return width <= 1024 ? 64 : width <= 4096 ? 256 : 1024; }
+
+// Workgroups of the backward pass, each of which leaves a row of partial column sums.
+int backward_blocks(int64_t rows, int width) {
+  const int64_t per = width <= 1024 ? 4 : 1, most = width <= 4096 ? 512 : 256;
+  const int64_t n = az_ceil(rows, per);
+  return (int)(n < most ? n : most);
+}
+
+// Calls f.operator()<T, P, NT, R>() for the row's threads and loads.
+template <typename T, typename P, typename F>
+void with_shape(int width, F&& f) {
+  constexpr int V = vec_of<T>(), FULL = 16 / V;   // 16 elements a thread
+  const int nt = threads_of(width);
+  if (nt == 64) {
+    if (width <= 64 * V) return f.template operator()<64, 1>();
+    if constexpr (FULL > 2)
+      if (width <= 128 * V) return f.template operator()<64, 2>();
+    return f.template operator()<64, FULL>();
+  }
+  if (nt == 256) {
+    if (width <= 256 * 2 * V && FULL > 2) return f.template operator()<256, 2>();
+    return f.template operator()<256, FULL>();
+  }
+  return f.template operator()<1024, FULL>();
+}
+
+int check(int dtype, int param_dtype, int64_t rows, int64_t width) {
+  if (dtype < AZ_TYPE_F32 || dtype > AZ_TYPE_F16 || (param_dtype != dtype && param_dtype != AZ_TYPE_F32))
+    return az_fail(AZ_ERR_INVALID, "layer norm: types %d and %d", dtype, param_dtype);
+  if (rows < 0 || width < 1)
+    return az_fail(AZ_ERR_INVALID, "layer norm: rows=%lld width=%lld", (long long)rows, (long long)width);
+  if (rows > 0x7fff0000 || width > AZ_NORM_MAX_WIDTH)
+    return az_fail(AZ_ERR_UNSUPPORTED, "layer norm: rows up to %d, width up to %d", 0x7fff0000, AZ_NORM_MAX_WIDTH);
+  return AZ_OK;
+}
+
+template <typename F>
+int with_types(int dtype, int param_dtype, F&& f) {
+  return az_dispatch_type(dtype, [&]<typename T>() -> int {
+    if (param_dtype == AZ_TYPE_F32) return f.template operator()<T, float>();
+    return f.template operator()<T, T>();
+  });
+}
+
+}  // namespace
+
+extern "C" int az_layer_norm_forward(int32_t dtype, int32_t param_dtype, int32_t rows, int32_t width, const void* x,
+                                     const void* scale, const void* bias, float eps, void* y, float* mean,
+                                     float* rstd, void* stream_) {
+  if (int rc = check(dtype, param_dtype, rows, width)) return rc;
+  if (rows == 0) return AZ_OK;
+  if (!x || !y || !mean != !rstd) return az_fail(AZ_ERR_INVALID, "layer norm: null x or y, or one of mean and rstd");
+  hipStream_t stream = (hipStream_t)stream_;
+  Norm p = {};
+  p.x = x, p.scale = scale, p.bias = bias, p.out = y, p.mean = mean, p.rstd = rstd, p.eps = eps;
+  p.rows = rows, p.width = width;
+  return with_types(dtype, param_dtype, [&]<typename T, typename P>() -> int {
+    if (width > IN_REGISTERS) {
+      k_norm_forward_wide<T, P><<<dim3(rows), dim3(1024), 0, stream>>>(p);
+    } else {
+      with_shape<T, P>(width, [&]<int NT, int R>() {
+        constexpr int ROWS = NT < 256 ? 256 / NT : 1;
+        k_norm_forward<T, P, NT, R><<<dim3((unsigned)az_ceil(rows, ROWS)), dim3(NT < 256 ? 256 : NT), 0, stream>>>(p);
+      });
+    }
+    AZ_LAUNCH_CHECK();
+    return AZ_OK;
+  });
+}
+
+extern "C" int64_t az_layer_norm_workspace_bytes(int32_t rows, int32_t width) {
+  if (check(AZ_TYPE_F32, AZ_TYPE_F32, rows, width) != AZ_OK) return -1;
+  return rows == 0 ? 0 : (int64_t)backward_blocks(rows, width) * 2 * width * 4;
+}
+
+extern "C" int az_layer_norm_backward(int32_t dtype, int32_t param_dtype, int32_t rows, int32_t width, const void* x,
+                                      const void* scale, const float* mean, const float* rstd, const void* dy,
+                                      void* dx, void* dscale, void* dbias, void* workspace, int64_t workspace_bytes,
+                                      void* stream_) {
+  if (int rc = check(dtype, param_dtype, rows, width)) return rc;
+  hipStream_t stream = (hipStream_t)stream_;
+  const bool columns = dscale || dbias;
+  if (!columns && !dx) return AZ_OK;
+  return with_types(dtype, param_dtype, [&]<typename T, typename P>() -> int {
+    if (rows == 0) {
+      if (columns)
+        k_norm_zero<P><<<dim3((unsigned)az_ceil(width, 256)), dim3(256), 0, stream>>>((P*)dscale, (P*)dbias, width);
+      AZ_LAUNCH_CHECK();
+      return AZ_OK;
+    }
+    if (!x || !mean || !rstd || !dy) return az_fail(AZ_ERR_INVALID, "layer norm backward: null x, mean, rstd or dy");
+    const int blocks = backward_blocks(rows, width);
+    if (columns && (workspace_bytes < (int64_t)blocks * 2 * width * 4 || !workspace || !az_aligned16(workspace)))
+      return az_fail(AZ_ERR_INVALID, "layer norm: the workspace must hold %lld bytes, 16-byte aligned",
+                     (long long)blocks * 2 * width * 4);
+    Norm p = {};
+    p.x = x, p.scale = scale, p.dy = dy, p.out = dx, p.mean = const_cast<float*>(mean);
+    p.rstd = const_cast<float*>(rstd), p.partial = columns ? (float*)workspace : nullptr;
+    p.rows = rows, p.width = width;
+    if (width > IN_REGISTERS) {
+      if (dx) k_norm_backward_wide<T, P><<<dim3(rows), dim3(1024), 0, stream>>>(p);
+      if (columns)
+        k_norm_columns_wide<T><<<dim3((unsigned)az_ceil(width, 256), blocks), dim3(256), 0, stream>>>(p);
+    } else {
+      with_shape<T, P>(width, [&]<int NT, int R>() {
+        k_norm_backward<T, P, NT, R><<<dim3(blocks), dim3(NT < 256 ? 256 : NT), 0, stream>>>(p);
+      });
+    }
+    AZ_LAUNCH_CHECK();
+    if (columns) {
+      k_norm_join<P><<<dim3((unsigned)az_ceil(width, 64), 2), dim3(1024), 0, stream>>>((const float*)workspace, blocks,
+                                                                                     width, (P*)dscale, (P*)dbias);
+      AZ_LAUNCH_CHECK();
+    }
+    return AZ_OK;
+  });
+}

@@ -1,0 +1,202 @@
+"""Network layers as single operators: `dense` and `layer_norm`, with their gradients.
+
+The reference's networks are stacks of flax Dense layers and activations
+(networks/networks.py:25-48, kernel [in, out], bias [out]); these are such layers, and the ones a
+residual network puts around them, as HIP kernels of libaz_mcts.so (include/az_layers.h).  Float32,
+bfloat16 and float16; sums are held in float32 and an output is rounded once.  There is no CPU path.
+"""
+import torch
+
+from . import _native as nat
+
+DTYPES = {torch.float32: nat.TYPE_F32, torch.bfloat16: nat.TYPE_BF16, torch.float16: nat.TYPE_F16}
+ACTIVATIONS = {None: nat.ACT_NONE, "relu": nat.ACT_RELU, "swish": nat.ACT_SWISH, "gelu": nat.ACT_GELU}
+
+
+def _on(device):
+    """Native launches go to the current device's stream: makes `device` current if it is not."""
+    if device.index == torch.cuda.current_device():
+        return None
+    return torch.cuda.device(device)
+
+
+def _native(device, fn, *args):
+    guard = _on(device)
+    if guard is None:
+        nat.check(fn(*args, nat.stream_ptr()))
+    else:
+        with guard:
+            nat.check(fn(*args, nat.stream_ptr()))
+
+
+def _checked(op, x, others):
+    if x.dtype not in DTYPES:
+        raise TypeError(f"{op}: float32, bfloat16 or float16 tensors, got {x.dtype}")
+    for name, t in others:
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{op}: {name} is on {t.device}, x on {x.device}")
+    if x.device.type != "cuda":
+        raise NotImplementedError(f"{op}: tensors must be on the GPU (there is no CPU path)")
+
+
+# ---------------------------------------------------------------- dense
+def _dense_forward(x, kernel, bias, residual, act, keep_z):
+    """(y, z): x [M, K] and residual [M, N] contiguous."""
+    M, K = x.shape
+    N = kernel.shape[1]
+    code = DTYPES[x.dtype]
+    lib = nat.lib()
+    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    z = None
+    if keep_z and act != nat.ACT_NONE:
+        z = torch.empty((M, N), dtype=torch.float32 if x.dtype == torch.float32 else torch.float16, device=x.device)
+    n = lib.az_dense_workspace_bytes(code, M, K, N, 0)
+    if n < 0:
+        nat.check(-2)
+    ws = torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
+    _native(x.device, lib.az_dense_forward, code, act, M, K, N, nat.ptr(x), nat.ptr(kernel), nat.ptr(bias),
+            nat.ptr(residual), nat.ptr(y), nat.ptr(z), nat.ptr(ws), n)
+    return y, z
+
+
+class _Dense(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, kernel, bias, residual, act):
+        y, z = _dense_forward(x, kernel, bias, residual, act, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, kernel, z)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, kernel, z = ctx.saved_tensors
+        M, K = x.shape
+        N = kernel.shape[1]
+        need = ctx.needs_input_grad
+        dx = torch.empty_like(x) if need[0] else None
+        dkernel = torch.empty_like(kernel) if need[1] else None
+        dbias = torch.empty((N,), dtype=x.dtype, device=x.device) if need[2] else None
+        if need[0] or need[1] or need[2]:
+            g = dy.contiguous()
+            code = DTYPES[x.dtype]
+            lib = nat.lib()
+            n = lib.az_dense_workspace_bytes(code, M, K, N, 1)
+            ws = torch.empty((n,), dtype=torch.uint8, device=x.device)
+            _native(x.device, lib.az_dense_backward, code, ctx.act, M, K, N, nat.ptr(x), nat.ptr(kernel), nat.ptr(z),
+                    nat.ptr(g), nat.ptr(dx), nat.ptr(dkernel), nat.ptr(dbias), nat.ptr(ws), n)
+        return dx, dkernel, dbias, dy if need[3] else None, None
+
+
+def dense(x, kernel, bias=None, activation=None, residual=None):
+    """act(x @ kernel + bias) + residual, differentiable in every tensor.
+
+    x [..., fan_in], kernel [fan_in, fan_out], bias [fan_out], residual [..., fan_out] of one type
+    (float32, bfloat16 or float16) on one GPU; strided tensors are copied first.
+    activation: None, "relu", "swish" (z * sigmoid(z), networks/networks.py:25-48) or "gelu" (erf form).
+    """
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"dense: activation {activation!r} is not one of {list(ACTIVATIONS)}")
+    if kernel.dim() != 2 or x.dim() < 1 or x.shape[-1] != kernel.shape[0]:
+        raise ValueError(f"dense: x {tuple(x.shape)} and kernel {tuple(kernel.shape)} do not match")
+    shape = tuple(x.shape[:-1]) + (kernel.shape[1],)
+    if kernel.shape[0] < 1 or kernel.shape[1] < 1:
+        raise ValueError(f"dense: empty kernel {tuple(kernel.shape)}")
+    if bias is not None and tuple(bias.shape) != shape[-1:]:
+        raise ValueError(f"dense: bias {tuple(bias.shape)} does not match kernel {tuple(kernel.shape)}")
+    if residual is not None and tuple(residual.shape) != shape:
+        raise ValueError(f"dense: residual {tuple(residual.shape)} is not of the output's shape {shape}")
+    others = (("kernel", kernel), ("bias", bias), ("residual", residual))
+    for name, t in others:
+        if t is not None and t.dtype != x.dtype:
+            raise TypeError(f"dense: {name} is {t.dtype}, x {x.dtype}")
+    _checked("dense", x, others)
+    act = ACTIVATIONS[activation]
+    x2 = x.reshape(-1, kernel.shape[0]).contiguous()
+    kernel = kernel.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    r2 = None if residual is None else residual.reshape(-1, shape[-1]).contiguous()
+    if torch.is_grad_enabled() and (x2.requires_grad or kernel.requires_grad or
+                                    (bias is not None and bias.requires_grad) or
+                                    (r2 is not None and r2.requires_grad)):
+        y = _Dense.apply(x2, kernel, bias, r2, act)
+    else:
+        y, _ = _dense_forward(x2, kernel, bias, r2, act, False)
+    return y if x.dim() == 2 else y.view(shape)
+
+
+# ---------------------------------------------------------------- layer norm
+def _norm_forward(x, scale, bias, eps, keep):
+    M, D = x.shape
+    code = DTYPES[x.dtype]
+    p = scale if scale is not None else bias
+    pcode = code if p is None else DTYPES[p.dtype]
+    y = torch.empty_like(x)
+    mean = rstd = None
+    if keep:
+        mean, rstd = torch.empty((2, M), dtype=torch.float32, device=x.device)
+    _native(x.device, nat.lib().az_layer_norm_forward, code, pcode, M, D, nat.ptr(x), nat.ptr(scale), nat.ptr(bias),
+            eps, nat.ptr(y), nat.ptr(mean), nat.ptr(rstd))
+    return y, mean, rstd
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, scale, bias, eps):
+        y, mean, rstd = _norm_forward(x, scale, bias, eps, True)
+        ctx.save_for_backward(x, scale, mean, rstd)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, scale, mean, rstd = ctx.saved_tensors
+        M, D = x.shape
+        need = ctx.needs_input_grad
+        code = DTYPES[x.dtype]
+        ptype = scale.dtype if scale is not None else ctx.bias_dtype or x.dtype
+        dx = torch.empty_like(x) if need[0] else None
+        dscale = torch.empty((D,), dtype=ptype, device=x.device) if need[1] else None
+        dbias = torch.empty((D,), dtype=ptype, device=x.device) if need[2] else None
+        g = dy.contiguous()
+        lib = nat.lib()
+        n = lib.az_layer_norm_workspace_bytes(M, D) if need[1] or need[2] else 0
+        ws = torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
+        _native(x.device, lib.az_layer_norm_backward, code, DTYPES[ptype], M, D, nat.ptr(x), nat.ptr(scale),
+                nat.ptr(mean), nat.ptr(rstd), nat.ptr(g), nat.ptr(dx), nat.ptr(dscale), nat.ptr(dbias), nat.ptr(ws),
+                n)
+        return dx, dscale, dbias, None
+
+
+def layer_norm(x, scale=None, bias=None, eps=1e-6):
+    """(x - mean) / sqrt(variance + eps) * scale + bias over the last axis, differentiable in every tensor.
+
+    x [..., width] in float32, bfloat16 or float16; scale and bias [width], both of x's type or
+    both float32; strided tensors are copied first.
+    """
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"layer_norm: x {tuple(x.shape)} has no last axis to normalise")
+    D = x.shape[-1]
+    ptype = None
+    for name, t in (("scale", scale), ("bias", bias)):
+        if t is None:
+            continue
+        if tuple(t.shape) != (D,):
+            raise ValueError(f"layer_norm: {name} {tuple(t.shape)} does not match x {tuple(x.shape)}")
+        if t.dtype not in (x.dtype, torch.float32) or (ptype is not None and t.dtype != ptype):
+            raise TypeError(f"layer_norm: scale and bias must share a type, x's ({x.dtype}) or float32")
+        ptype = t.dtype
+    eps = float(eps)
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"layer_norm: eps {eps}")
+    _checked("layer_norm", x, (("scale", scale), ("bias", bias)))
+    x2 = x.reshape(-1, D).contiguous()
+    scale = None if scale is None else scale.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    if torch.is_grad_enabled() and (x2.requires_grad or (scale is not None and scale.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
+        y = _LayerNorm.apply(x2, scale, bias, eps)
+    else:
+        y = _norm_forward(x2, scale, bias, eps, False)[0]
+    return y if x.dim() == 2 else y.view(x.shape)

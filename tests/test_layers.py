@@ -1,0 +1,133 @@
+"""CPU tests of the layer operators: the C ABI of include/az_layers.h, the refusals of every entry point (none
+of which reaches a GPU)."""
+import ctypes as C
+import os
+import re
+
+import pytest
+import torch
+
+import alphazero_amd as mctx
+from alphazero_amd import _native as nat
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def test_library_exports_every_declared_layer_symbol():
+    header = open(os.path.join(ROOT, "include", "az_layers.h")).read()
+    header = re.sub(r"/\*.*?\*/", "", header, flags=re.S)
+    declared = set(re.findall(r"\b(az_[a-z_0-9]+)\s*\(", header))
+    assert declared == set(nat.LAYER_SIGNATURES), declared ^ set(nat.LAYER_SIGNATURES)
+    for name in declared:
+        assert hasattr(nat.lib(), name)
+    assert C.sizeof(nat.SampleDesc) == 4 * 4 + 3 * 8 + 7 * 8
+
+
+F, H = torch.float32, torch.float16
+
+
+def t(*shape, dtype=F):
+    return torch.zeros(shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("error,args,kw", [
+    (ValueError, (t(3, 4), t(5, 2)), {}),                                   # fan_in
+    (ValueError, (t(3, 4), t(4)), {}),
+    (ValueError, (t(3, 0), t(0, 2)), {}),
+    (ValueError, (t(3, 4), t(4, 0)), {}),
+    (ValueError, (t(3, 4), t(4, 2)), dict(bias=t(3))),
+    (ValueError, (t(3, 4), t(4, 2)), dict(bias=t(1, 2))),
+    (ValueError, (t(3, 4), t(4, 2)), dict(residual=t(1, 2))),               # no broadcasting
+    (ValueError, (t(3, 4), t(4, 2)), dict(residual=t(3, 4))),
+    (ValueError, (t(3, 4), t(4, 2)), dict(activation="tanh")),
+    (TypeError, (t(3, 4), t(4, 2, dtype=H)), {}),
+    (TypeError, (t(3, 4), t(4, 2)), dict(bias=t(2, dtype=H))),
+    (TypeError, (t(3, 4), t(4, 2)), dict(residual=t(3, 2, dtype=H))),
+    (TypeError, (t(3, 4, dtype=torch.float64), t(4, 2, dtype=torch.float64)), {}),
+    (ValueError, (t(3, 4), t(4, 2).to("meta")), {}),                        # another device
+    (NotImplementedError, (t(3, 4), t(4, 2)), {}),                          # no CPU path
+])
+def test_dense_refusals(error, args, kw):
+    with pytest.raises(error):
+        mctx.dense(*args, **kw)
+
+
+@pytest.mark.parametrize("error,args,kw", [
+    (ValueError, (t(3, 0),), {}),
+    (ValueError, (torch.tensor(1.0),), {}),
+    (ValueError, (t(3, 4), t(3)), {}),
+    (ValueError, (t(3, 4),), dict(bias=t(1, 4))),
+    (ValueError, (t(3, 4),), dict(eps=-1.0)),
+    (ValueError, (t(3, 4),), dict(eps=float("nan"))),
+    (TypeError, (t(3, 4), t(4, dtype=H)), {}),
+    (TypeError, (t(3, 4, dtype=H), t(4, dtype=H), t(4)), {}),               # scale and bias of two types
+    (TypeError, (t(3, 4, dtype=torch.int32),), {}),
+    (NotImplementedError, (t(3, 4),), {}),
+])
+def test_layer_norm_refusals(error, args, kw):
+    with pytest.raises(error):
+        mctx.layer_norm(*args, **kw)
+
+
+@pytest.mark.parametrize("error,args,kw", [
+    (ValueError, (t(4), t(4)), {}),
+    (ValueError, (t(4, 0), t(4)), {}),
+    (ValueError, (t(4, 3), t(3)), {}),
+    (ValueError, (t(4, 3), t(4, dtype=H)), {}),
+    (TypeError, (t(4, 3, dtype=torch.float64), t(4)), {}),
+    (ValueError, (t(4, 3), t(4)), dict(invalid_actions=t(3))),
+    (ValueError, (t(4, 3), t(4)), dict(temperature=-1.0)),
+    (ValueError, (t(4, 3), t(4)), dict(temperature=float("nan"))),
+    (ValueError, (t(4, 3), t(4)), dict(temperature=float("inf"))),
+    (ValueError, (t(4, 3), t(4)), dict(temperature=t(3))),
+    (ValueError, (t(4, 3), t(4)), dict(top_k=-1)),
+    (ValueError, (t(4, 3), t(4)), dict(top_k=1.5)),
+    (ValueError, (t(4, 3), t(4)), dict(top_p=1.5)),
+    (ValueError, (t(4, 3), t(4)), dict(min_p=-0.1)),
+    (ValueError, (t(4, 3), t(4)), dict(min_p=t(4, 1))),
+    (ValueError, (t(4, 3), t(4)), dict(top_p=t(4).to("meta"))),
+    (NotImplementedError, (t(4, 3), t(4)), {}),
+])
+def test_sample_actions_refusals(error, args, kw):
+    with pytest.raises(error):
+        mctx.sample_actions(*args, **kw)
+
+
+def test_native_refusals():
+    """The C entry points refuse before they launch (all pointers here are null or never read)."""
+    lib = nat.lib()
+    some = C.c_void_p(4096)
+    assert lib.az_dense_workspace_bytes(3, 4, 4, 4, 0) == -1
+    assert lib.az_dense_workspace_bytes(0, -1, 4, 4, 0) == -1
+    assert lib.az_dense_workspace_bytes(0, 4, 0, 4, 0) == -1
+    assert lib.az_dense_workspace_bytes(0, 4, 4, 2 ** 20 + 1, 0) == -1
+    assert lib.az_dense_workspace_bytes(0, 2 ** 31 - 1, 4, 4, 0) == -1
+    assert lib.az_dense_workspace_bytes(0, 4, 4, 4, 2) == -1
+    assert lib.az_dense_workspace_bytes(0, 0, 4, 4, 1) == 0
+    dense = lib.az_dense_forward
+    assert dense(0, 9, 4, 4, 4, some, some, None, None, some, None, some, 1 << 30, None) == -1
+    assert dense(0, 0, 4, 4, 4, None, some, None, None, some, None, some, 1 << 30, None) == -1
+    assert dense(0, 0, 0, 4, 4, None, None, None, None, None, None, None, 0, None) == 0      # no rows
+    n = lib.az_dense_workspace_bytes(0, 1, 4096, 64, 0)
+    assert n > 0
+    assert dense(0, 0, 1, 4096, 64, some, some, None, None, some, None, some, n - 1, None) == -1
+    assert dense(0, 0, 1, 4096, 64, some, some, None, None, some, None, None, n, None) == -1
+    assert dense(0, 0, 1, 4096, 64, some, some, None, None, some, None, C.c_void_p(4100), n, None) == -1
+    back = lib.az_dense_backward
+    assert back(0, 1, 4, 4, 4, some, some, None, some, some, some, some, some, 1 << 30, None) == -1   # z is missing
+    assert back(0, 0, 4, 4, 4, None, some, None, some, some, some, some, some, 1 << 30, None) == -1
+    assert back(0, 0, 4, 4, 4, some, some, None, some, None, None, None, None, 0, None) == 0          # nothing asked
+    assert lib.az_layer_norm_workspace_bytes(4, 0) == -1
+    norm = lib.az_layer_norm_forward
+    assert norm(0, 1, 4, 4, some, some, some, 1e-6, some, None, None, None) == -1            # parameter type
+    assert norm(0, 0, 4, 4, some, some, some, 1e-6, some, some, None, None) == -1            # mean without rstd
+    assert norm(0, 0, 4, 2 ** 20 + 1, some, some, some, 1e-6, some, None, None, None) == -2
+    assert lib.az_layer_norm_backward(0, 0, 4, 4, some, some, some, some, some, some, some, some, None, 0, None) == -1
+    d = nat.SampleDesc(dtype=0, rows=4, actions=0)
+    assert lib.az_sample_actions(C.byref(d), some, some, None) == -1
+    d.actions = 2 ** 20 + 1
+    assert lib.az_sample_actions(C.byref(d), some, some, None) == -2
+    d.actions = 4
+    assert lib.az_sample_actions(C.byref(d), some, some, None) == -1
+    d.rows = 0
+    assert lib.az_sample_actions(C.byref(d), None, None, None) == 0
