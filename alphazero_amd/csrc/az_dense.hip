@@ -9,139 +9,13 @@
 // so a kernel takes, for each operand, whether its reduction axis is the contiguous one.
 #include <hip/hip_runtime.h>
 
-#include "az_host.h"
-#include "az_types.h"
+#include <type_traits>
+
+#include "az_dense.h"
+
+using namespace az_dense;
 
 namespace {
-
-// ---------------------------------------------------------------------------
-// activations, in float32
-__device__ __forceinline__ float act_value(float z, int act) {
-  if (act == AZ_ACT_RELU) return z != z ? z : fmaxf(z, 0.0f);
-  if (act == AZ_ACT_SWISH) return z / (1.0f + expf(-z));
-  if (act == AZ_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
-  return z;
-}
-
-__device__ __forceinline__ float act_slope(float z, int act) {
-  if (act == AZ_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-  if (act == AZ_ACT_SWISH) {
-    const float p = 1.0f / (1.0f + expf(-z));
-    return p * (1.0f + z * (1.0f - p));
-  }
-  if (act == AZ_ACT_GELU)
-    return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * (0.39894228f * expf(-0.5f * z * z));
-  return 1.0f;
-}
-
-// The kept pre-activation.  A 16-bit layer keeps it as float16 for both 16-bit types: it is read only for the
-// slope, whose relative error from this rounding is at most 2^-11 |z act''(z) / act'(z)|, an eighth of what
-// bfloat16 would give, and the slope does not change beyond +-65504, where a finite z is clamped.  A positive z
-// too small for float16 stays positive (the slope of relu).
-template <typename T>
-struct Kept {
-  typedef az_f16 type;
-};
-template <>
-struct Kept<float> {
-  typedef float type;
-};
-__device__ __forceinline__ void keep(float* p, float z) { *p = z; }
-__device__ __forceinline__ void keep(az_f16* p, float z) {
-  if (fabsf(z) < INFINITY) z = fminf(fmaxf(z, -65504.0f), 65504.0f);
-  if (z > 0.0f) z = fmaxf(z, 5.9604645e-8f);
-  *p = (az_f16)z;
-}
-
-// ---------------------------------------------------------------------------
-enum { EPI_FORWARD, EPI_STORE, EPI_PARTIAL };
-
-struct Prod {
-  const void* a;
-  const void* b;
-  int64_t lda, ldb;
-  int M, N, K;
-  int k_chunk;          // reduction length of one split (blockIdx.z)
-  int a_vec, b_vec;     // 16-byte loads are aligned
-  int tiles_m, tiles_n;
-  // epilogue
-  int act, out_vec;     // out_vec: rows of the outputs can be read and written four elements at a time
-  const void* bias;
-  const void* residual;
-  void* z;
-  void* out;
-  float* partial;       // [splits][M][N]
-};
-
-// Four consecutive outputs of row m from column n.
-template <typename T, int EPI>
-__device__ __forceinline__ void finish(const Prod& p, int m, int n, const float* v) {
-  if (m >= p.M || n >= p.N) return;
-  const int64_t at = (int64_t)m * p.N + n;
-  const int have = p.N - n < 4 ? p.N - n : 4;
-  if constexpr (EPI == EPI_PARTIAL) {
-    float* out = p.partial + (int64_t)blockIdx.z * p.M * p.N + at;
-    if (p.out_vec) {
-      *reinterpret_cast<float4*>(out) = float4{v[0], v[1], v[2], v[3]};
-    } else {
-      for (int i = 0; i < have; ++i) out[i] = v[i];
-    }
-  } else {
-    T* out = (T*)p.out + at;
-    if constexpr (EPI == EPI_STORE) {
-      if (p.out_vec) {
-        AzVec<T, 4> o;
-        for (int i = 0; i < 4; ++i) o.v[i] = (T)v[i];
-        az_storev<T, 4>(out, o);
-      } else {
-        for (int i = 0; i < have; ++i) out[i] = (T)v[i];
-      }
-    } else {
-      typedef typename Kept<T>::type Z;
-      const T* bias = (const T*)p.bias;
-      const T* res = p.residual ? (const T*)p.residual + at : nullptr;
-      Z* z = p.z ? (Z*)p.z + at : nullptr;
-      if (p.out_vec) {
-        AzVec<T, 4> o, r, b;
-        AzVec<Z, 4> zz;
-        if (bias) b = az_loadv<T, 4>(bias + n);
-        if (res) r = az_loadv<T, 4>(res);
-        for (int i = 0; i < 4; ++i) {
-          const float s = v[i] + (bias ? (float)b.v[i] : 0.0f);
-          keep(&zz.v[i], s);
-          o.v[i] = (T)(act_value(s, p.act) + (res ? (float)r.v[i] : 0.0f));
-        }
-        if (z) az_storev<Z, 4>(z, zz);
-        az_storev<T, 4>(out, o);
-      } else {
-        for (int i = 0; i < have; ++i) {
-          const float s = v[i] + (bias ? (float)bias[n + i] : 0.0f);
-          if (z) keep(z + i, s);
-          out[i] = (T)(act_value(s, p.act) + (res ? (float)res[i] : 0.0f));
-        }
-      }
-    }
-  }
-}
-
-// ---------------------------------------------------------------------------
-// The matrix instructions on 64 bytes of reduction: 16 float32 values (four 16x16x4 steps) or 32 of 16 bits
-// (one 16x16x32 step).  Lane l gives 16 bytes of row l % 16, those at (l / 16) * 16; which reduction
-// index a lane's j-th element stands for is the same for both operands, so any order does.
-__device__ __forceinline__ az_f32x4 mma(const AzPack<float>& a, const AzPack<float>& b, az_f32x4 c) {
-  for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], c, 0, 0, 0);
-  return c;
-}
-typedef az_bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef az_f16 f16x8 __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ az_f32x4 mma(const AzPack<az_bf16>& a, const AzPack<az_bf16>& b, az_f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
-                                                 0, 0);
-}
-__device__ __forceinline__ az_f32x4 mma(const AzPack<az_f16>& a, const AzPack<az_f16>& b, az_f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
-                                                0);
-}
 
 // ---------------------------------------------------------------------------
 // Any sizes and alignments: 64 x 64 outputs a workgroup, four waves of 32 x 32, 64 bytes of reduction a step.
@@ -273,14 +147,27 @@ __global__ __launch_bounds__(256) void k_join(Join q, Prod p) {
 }
 
 // ---------------------------------------------------------------------------
+// The three bfloat16 planes of a float32 value: each the rounding of what is left.  (A value that is not finite has
+// no such planes; the wide kernel works its outputs out again.)
+__device__ __forceinline__ void planes_of(float x, az_bf16* p) {
+  p[0] = (az_bf16)x;
+  x -= (float)p[0];
+  p[1] = (az_bf16)x;
+  x -= (float)p[1];
+  p[2] = (az_bf16)x;
+}
+
 // dz = dy act'(z), rounded to T, and the partial column sums of dz before the rounding: a workgroup takes 64 V
 // columns (V a thread) of a chunk of rows, four rows at a time.
 struct Slope {
   const void* dy;
   const void* z;
   void* dz;            // may be null (no activation: dy itself is dz)
+  az_bf16* planes;     // float32 only: dz as planes, may be null
+  int64_t plane;
   float* partial;      // [chunks][N], may be null
   int M, N, act, rows_per_chunk;
+  int ld;              // of dz and the planes: columns N .. ld are set to zero
 };
 
 template <typename T, int V>
@@ -291,19 +178,35 @@ __global__ __launch_bounds__(256) void k_slope(Slope p) {
   const int n = (blockIdx.x * 64 + g) * V;
   const int m_end = min(p.M, (int)(blockIdx.y + 1) * p.rows_per_chunk);
   float s[V] = {};
-  if (n < p.N) {
+  if (n < p.N || ((p.dz || p.planes) && n < p.ld)) {
     for (int m = blockIdx.y * p.rows_per_chunk + w; m < m_end; m += 4) {
-      const int64_t at = (int64_t)m * p.N + n;
-      const AzVec<T, V> dy = az_loadv<T, V>((const T*)p.dy + at);
-      AzVec<Z, V> z;
-      if (p.act != AZ_ACT_NONE) z = az_loadv<Z, V>((const Z*)p.z + at);
-      AzVec<T, V> o;
-      for (int i = 0; i < V; ++i) {
-        const float d = p.act == AZ_ACT_NONE ? (float)dy.v[i] : (float)dy.v[i] * act_slope((float)z.v[i], p.act);
-        s[i] += d;
-        o.v[i] = (T)d;
+      const int64_t at = (int64_t)m * p.N + n, to = (int64_t)m * p.ld + n;
+      float d[V] = {};
+      if (n < p.N) {
+        const AzVec<T, V> dy = az_loadv<T, V>((const T*)p.dy + at);
+        AzVec<Z, V> z;
+        if (p.act != AZ_ACT_NONE) z = az_loadv<Z, V>((const Z*)p.z + at);
+        for (int i = 0; i < V; ++i) {
+          d[i] = p.act == AZ_ACT_NONE ? (float)dy.v[i] : (float)dy.v[i] * act_slope((float)z.v[i], p.act);
+          s[i] += d[i];
+        }
       }
-      if (p.dz) az_storev<T, V>((T*)p.dz + at, o);
+      if (p.dz) {
+        AzVec<T, V> o;
+        for (int i = 0; i < V; ++i) o.v[i] = (T)d[i];
+        az_storev<T, V>((T*)p.dz + to, o);
+      }
+      if constexpr (sizeof(T) == 4) {
+        if (p.planes) {
+          AzVec<az_bf16, V> o[3];
+          for (int i = 0; i < V; ++i) {
+            az_bf16 q[3];
+            planes_of(d[i], q);
+            for (int k = 0; k < 3; ++k) o[k].v[i] = q[k];
+          }
+          for (int k = 0; k < 3; ++k) az_storev<az_bf16, V>(p.planes + k * p.plane + to, o[k]);
+        }
+      }
     }
   }
   if (!p.partial) return;
@@ -313,6 +216,35 @@ __global__ __launch_bounds__(256) void k_slope(Slope p) {
   if (w > 0 || n >= p.N) return;
   for (int i = 0; i < V; ++i)
     p.partial[(int64_t)blockIdx.y * p.N + n + i] = ((s[i] + sums[0][g][i]) + sums[1][g][i]) + sums[2][g][i];
+}
+
+// Copies an operand for the wide kernel: rows of `ld` elements, the last ones zero; float32 as planes.
+template <typename T>
+__global__ __launch_bounds__(256) void k_pack(const T* src, int rows, int cols, int ld, void* dst, int64_t plane) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per = ld / 8;
+  if (i >= (int64_t)rows * per) return;
+  const int64_t m = i / per;
+  const int n = (int)(i % per) * 8;
+  const T* from = src + m * cols + n;
+  AzVec<T, 8> x;
+  if (n + 8 <= cols) {
+    x = az_loadu<T, 8>(from);
+  } else {
+    for (int e = 0; e < 8; ++e) x.v[e] = n + e < cols ? from[e] : (T)0.0f;
+  }
+  const int64_t to = m * ld + n;
+  if constexpr (sizeof(T) == 4) {
+    AzVec<az_bf16, 8> o[3];
+    for (int e = 0; e < 8; ++e) {
+      az_bf16 q[3];
+      planes_of(x.v[e], q);
+      for (int k = 0; k < 3; ++k) o[k].v[e] = q[k];
+    }
+    for (int k = 0; k < 3; ++k) az_storev<az_bf16, 8>((az_bf16*)dst + k * plane + to, o[k]);
+  } else {
+    az_storev<T, 8>((T*)dst + to, x);
+  }
 }
 
 template <typename T>
@@ -341,18 +273,28 @@ int slope_chunks(int64_t rows, int64_t col_tiles) {
   return (int)(c < most ? c : most);
 }
 
+int64_t round64(int64_t n) { return (n + 63) & ~(int64_t)63; }
+
+// How one product C[M, N] over K runs.
 struct Plan {
-  int splits_y, splits_dx, splits_dw, chunks;
-  int64_t partial_floats;   // of the largest product's splits
+  bool wide, big;
+  int splits;
 };
 
-Plan plan_of(int64_t M, int64_t K, int64_t N) {
-  auto tiles = [](int64_t a, int64_t b) { return az_ceil(a, TILE) * az_ceil(b, TILE); };
-  Plan p;
-  p.splits_y = splits_of(tiles(M, N), K);
-  p.splits_dx = splits_of(tiles(M, K), N);
-  p.splits_dw = splits_of(tiles(K, N), M);
-  p.chunks = slope_chunks(M, az_ceil(N, 64 * (N % 4 == 0 ? 4 : 1)));
+Plan plan_of(int dtype, int64_t M, int64_t N, int64_t K) {
+  Plan p = {};
+  const double work = (double)M * N * K;
+  p.wide = work >= (dtype == AZ_TYPE_F32 ? 0x1p31 : 0x1p27) && M >= 128 && N >= 64 && K >= 128;
+  if (!p.wide) {
+    p.splits = splits_of(az_ceil(M, TILE) * az_ceil(N, TILE), K);
+    return p;
+  }
+  const int64_t large = az_ceil(M, 256) * az_ceil(N, 256), small = az_ceil(M, 128) * az_ceil(N, 128);
+  p.big = large >= 128 || (large >= 16 && K >= 256 * 64 / large);
+  const int64_t tiles = p.big ? large : small, want = p.big ? 256 : 512, most = az_ceil(K, 512);
+  int64_t s = tiles >= want / 2 ? 1 : want / tiles;
+  if (s > most) s = most;
+  p.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
   return p;
 }
 
@@ -368,29 +310,33 @@ int check(int dtype, int act, int64_t rows, int64_t fan_in, int64_t fan_out) {
   return AZ_OK;
 }
 
-// One product (and, with `bias_part`, the join of the bias' gradient).  `partial` holds splits x M x N floats.
+// One product (and, with `extra`, the join of the bias' gradient).  `partial` holds splits x M x N floats.
 template <typename T, bool AKC, bool BKC, int EPI>
-int product(Prod p, int splits, float* partial, const Join* extra, hipStream_t stream) {
+int product(Prod p, const Plan& plan, float* partial, const Join* extra, hipStream_t stream) {
   const int E = AzPack<T>::N;
+  const int pass = EPI == EPI_FORWARD ? PASS_Y : AKC ? PASS_DX : PASS_DW;
+  const int dtype = sizeof(T) == 4 ? AZ_TYPE_F32 : std::is_same_v<T, az_bf16> ? AZ_TYPE_BF16 : AZ_TYPE_F16;
   p.a_vec = p.lda % E == 0 && az_aligned16(p.a);
   p.b_vec = p.ldb % E == 0 && az_aligned16(p.b);
   auto four = [](const void* q) { return ((uintptr_t)q & (4 * sizeof(T) - 1)) == 0; };
   p.out_vec = p.N % 4 == 0 && four(p.out) && four(p.bias) && four(p.residual) && az_aligned16(p.z);
-  p.tiles_m = (int)az_ceil(p.M, TILE), p.tiles_n = (int)az_ceil(p.N, TILE);
+  const int tile = !plan.wide ? TILE : plan.big ? 256 : 128;
+  p.tiles_m = (int)az_ceil(p.M, tile), p.tiles_n = (int)az_ceil(p.N, tile);
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
   if (tiles > 0x7fffffff) return az_fail(AZ_ERR_UNSUPPORTED, "dense: too many output tiles");
-  const int BK = Stage<T, true>::BK;
-  p.k_chunk = (int)(az_ceil(az_ceil(p.K, splits), BK) * BK);
-  splits = (int)az_ceil(p.K, p.k_chunk);
-  const dim3 grid((unsigned)tiles, 1, splits), block(256);
-  if (splits == 1) {
-    k_product_tile<T, AKC, BKC, EPI><<<grid, block, 0, stream>>>(p);
-    AZ_LAUNCH_CHECK();
+  const int step = plan.wide ? 64 : Stage<T, true>::BK;
+  p.k_chunk = (int)(az_ceil(az_ceil(p.K, plan.splits), step) * step);
+  const int splits = (int)az_ceil(p.K, p.k_chunk);
+  Prod q = p;
+  if (splits > 1) q.partial = partial, q.out_vec = p.N % 4 == 0;
+  if (plan.wide) {
+    if (int rc = az_product_wide(dtype, pass, splits > 1, plan.big, &q, splits, stream)) return rc;
   } else {
-    Prod q = p;
-    q.partial = partial;
-    q.out_vec = p.N % 4 == 0;
-    k_product_tile<T, AKC, BKC, EPI_PARTIAL><<<grid, block, 0, stream>>>(q);
+    const dim3 grid((unsigned)tiles, 1, splits), block(256);
+    if (splits == 1)
+      k_product_tile<T, AKC, BKC, EPI><<<grid, block, 0, stream>>>(q);
+    else
+      k_product_tile<T, AKC, BKC, EPI_PARTIAL><<<grid, block, 0, stream>>>(q);
     AZ_LAUNCH_CHECK();
   }
   if (splits > 1 || extra) {
@@ -406,23 +352,69 @@ int product(Prod p, int splits, float* partial, const Join* extra, hipStream_t s
   return AZ_OK;
 }
 
-// Workspace layout of a backward pass: [dz][bias partials][split sums]
+// A pass' plans and its workspace: copies of the operands for the wide kernel where it cannot read them in place
+// (always room for them), dz, the partial sums of the bias' gradient, the partial sums of a split product.
 struct Layout {
-  int64_t dz, bias, partial, total;
+  Plan y, dx, dw;
+  int chunks;
+  int64_t x, kernel, dz, dz_planes, bias, partial, total;
 };
 
 Layout layout_of(int dtype, int64_t M, int64_t K, int64_t N, int pass) {
-  const Plan p = plan_of(M, K, N);
-  Layout l = {0, 0, 0, 0};
+  Layout l = {};
+  const int64_t Kp = round64(K), Np = round64(N), each = dtype == AZ_TYPE_F32 ? 6 : 2;
+  int64_t at = 0;
+  auto room = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += (bytes + 255) & ~(int64_t)255;
+    return here;
+  };
   if (pass == 0) {
-    l.total = p.splits_y > 1 ? p.splits_y * M * N * 4 : 0;
-    return l;
+    l.y = plan_of(dtype, M, N, K);
+    if (l.y.wide) l.x = room(M * Kp * each), l.kernel = room(K * Np * each);
+    if (l.y.splits > 1) l.partial = room(l.y.splits * M * N * 4);
+  } else {
+    l.dx = plan_of(dtype, M, K, N), l.dw = plan_of(dtype, K, N, M);
+    l.chunks = slope_chunks(M, az_ceil(N, 64 * (N % 4 == 0 ? 4 : 1)));
+    l.dz = room(M * Np * size_of(dtype));
+    if (dtype == AZ_TYPE_F32 && (l.dx.wide || l.dw.wide)) l.dz_planes = room(M * Np * 6);
+    l.bias = room((int64_t)l.chunks * N * 4);
+    if (l.dw.wide) l.x = room(M * Kp * each);
+    if (l.dx.wide) l.kernel = room(K * Np * each);
+    const int64_t a = l.dx.splits > 1 ? l.dx.splits * M * K : 0, b = l.dw.splits > 1 ? l.dw.splits * K * N : 0;
+    l.partial = room(4 * (a > b ? a : b));
   }
-  l.bias = round16(M * N * size_of(dtype));
-  l.partial = l.bias + round16((int64_t)p.chunks * N * 4);
-  const int64_t dx = p.splits_dx > 1 ? p.splits_dx * M * K : 0, dw = p.splits_dw > 1 ? p.splits_dw * K * N : 0;
-  l.total = l.partial + 4 * (dx > dw ? dx : dw);
+  l.total = at;
   return l;
+}
+
+// An operand [rows, cols] as the wide kernel reads it: in place, or copied to `to` (float32 always: planes).
+// along: its rows are the reduction's axis and have to be whole steps long.
+struct Source {
+  const void* p;
+  int64_t ld, plane;
+};
+
+template <typename T>
+int source(const void* src, int64_t rows, int64_t cols, bool along, void* to, hipStream_t stream, Source* out) {
+  if (sizeof(T) == 2 && az_aligned16(src) && cols % (along ? 64 : 8) == 0) {
+    *out = {src, cols, 0};
+    return AZ_OK;
+  }
+  const int64_t ld = round64(cols), threads = rows * (ld / 8);
+  if (az_ceil(threads, 256) > 0x7fffffff) return az_fail(AZ_ERR_UNSUPPORTED, "dense: operand too large");
+  *out = {to, ld, rows * ld};
+  k_pack<T><<<dim3((unsigned)az_ceil(threads, 256)), dim3(256), 0, stream>>>((const T*)src, (int)rows, (int)cols,
+                                                                             (int)ld, to, rows * ld);
+  AZ_LAUNCH_CHECK();
+  return AZ_OK;
+}
+
+void operand_a(Prod& p, const Source& s, const void* raw, int64_t ld) {
+  p.a = s.p, p.lda = s.ld, p.a_plane = s.plane, p.a32 = (const float*)raw, p.lda32 = ld;
+}
+void operand_b(Prod& p, const Source& s, const void* raw, int64_t ld) {
+  p.b = s.p, p.ldb = s.ld, p.b_plane = s.plane, p.b32 = (const float*)raw, p.ldb32 = ld;
 }
 
 }  // namespace
@@ -435,20 +427,27 @@ extern "C" int64_t az_dense_workspace_bytes(int32_t dtype, int32_t rows, int32_t
 
 extern "C" int az_dense_forward(int32_t dtype, int32_t act, int32_t rows, int32_t fan_in, int32_t fan_out,
                                 const void* x, const void* kernel, const void* bias, const void* residual, void* y,
-                                void* z, void* workspace, int64_t workspace_bytes, void* stream) {
+                                void* z, void* workspace, int64_t workspace_bytes, void* stream_) {
   if (int rc = check(dtype, act, rows, fan_in, fan_out)) return rc;
   if (rows == 0) return AZ_OK;
   if (!x || !kernel || !y) return az_fail(AZ_ERR_INVALID, "dense: null x, kernel or y");
   const Layout l = layout_of(dtype, rows, fan_in, fan_out, 0);
   if (workspace_bytes < l.total || (l.total && (!workspace || !az_aligned16(workspace))))
     return az_fail(AZ_ERR_INVALID, "dense: the workspace must hold %lld bytes, 16-byte aligned", (long long)l.total);
-  return az_dispatch_type(dtype, [&]<typename T>() {
+  hipStream_t stream = (hipStream_t)stream_;
+  char* ws = (char*)workspace;
+  return az_dispatch_type(dtype, [&]<typename T>() -> int {
     Prod p = {};
-    p.a = x, p.lda = fan_in, p.b = kernel, p.ldb = fan_out;
+    Source sx = {x, fan_in, 0}, sk = {kernel, fan_out, 0};
+    if (l.y.wide) {
+      if (int rc = source<T>(x, rows, fan_in, true, ws + l.x, stream, &sx)) return rc;
+      if (int rc = source<T>(kernel, fan_in, fan_out, false, ws + l.kernel, stream, &sk)) return rc;
+    }
+    operand_a(p, sx, x, fan_in);
+    operand_b(p, sk, kernel, fan_out);
     p.M = rows, p.N = fan_out, p.K = fan_in;
     p.act = act, p.bias = bias, p.residual = residual, p.z = act == AZ_ACT_NONE ? nullptr : z, p.out = y;
-    const Plan plan = plan_of(rows, fan_in, fan_out);
-    return product<T, true, false, EPI_FORWARD>(p, plan.splits_y, (float*)workspace, nullptr, (hipStream_t)stream);
+    return product<T, true, false, EPI_FORWARD>(p, l.y, (float*)(ws + l.partial), nullptr, stream);
   });
 }
 
@@ -474,38 +473,56 @@ extern "C" int az_dense_backward(int32_t dtype, int32_t act, int32_t rows, int32
       return az_fail(AZ_ERR_INVALID, "dense: the workspace must hold %lld bytes, 16-byte aligned",
                      (long long)l.total);
     char* ws = (char*)workspace;
-    const Plan plan = plan_of(rows, fan_in, fan_out);
-    const void* dz = dy;
-    if (act != AZ_ACT_NONE || dbias) {
+    const bool wide_dx = dx && l.dx.wide, wide_dw = dkernel && l.dw.wide, wide = wide_dx || wide_dw;
+    // dz: dy itself, or written by k_slope (padded for the wide kernel: it reduces along dz's rows for dx), for
+    // float32 also or only as planes
+    const int64_t ld = wide ? round64(fan_out) : fan_out;
+    constexpr bool F32 = sizeof(T) == 4;
+    const bool copy = act != AZ_ACT_NONE ||
+                      (wide && !F32 && (!az_aligned16(dy) || fan_out % 8 || (wide_dx && fan_out % 64)));
+    Source sdz = {dy, fan_out, 0}, sdzw = sdz;
+    if (copy) sdz = sdzw = {ws + l.dz, ld, 0};
+    if (F32 && wide) sdzw = {ws + l.dz_planes, ld, rows * ld};
+    if (copy || dbias || (F32 && wide)) {
       Slope s = {};
-      s.dy = dy, s.z = z, s.dz = act != AZ_ACT_NONE ? ws + l.dz : nullptr;
+      s.dy = dy, s.z = z, s.dz = copy ? ws + l.dz : nullptr;
+      if (F32 && wide) s.planes = (az_bf16*)(ws + l.dz_planes), s.plane = rows * ld;
       s.partial = dbias ? (float*)(ws + l.bias) : nullptr;
-      s.M = rows, s.N = fan_out, s.act = act, s.rows_per_chunk = (int)az_ceil(rows, plan.chunks);
+      s.M = rows, s.N = fan_out, s.act = act, s.rows_per_chunk = (int)az_ceil(rows, l.chunks), s.ld = (int)ld;
       const bool vec = fan_out % 4 == 0 && ((uintptr_t)dy & (4 * sizeof(T) - 1)) == 0 && az_aligned16(z);
       const int V = vec ? 4 : 1;
-      const dim3 grid((unsigned)az_ceil(fan_out, 64 * V), plan.chunks), block(256);
+      const dim3 grid((unsigned)az_ceil(ld, 64 * V), l.chunks), block(256);
       if (vec)
         k_slope<T, 4><<<grid, block, 0, stream>>>(s);
       else
         k_slope<T, 1><<<grid, block, 0, stream>>>(s);
       AZ_LAUNCH_CHECK();
-      if (s.dz) dz = s.dz;
     }
+    // (the float32 operands of an output that the planes leave not finite)
+    const void* dz32 = copy ? ws + l.dz : dy;
+    const int64_t ld32 = copy ? ld : fan_out;
+    float* partial = (float*)(ws + l.partial);
     if (dx) {
       Prod p = {};
-      p.a = dz, p.lda = fan_out, p.b = kernel, p.ldb = fan_out;
+      Source sk = {kernel, fan_out, 0};
+      if (wide_dx)
+        if (int rc = source<T>(kernel, fan_in, fan_out, true, ws + l.kernel, stream, &sk)) return rc;
+      operand_a(p, wide_dx ? sdzw : sdz, dz32, ld32);
+      operand_b(p, sk, kernel, fan_out);
       p.M = rows, p.N = fan_in, p.K = fan_out, p.out = dx;
-      if (int rc = product<T, true, true, EPI_STORE>(p, plan.splits_dx, (float*)(ws + l.partial), nullptr, stream))
-        return rc;
+      if (int rc = product<T, true, true, EPI_STORE>(p, l.dx, partial, nullptr, stream)) return rc;
     }
     Join j = {};
-    j.part[1] = (const float*)(ws + l.bias), j.length[1] = fan_out, j.splits[1] = plan.chunks, j.out1 = dbias;
+    j.part[1] = (const float*)(ws + l.bias), j.length[1] = fan_out, j.splits[1] = l.chunks, j.out1 = dbias;
     if (dkernel) {
       Prod p = {};
-      p.a = x, p.lda = fan_in, p.b = dz, p.ldb = fan_out;
+      Source sx = {x, fan_in, 0};
+      if (wide_dw)
+        if (int rc = source<T>(x, rows, fan_in, false, ws + l.x, stream, &sx)) return rc;
+      operand_a(p, sx, x, fan_in);
+      operand_b(p, wide_dw ? sdzw : sdz, dz32, ld32);
       p.M = fan_in, p.N = fan_out, p.K = rows, p.out = dkernel;
-      return product<T, false, false, EPI_STORE>(p, plan.splits_dw, (float*)(ws + l.partial), dbias ? &j : nullptr,
-                                                 stream);
+      return product<T, false, false, EPI_STORE>(p, l.dw, partial, dbias ? &j : nullptr, stream);
     }
     if (dbias) {
       k_join<T, EPI_STORE><<<dim3((unsigned)az_ceil(fan_out, 256)), dim3(256), 0, stream>>>(j, Prod{});

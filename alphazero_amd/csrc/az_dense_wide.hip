@@ -1,0 +1,247 @@
+// az_dense_wide.hip -- the large products of a dense layer on the 16-bit matrix instructions.
+// Part of libaz_mcts.so (gfx950 only).
+//
+// A workgroup computes BM x BN outputs, 64 reduction steps at a time: the next step's operands go from global memory
+// straight into LDS (16 bytes a lane, no registers) while the waves multiply the current ones, two buffers in
+// turn.  An operand whose reduction axis is contiguous lies in LDS as rows of 128 bytes and is read 16 bytes a lane;
+// one whose other axis is contiguous lies as 64 rows of BM (BN) elements and is read by the transposing LDS read, which
+// hands lane i column i of a 4 x 16 block.  Both are swizzled in 16-byte chunks so that the lanes of
+// one read fall on all banks: a direct load puts lane l's bytes at l * 16, so the swizzle is in the global address that a
+// lane loads from.  The buffer descriptor ends where the matrix ends: what is loaded beyond it is zero, which
+// covers the ragged edges (rows beyond M or N are not stored; a reduction over rows that ends inside a step adds
+// zeros; a reduction along contiguous rows is a multiple of 64 here).
+//
+// float32 products run on the same instructions: an operand is split into three bfloat16 planes x = x0 + x1 + x2
+// (each the rounding of what the planes before it left, so the three hold all 24 bits), and of the nine products the
+// six that matter, x0 y0, x0 y1, x1 y0, x1 y1, x0 y2, x2 y0, are added in one float32 accumulator, the small ones
+// first.  What is left out is below 2^-26 of the terms' magnitudes.  Six bfloat16 products cost 6 / 16 of
+// the float32 instruction's time.  An infinity or an overflow turns into NaN on the way (inf - inf, inf * 0): an output
+// that is not finite is worked out again from the float32 operands, term by term.
+#include <hip/hip_runtime.h>
+
+#include "az_dense.h"
+
+using namespace az_dense;
+
+namespace {
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr int STEP = 64;   // reduction steps per stage
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// A buffer descriptor of the bytes from p to end: what is loaded from beyond is zero.
+__device__ __forceinline__ i32x4 descriptor(const char* p, const char* end) {
+  const int64_t left = end - p;
+  const uint32_t n = left <= 0 ? 0u : left > 0xffffffffll ? 0xffffffffu : (uint32_t)left;
+  const uint64_t at = (uint64_t)p;
+  i32x4 r;
+  r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)at);
+  r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32) & 0xffff);
+  r[2] = __builtin_amdgcn_readfirstlane((int)n);
+  r[3] = 0x00027000;
+  return r;
+}
+
+// Lane l's 16 bytes at `offset` behind the descriptor's start go to LDS byte `to` + 16 l.  In assembly, because for the
+// builtin the compiler waits for every load in flight in front of each LDS read; the kernel's own waits are in front
+// of its barriers.  (No register is written; the load reads M0 one instruction after it is set.)
+__device__ __forceinline__ void load_to_lds(i32x4 r, uint32_t offset, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(to), "v"(offset), "s"(r)
+               : "memory", "m0");
+}
+
+// chunk swizzle of reduction row k of an operand that is not reduction-contiguous: the eight 32-byte pieces that two
+// groups of 16 lanes read at once (rows k..k+3 and k+8..k+11) go to eight places
+__device__ __forceinline__ int row_swizzle(int k) { return 2 * ((k & 3) | ((k >> 1) & 4)); }
+
+// One operand's stage: R rows (or columns) of the output, NW waves that load it.
+template <bool KC, int R, int NW>
+struct Operand {
+  static constexpr int BYTES = R * STEP * 2, LOADS = BYTES / 1024 / NW;
+  uint32_t offset[LOADS];   // this lane's byte offset from the stage's first element
+  const char* base;
+  const char* end;
+  int64_t step;             // bytes from one stage to the next
+
+  __device__ void init(const void* p, int64_t ld, int rows, int K, int r0, int wave, int lane) {
+    for (int i = 0; i < LOADS; ++i) {
+      const int ins = wave * LOADS + i;
+      if constexpr (KC) {
+        offset[i] = (uint32_t)((ins * 8 + (lane >> 3)) * ld * 2) + (((lane & 7) ^ (lane >> 3)) * 16);
+      } else {
+        constexpr int LANES = R / 8;   // lanes (16-byte chunks) a reduction row
+        const int k = ins * (64 / LANES) + lane / LANES;
+        offset[i] = (uint32_t)(k * ld * 2) + (((lane % LANES) ^ row_swizzle(k)) * 16);
+      }
+    }
+    end = (const char*)p + (KC ? (int64_t)rows : (int64_t)K) * ld * 2;
+    base = (const char*)p + (KC ? r0 * ld : (int64_t)r0) * 2;
+    step = KC ? STEP * 2 : STEP * ld * 2;
+  }
+  // stage t (of the plane `plane` bytes further) into lds
+  __device__ __forceinline__ void load(int t, int64_t plane, uint32_t lds, int wave) const {
+    const i32x4 r = descriptor(base + plane + t * step, end + plane);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) load_to_lds(r, offset[i], lds + (wave * LOADS + i) * 1024);
+  }
+};
+
+// The 16 x 32 fragment of rows r0.. and reduction steps sub * 32.. of a stage.
+template <bool KC, int R>
+__device__ __forceinline__ uint4 fragment(const char* lds, int r0, int sub, int lane) {
+  if constexpr (KC) {
+    const int row = r0 + (lane & 15), chunk = sub * 4 + (lane >> 4);
+    return *reinterpret_cast<const uint4*>(lds + row * 128 + ((chunk ^ (row & 7)) * 16));
+  } else {
+    const int k = sub * 32 + (lane >> 4) * 8 + ((lane >> 2) & 3);
+    const int chunk = r0 / 8 + ((lane >> 1) & 1), byte = (lane & 1) * 8;
+    // rows k and k + 4 have the same swizzle
+    const char* p = lds + k * (R * 2) + ((chunk ^ row_swizzle(k)) * 16) + byte;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * (R * 2)));
+    uint4 r;
+    __builtin_memcpy(&r, &lo, 8);
+    __builtin_memcpy((char*)&r + 8, &hi, 8);
+    return r;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ az_f32x4 mma16(uint4 a, uint4 b, az_f32x4 c) {
+  return mma(__builtin_bit_cast(AzPack<T>, a), __builtin_bit_cast(AzPack<T>, b), c);
+}
+
+// Workgroups go to the eight dies in turn, each with an L2 of its own: a die takes a contiguous run of tiles, and
+// the run goes down columns of GROUP tiles, so that the operands of the tiles in flight on a die are few.
+__device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int* tm, int* tn) {
+  const int n = tiles_m * tiles_n, per = n / 8, rest = n % 8, die = id % 8;
+  const int at = die * per + min(die, rest) + id / 8;
+  constexpr int GROUP = 4;
+  const int group = at / (GROUP * tiles_n), first = group * GROUP, height = min(GROUP, tiles_m - first);
+  const int in = at - group * GROUP * tiles_n;
+  *tm = first + in % height;
+  *tn = in / height;
+}
+
+// T: type of the operands in memory and LDS; TO: of the outputs; SPLIT: T is bfloat16 planes of float32 operands.
+template <typename T, typename TO, int BM, int BN, int WM, int WN, bool AKC, bool BKC, int EPI, bool SPLIT>
+__global__ __launch_bounds__(WM* WN * 64, 2) void k_product_wide(Prod p) {
+  constexpr int NW = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
+  typedef Operand<AKC, BM, NW> OpA;
+  typedef Operand<BKC, BN, NW> OpB;
+  constexpr int STAGE = OpA::BYTES + OpB::BYTES;
+  __shared__ alignas(16) char lds[2 * STAGE];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_void*)lds;
+  int tm, tn;
+  tile_of(blockIdx.x, p.tiles_m, p.tiles_n, &tm, &tn);
+  const int m0 = tm * BM, n0 = tn * BN;
+  const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
+  OpA a;
+  OpB b;
+  a.init(p.a, p.lda, p.M, p.K, m0, wave, lane);
+  b.init(p.b, p.ldb, p.N, p.K, n0, wave, lane);
+  // stages of this split; float32 operands go through them once for each pair of planes
+  const int t0 = blockIdx.z * (p.k_chunk / STEP), t1 = min((p.K + STEP - 1) / STEP, t0 + p.k_chunk / STEP);
+  const int stages = (t1 - t0) * (SPLIT ? 6 : 1);
+  auto load = [&](int s, int buf) {
+    int t = t0 + s;
+    int64_t pa = 0, pb = 0;
+    if constexpr (SPLIT) {
+      const int pair = s / (t1 - t0);          // (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
+      t -= pair * (t1 - t0);
+      pa = ((0x011020 >> (20 - 4 * pair)) & 15) * p.a_plane * 2;
+      pb = ((0x101002 >> (20 - 4 * pair)) & 15) * p.b_plane * 2;
+    }
+    a.load(t, pa, lds_at + buf * STAGE, wave);
+    b.load(t, pb, lds_at + buf * STAGE + OpA::BYTES, wave);
+  };
+  az_f32x4 acc[FM][FN] = {};
+  load(0, 0);
+  for (int s = 0; s < stages; ++s) {
+    const int buf = s & 1;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();   // this stage is in LDS, and the other buffer's readers are done
+    if (s + 1 < stages) load(s + 1, buf ^ 1);
+    const char* la = lds + buf * STAGE;
+    const char* lb = la + OpA::BYTES;
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      uint4 fa[FM], fb[FN];
+#pragma unroll
+      for (int j = 0; j < FN; ++j) fb[j] = fragment<BKC, BN>(lb, wn + j * 16, sub, lane);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) fa[i] = fragment<AKC, BM>(la, wm + i * 16, sub, lane);
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mma16<T>(fb[j], fa[i], acc[i][j]);
+    }
+  }
+  // The outputs leave 16 rows of a wave at a time through LDS, so that a row's columns are written together.
+  constexpr int COLS = FN * 16, PITCH = COLS + 4, QUADS = COLS / 4;
+  static_assert(NW * 16 * PITCH * 4 <= 2 * STAGE);
+  float* out = reinterpret_cast<float*>(lds) + wave * 16 * PITCH;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+      *reinterpret_cast<az_f32x4*>(out + (lane & 15) * PITCH + j * 16 + (lane >> 4) * 4) = acc[i][j];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int q = lane; q < 16 * QUADS; q += 64) {
+      const int m = m0 + wm + i * 16 + q / QUADS, n = n0 + wn + (q % QUADS) * 4;
+      const az_f32x4 x = *reinterpret_cast<const az_f32x4*>(out + (q / QUADS) * PITCH + (q % QUADS) * 4);
+      float v[4] = {x[0], x[1], x[2], x[3]};
+      if constexpr (SPLIT) {
+        for (int e = 0; e < 4; ++e)
+          if (!(fabsf(v[e]) < INFINITY) && m < p.M && n + e < p.N) {
+            float sum = 0.0f;
+            const int k1 = min(p.K, t1 * STEP);
+            for (int k = t0 * STEP; k < k1; ++k)
+              sum = fmaf(p.a32[AKC ? m * p.lda32 + k : k * p.lda32 + m],
+                         p.b32[BKC ? (n + e) * p.ldb32 + k : k * p.ldb32 + n + e], sum);
+            v[e] = sum;
+          }
+      }
+      finish<TO, EPI>(p, m, n, v);
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+template <typename T, typename TO, bool AKC, bool BKC, int EPI, bool SPLIT>
+int launch(const Prod& p, bool big, int splits, hipStream_t stream) {
+  const dim3 grid(p.tiles_m * p.tiles_n, 1, splits);
+  if (big)
+    k_product_wide<T, TO, 256, 256, 2, 4, AKC, BKC, EPI, SPLIT><<<grid, dim3(512), 0, stream>>>(p);
+  else
+    k_product_wide<T, TO, 128, 128, 2, 2, AKC, BKC, EPI, SPLIT><<<grid, dim3(256), 0, stream>>>(p);
+  AZ_LAUNCH_CHECK();
+  return AZ_OK;
+}
+
+}  // namespace
+
+int az_product_wide(int dtype, int pass, bool split_k, bool big, const Prod* p, int splits, hipStream_t stream) {
+  auto run = [&]<typename T, typename TO, bool SPLIT>() -> int {
+    if (pass == PASS_Y)
+      return split_k ? launch<T, TO, true, false, EPI_PARTIAL, SPLIT>(*p, big, splits, stream)
+                     : launch<T, TO, true, false, EPI_FORWARD, SPLIT>(*p, big, splits, stream);
+    if (pass == PASS_DX)
+      return split_k ? launch<T, TO, true, true, EPI_PARTIAL, SPLIT>(*p, big, splits, stream)
+                     : launch<T, TO, true, true, EPI_STORE, SPLIT>(*p, big, splits, stream);
+    return split_k ? launch<T, TO, false, false, EPI_PARTIAL, SPLIT>(*p, big, splits, stream)
+                   : launch<T, TO, false, false, EPI_STORE, SPLIT>(*p, big, splits, stream);
+  };
+  if (dtype == AZ_TYPE_F32) return run.template operator()<az_bf16, float, true>();
+  if (dtype == AZ_TYPE_BF16) return run.template operator()<az_bf16, az_bf16, false>();
+  return run.template operator()<az_f16, az_f16, false>();
+}
