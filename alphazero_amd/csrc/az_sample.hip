@@ -6,9 +6,12 @@
 // (top_k) or weights (top_p): first over logit / temperature in linear bins, whose bins a row of logits fills
 // evenly, then over the order-preserving integer of the logit within the bin that holds the cut, until that bin is a
 // single logit.  Weights are summed as 64-bit integers: the order of the LDS atomics does not matter.
-// A row is held in the registers of one workgroup (one wave for small action sets); only rows beyond that are read
-// again from L2.  float64 exponentials are taken where a weight is needed: of every action for top_p
-// alone or without truncation, of the kept actions otherwise.
+//
+// Up to 1024 actions a wave takes a row, which it holds in LDS.  Beyond, a workgroup holds the row in registers (up to
+// 32768 actions; wider rows are read from L2 again), takes the first histogram over it, and moves the actions of the bins
+// up to the cut's, in index order, into a list in LDS; one wave ends the draw on the list while the
+// others make room for the next row.  A list that would not fit (ties, a flat distribution) is left, and the
+// workgroup goes on over the row in memory.
 #include <hip/hip_runtime.h>
 
 #include "az_host.h"
@@ -19,32 +22,77 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr double LEAST = 0x1p-40;   // weights below this share of the largest are never drawn
+constexpr int LIST = 4096;          // actions of the list
+constexpr int BINS = 2048;          // of the workgroup's histogram
 
 __device__ __forceinline__ uint32_t key_of(float l) {
   const uint32_t b = __float_as_uint(l + 0.0f);   // (-0 and +0 are one logit)
   return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
-// A row spread over NT threads: a wave owns a run of chunks, a chunk is 64 x V consecutive actions, V a lane.
-template <typename T, int NT, int CHUNKS, bool REGS>
-struct Row {
-  static constexpr int V = 16 / sizeof(T), NW = NT / 64;
+__device__ __forceinline__ float logit_of(uint32_t key) {
+  return __uint_as_float((key >> 31) ? key ^ 0x80000000u : ~key);
+}
+
+// exp(x) for x <= 0, to about one unit in the last place down to 2^-1000 (then 0): 2^n times the Taylor polynomial
+// of degree 13 on |r| <= ln 2 / 2, whose remainder is below 2^-57.
+__device__ __forceinline__ double exp_neg(double x) {
+  const double n = rint(x * 1.4426950408889634);
+  double r = fma(n, -0x1.62e42fefa38p-1, x);       // ln 2 in two parts, the first with zeros at its end
+  r = fma(n, -0x1.ef35793c7673p-45, r);
+  double p = 1.0 / 6227020800.0;
+  p = fma(p, r, 1.0 / 479001600.0);
+  p = fma(p, r, 1.0 / 39916800.0);
+  p = fma(p, r, 1.0 / 3628800.0);
+  p = fma(p, r, 1.0 / 362880.0);
+  p = fma(p, r, 1.0 / 40320.0);
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return x < -690.0 ? 0.0 : ldexp(p, (int)fmax(n, -1000.0));
+}
+
+// A row's weights: exp((l - top) / temperature), also in units of 1 / unit, rounded.
+struct Weights {
+  float top;
+  double inv_t, unit;
+  __device__ __forceinline__ double operator()(float l) const { return exp_neg(((double)l - (double)top) * inv_t); }
+  __device__ __forceinline__ u64 whole(double w) const {   // (w * unit <= 2^51)
+    return (u64)__double_as_longlong(fma(w, unit, 0x1p52)) - 0x4330000000000000ull;
+  }
+  __device__ __forceinline__ u64 mass(float l) const { return whole((*this)(l)); }
+  // linear bins over 32 temperatures below the top; the last one takes what is beyond
+  __device__ __forceinline__ float scale(int bins) const { return (float)fmin(inv_t * (bins / 32), 1e30); }
+};
+
+__device__ __forceinline__ int bin_of(float top, float l, float scale, int bins) {
+  return (int)fminf((top - l) * scale, (float)(bins - 1));
+}
+
+// ---------------------------------------------------------------------------
+// Rows: `fetch(c, l)` gives this lane's V logits of chunk c (64 V consecutive actions of its wave's run), -inf where there
+// is no legal action, `index(c, v)` their actions; chunks, lanes, elements in this order are in index order.
+
+// in memory, spread over NT threads
+template <typename T, int NT>
+struct MemoryRow {
+  static constexpr int V = 16 / sizeof(T), THREADS = NT;
   const T* logits;
   const uint8_t* invalid;
-  int actions, chunks, wave, lane, start;   // start: this lane's first action
-  float reg[REGS ? CHUNKS : 1][V];
-  float infinite;   // 0, or +inf where such logits are present: they become 0, all others -inf
+  int actions, chunks, start;   // start: this lane's first action
+  bool infinite;                // +inf logits are present: they become 0, all others -inf
 
-  __device__ void init(const T* l, const uint8_t* inv, int n) {
-    logits = l, invalid = inv, actions = n, infinite = 0.0f;
-    chunks = REGS ? CHUNKS : (n + NT * V - 1) / (NT * V);
-    wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    start = wave * chunks * 64 * V + lane * V;
-    if constexpr (REGS)
-      for (int c = 0; c < CHUNKS; ++c) fetch(c, reg[c]);
+  __device__ __forceinline__ void init(const T* l, const uint8_t* inv, int n, int chunks_) {
+    logits = l, invalid = inv, actions = n, infinite = false, chunks = chunks_;
+    start = (threadIdx.x >> 6) * chunks * 64 * V + (threadIdx.x & 63) * V;
   }
-  // the chunk's logits of this lane, -inf where there is no legal action
-  __device__ void fetch(int c, float* l) const {
+  __device__ __forceinline__ int index(int c, int v) const { return start + c * 64 * V + v; }
+  __device__ __forceinline__ void fetch(int c, float* l) const {
     const int i = start + c * 64 * V;
     if (i + V <= actions) {
       const AzVec<T, V> r = az_loadu<T, V>(logits + i);
@@ -60,44 +108,59 @@ struct Row {
     }
     for (int v = 0; v < V; ++v) {
       if (l[v] != l[v]) l[v] = -INFINITY;
-      if (infinite > 0.0f) l[v] = l[v] == infinite ? 0.0f : -INFINITY;
-    }
-  }
-  __device__ void only_infinite() {
-    infinite = INFINITY;
-    if constexpr (REGS)
-      for (int c = 0; c < CHUNKS; ++c)
-        for (int v = 0; v < V; ++v) reg[c][v] = reg[c][v] == INFINITY ? 0.0f : -INFINITY;
-  }
-  // f(logit, action) for each legal action of this lane, in index order
-  template <typename F>
-  __device__ __forceinline__ void each(F&& f) const {
-    if constexpr (REGS) {
-#pragma unroll
-      for (int c = 0; c < CHUNKS; ++c)
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          if (reg[c][v] > -INFINITY) f(reg[c][v], start + c * 64 * V + v);
-    } else {
-      for (int c = 0; c < chunks; ++c) {
-        float l[V];
-        fetch(c, l);
-        for (int v = 0; v < V; ++v)
-          if (l[v] > -INFINITY) f(l[v], start + c * 64 * V + v);
-      }
+      if (infinite) l[v] = l[v] == INFINITY ? 0.0f : -INFINITY;
     }
   }
 };
 
+// in LDS, for one wave
+struct ListRow {
+  static constexpr int V = 1, THREADS = 64;
+  const float* l;
+  const int* at;    // null: the place itself
+  int n, chunks;
+  __device__ __forceinline__ int index(int c, int) const {
+    const int j = c * 64 + (threadIdx.x & 63);
+    return at ? (j < n ? at[j] : 0) : j;
+  }
+  __device__ __forceinline__ void fetch(int c, float* x) const {
+    const int j = c * 64 + (threadIdx.x & 63);
+    *x = j < n ? l[j] : -INFINITY;
+  }
+};
+
+// f(logit, action) for each legal action of this thread
+template <typename Row, typename F>
+__device__ __forceinline__ void each(const Row& row, F&& f) {
+  for (int c = 0; c < row.chunks; ++c) {
+    float l[Row::V];
+    row.fetch(c, l);
+    for (int v = 0; v < Row::V; ++v)
+      if (l[v] > -INFINITY) f(l[v], row.index(c, v));
+  }
+}
+
+// ---------------------------------------------------------------------------
 template <int NT, int NB>
 struct Shared {
   u64 bins[NB];
   u64 waves[NT / 64];
-  u64 before, found_before;
+  u64 found_before;
   uint32_t lo, hi;
   int found, index;
-  float top[NT / 64];
 };
+
+// Orders LDS accesses of a row's threads; a single wave needs no barrier (and has none: the workgroup's other waves
+// may have ended).
+template <int NT>
+__device__ __forceinline__ void sync() {
+  if constexpr (NT == 64) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    __builtin_amdgcn_wave_barrier();
+  } else {
+    __syncthreads();
+  }
+}
 
 __device__ __forceinline__ u64 shfl_up64(u64 x, int d) {
   const uint32_t lo = __shfl_up((uint32_t)x, d), hi = __shfl_up((uint32_t)(x >> 32), d);
@@ -126,11 +189,12 @@ __device__ __forceinline__ u64 wave_scan(u64 x) {   // inclusive
 template <int NT, typename S>
 __device__ __forceinline__ u64 group_sum(u64 x, S& s, u64* ahead) {
   x = wave_sum(x);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s.waves[threadIdx.x >> 6] = x;
-  __syncthreads();
-  u64 total = 0;
   *ahead = 0;
+  if constexpr (NT == 64) return x;
+  sync<NT>();
+  if ((threadIdx.x & 63) == 0) s.waves[threadIdx.x >> 6] = x;
+  sync<NT>();
+  u64 total = 0;
   for (int w = 0; w < NT / 64; ++w) {
     if (w == (int)(threadIdx.x >> 6)) *ahead = total;
     total += s.waves[w];
@@ -148,13 +212,13 @@ struct Cut {
 struct Share {
   u64 m;
   int shift;
-  __device__ explicit Share(double x) {
+  __device__ __forceinline__ explicit Share(double x) {
     int e;
     m = (u64)ldexp(frexp(x, &e), 53);
     shift = x > 0.0 ? 53 - e : 53;
   }
   // n times it, rounded down or up
-  __device__ u64 of(u64 n, bool up) const {
+  __device__ __forceinline__ u64 of(u64 n, bool up) const {
     u64 hi = __umul64hi(n, m), lo = n * m;
     if (shift >= 128) return up && (hi | lo) ? 1 : 0;
     if (shift >= 64) {
@@ -165,212 +229,181 @@ struct Share {
   }
 };
 
-template <typename T, int NT, int CHUNKS, bool REGS, int NB>
-struct Draw {
-  Row<T, NT, CHUNKS, REGS> row;
-  Shared<NT, NB>& s;
-  float top;
-  double inv_t, unit;
-
-  __device__ double weight(float l) const { return exp(((double)l - (double)top) * inv_t); }
-  __device__ u64 mass(float l) const { return (u64)(weight(l) * unit + 0.5); }
-
-  // Scans the bins: the first whose inclusive sum, with `before`, reaches the goal is left in s.found (NB: none),
-  // the sum ahead of it in s.found_before.  With `share` the goal is that share of the bins' total but `less`.
-  __device__ u64 find(u64 before, u64 goal, const Share* share, u64 less) {
-    constexpr int PER = NB / NT;
-    u64 mine = 0, ahead, h[PER];
-    for (int i = 0; i < PER; ++i) mine += h[i] = s.bins[threadIdx.x * PER + i];
-    const u64 scan = wave_scan(mine);
-    const u64 total = group_sum<NT>(mine, s, &ahead);
-    if (threadIdx.x == 0) s.found = NB;
-    __syncthreads();
-    if (share) {
-      goal = share->of(total - less, true);
-      if (goal == 0) goal = 1;   // the first one at least
-    }
-    u64 cum = before + ahead + scan - mine;
-    for (int i = 0; i < PER; ++i) {   // exactly one bin crosses
-      const u64 next = cum + h[i];
-      if (cum < goal && next >= goal) s.found = threadIdx.x * PER + i, s.found_before = cum;
-      cum = next;
-    }
-    __syncthreads();
-    return goal;
+// Scans the bins: the first whose inclusive sum, with `before`, reaches the goal is left in s.found (NB: none),
+// the sum ahead of it in s.found_before.  With `share` the goal is that share of the bins' total but `less` (of the
+// first one at least).
+template <int NT, int NB>
+__device__ __forceinline__ u64 find(Shared<NT, NB>& s, u64 before, u64 goal, const Share* share, u64 less) {
+  constexpr int PER = NB / NT;
+  const int t = threadIdx.x & (NT - 1);
+  u64 mine = 0, ahead, h[PER];
+  for (int i = 0; i < PER; ++i) mine += h[i] = s.bins[t * PER + i];
+  const u64 scan = wave_scan(mine);
+  const u64 total = group_sum<NT>(mine, s, &ahead);
+  if (t == 0) s.found = NB;
+  sync<NT>();
+  if (share) {
+    goal = share->of(total - less, true);
+    if (goal == 0) goal = 1;
   }
+  u64 cum = before + ahead + scan - mine;
+  for (int i = 0; i < PER; ++i) {   // one bin crosses at most
+    const u64 next = cum + h[i];
+    if (cum < goal && next >= goal) s.found = t * PER + i, s.found_before = cum;
+    cum = next;
+  }
+  sync<NT>();
+  return goal;
+}
 
-  // The shortest prefix of the descending order, among logits with a key >= `least`, whose counts (MASS: weights) sum up
-  // to the goal; false if there is none (no cut).
-  template <bool MASS>
-  __device__ bool select(u64 goal, const Share* share, uint32_t least, u64 less, Cut* cut) {
-    // linear bins over (top - l) / temperature: 32 of it, the last bin takes what is beyond
-    const float scale = (float)fmin(inv_t * (NB / 32), 1e30);
-    auto bin_of = [&](float l) { return (int)fminf((top - l) * scale, (float)(NB - 1)); };
-    auto add = [&](int bin, float l) {
-      if constexpr (MASS)
-        atomicAdd(&s.bins[bin], mass(l));
-      else
-        atomicAdd(reinterpret_cast<uint32_t*>(&s.bins[bin]), 1u);
-    };
-    auto clear = [&] {
-      __syncthreads();
-      for (int i = threadIdx.x; i < NB; i += NT) s.bins[i] = 0;
-      __syncthreads();
-    };
-    clear();
-    row.each([&](float l, int) {
-      if (key_of(l) >= least) add(bin_of(l), l);
-    });
-    __syncthreads();
-    goal = find(0, goal, share, less);
-    const int bin = s.found;
-    u64 before = s.found_before;
-    // (a count that ends in the last bin cuts only weights that are never drawn)
-    if (bin == NB || (!MASS && bin == NB - 1)) return false;
-    if (threadIdx.x == 0) s.lo = 0xffffffffu, s.hi = 0;
-    __syncthreads();
-    uint32_t lo = 0xffffffffu, hi = 0;
-    row.each([&](float l, int) {
+template <int NT, int NB>
+__device__ __forceinline__ void clear(Shared<NT, NB>& s) {
+  sync<NT>();
+  for (int i = threadIdx.x & (NT - 1); i < NB; i += NT) s.bins[i] = 0;
+  sync<NT>();
+}
+
+template <bool MASS, int NT, int NB>
+__device__ __forceinline__ void count(Shared<NT, NB>& s, int bin, const Weights& w, float l) {
+  if constexpr (MASS)
+    atomicAdd(&s.bins[bin], w.mass(l));
+  else
+    atomicAdd(reinterpret_cast<uint32_t*>(&s.bins[bin]), 1u);
+}
+
+// The shortest prefix of the descending order, among logits with a key >= `least`, whose counts (MASS: weights) sum up
+// to the goal; false if there is none (no cut).
+template <bool MASS, int NB, typename Row>
+__device__ __forceinline__ bool select(const Row& row, Shared<Row::THREADS, NB>& s, const Weights& w, u64 goal, const Share* share,
+                       uint32_t least, u64 less, Cut* cut) {
+  constexpr int NT = Row::THREADS;
+  const float scale = w.scale(NB);
+  clear(s);
+  each(row, [&](float l, int) {
+    if (key_of(l) >= least) count<MASS>(s, bin_of(w.top, l, scale, NB), w, l);
+  });
+  sync<NT>();
+  goal = find(s, 0, goal, share, less);
+  const int bin = s.found;
+  u64 before = s.found_before;
+  // (a count that ends in the last bin cuts only weights that are never drawn)
+  if (bin == NB || (!MASS && bin == NB - 1)) return false;
+  if ((threadIdx.x & (NT - 1)) == 0) s.lo = 0xffffffffu, s.hi = 0;
+  sync<NT>();
+  uint32_t lo = 0xffffffffu, hi = 0;
+  each(row, [&](float l, int) {
+    const uint32_t k = key_of(l);
+    if (k >= least && bin_of(w.top, l, scale, NB) == bin) lo = min(lo, k), hi = max(hi, k);
+  });
+  if (lo <= hi) atomicMin(&s.lo, lo), atomicMax(&s.hi, hi);
+  sync<NT>();
+  lo = s.lo, hi = s.hi;
+  while (lo < hi) {
+    const int bits = 32 - __clz(hi - lo), shift = max(0, bits - (31 - __clz(NB)));
+    clear(s);
+    each(row, [&](float l, int) {
       const uint32_t k = key_of(l);
-      if (k >= least && bin_of(l) == bin) lo = min(lo, k), hi = max(hi, k);
+      if (k >= lo && k <= hi) count<MASS>(s, (hi - k) >> shift, w, l);
     });
-    for (int off = 32; off > 0; off >>= 1)
-      lo = min(lo, (uint32_t)__shfl_xor(lo, off)), hi = max(hi, (uint32_t)__shfl_xor(hi, off));
-    if ((threadIdx.x & 63) == 0 && lo <= hi) atomicMin(&s.lo, lo), atomicMax(&s.hi, hi);
-    __syncthreads();
-    lo = s.lo, hi = s.hi;
-    while (lo < hi) {
-      const int bits = 32 - __clz(hi - lo), shift = max(0, bits - (31 - __clz(NB)));
-      clear();
-      row.each([&](float l, int) {
-        const uint32_t k = key_of(l);
-        if (k >= lo && k <= hi) add((hi - k) >> shift, l);
-      });
-      __syncthreads();
-      find(before, goal, nullptr, 0);
-      // (the sums over these keys are those of the bin that crossed, so one of its bins crosses)
-      if (s.found >= NB) break;
-      const uint32_t b = s.found;
-      before = s.found_before;
-      hi -= b << shift;
-      const uint32_t width = (1u << shift) - 1;
-      lo = hi - lo > width ? hi - width : lo;
-      __syncthreads();
-    }
-    cut->key = lo;
-    // the fewest ties that reach the goal
-    const u64 w = MASS ? mass(logit_of(lo)) : 1;
-    cut->ties = (goal - before + w - 1) / max(w, (u64)1);
-    return true;
+    sync<NT>();
+    find(s, before, goal, nullptr, 0);
+    // (the sums over these keys are those of the bin that crossed, so one of its bins crosses)
+    if (s.found >= NB) break;
+    const uint32_t b = s.found;
+    before = s.found_before;
+    hi -= b << shift;
+    const uint32_t width = (1u << shift) - 1;
+    lo = hi - lo > width ? hi - width : lo;
+    sync<NT>();
   }
+  cut->key = lo;
+  // the fewest ties that reach the goal
+  const u64 one = MASS ? w.mass(logit_of(lo)) : 1;
+  cut->ties = one > 1 ? (goal - before + one - 1) / one : goal - before;
+  return true;
+}
 
-  __device__ static float logit_of(uint32_t key) {
-    return __uint_as_float((key >> 31) ? key ^ 0x80000000u : ~key);
-  }
-
-  // The action at which the running sum of `value`, in index order, first exceeds `target` (less than the total).
-  template <typename F>
-  __device__ int at_sum(u64 target, F&& value) {
-    u64 mine = 0, ahead;
-    row.each([&](float l, int i) { mine += value(l, i); });
+// The action at which the running sum of `value`, in index order, first exceeds `target` (less than the total).
+template <int NB, typename Row, typename F>
+__device__ __forceinline__ int at_sum(const Row& row, Shared<Row::THREADS, NB>& s, u64 target, F&& value) {
+  constexpr int NT = Row::THREADS, V = Row::V;
+  u64 ahead = 0;
+  bool here = true;
+  if constexpr (NT > 64) {
+    u64 mine = 0;
+    each(row, [&](float l, int i) { mine += value(l, i); });
     const u64 in_wave = wave_sum(mine);
     group_sum<NT>(mine, s, &ahead);
-    if (target >= ahead && target < ahead + in_wave) {
-      // this wave has it: chunk by chunk
-      u64 run = ahead;
-      int found = -1;
-      auto chunk = [&](int c, const float* l) {
-        if (found >= 0) return;
-        u64 v[Row<T, NT, CHUNKS, REGS>::V], sum = 0;
-        for (int j = 0; j < row.V; ++j)
-          sum += v[j] = l[j] > -INFINITY ? value(l[j], row.start + c * 64 * row.V + j) : 0;
-        const u64 scan = wave_scan(sum);
-        const u64 total = (u64)__shfl((uint32_t)(scan >> 32), 63) << 32 | (u64)(uint32_t)__shfl((uint32_t)scan, 63);
-        if (target < run + total) {
-          const u64 mask = __ballot(target < run + scan);
-          const int first = __ffsll((unsigned long long)mask) - 1;
-          found = 0;
-          if (row.lane == first) {
-            u64 cum = run + scan - sum;
-            for (int j = 0; j < row.V; ++j) {
-              cum += v[j];
-              if (target < cum) {
-                s.index = row.start + c * 64 * row.V + j;
-                break;
-              }
-            }
-          }
-        }
-        run += total;
-      };
-      if constexpr (REGS) {
-#pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) chunk(c, row.reg[c]);
-      } else {
-        for (int c = 0; c < row.chunks && found < 0; ++c) {
-          float l[Row<T, NT, CHUNKS, REGS>::V];
-          row.fetch(c, l);
-          chunk(c, l);
-        }
-      }
-    }
-    __syncthreads();
-    return s.index;
+    here = target >= ahead && target < ahead + in_wave;
   }
+  if (here) {   // this wave has it: chunk by chunk
+    u64 run = ahead;
+    for (int c = 0; c < row.chunks; ++c) {
+      float l[V];
+      u64 x[V], sum = 0;
+      row.fetch(c, l);
+      for (int v = 0; v < V; ++v) sum += x[v] = l[v] > -INFINITY ? value(l[v], row.index(c, v)) : 0;
+      const u64 scan = wave_scan(sum);
+      const u64 total = (u64)__shfl((uint32_t)(scan >> 32), 63) << 32 | (u64)(uint32_t)__shfl((uint32_t)scan, 63);
+      if (target < run + total) {
+        const u64 mask = __ballot(target < run + scan);
+        if ((int)(threadIdx.x & 63) == __ffsll(mask) - 1) {
+          u64 cum = run + scan - sum;
+          int found = -1;
+          for (int v = 0; v < V; ++v) {
+            cum += x[v];
+            if (found < 0 && target < cum) found = row.index(c, v);
+          }
+          s.index = found;
+        }
+        break;
+      }
+      run += total;
+    }
+  }
+  sync<NT>();
+  return s.index;
+}
+
+struct Options {
+  int top_k;          // 0: all
+  double top_p;       // 1: all
+  double min_p;       // at least LEAST
+  float uniform;
+  u64 goal;           // the weight that top_p asks for where it is known (0: the row has it)
 };
 
-template <typename T, int NT, int CHUNKS, bool REGS>
-__global__ __launch_bounds__(NT) void k_sample(az_sample_desc d, int32_t* action, float* log_prob, double unit) {
-  constexpr int NB = NT == 64 ? 256 : NT == 256 ? 1024 : 2048;
-  __shared__ Shared<NT, NB> s;
-  const int b = blockIdx.x;
-  Draw<T, NT, CHUNKS, REGS, NB> w{{}, s};
-  w.row.init((const T*)d.logits + (int64_t)b * d.actions, d.invalid ? d.invalid + (int64_t)b * d.actions : nullptr,
-             d.actions);
-  double temperature = d.temperature_rows ? (double)d.temperature_rows[b] : d.temperature;
-  int top_k = d.top_k_rows ? d.top_k_rows[b] : d.top_k;
-  double top_p = d.top_p_rows ? (double)d.top_p_rows[b] : d.top_p;
-  double min_p = d.min_p_rows ? (double)d.min_p_rows[b] : d.min_p;
-  if (!(temperature > 0)) temperature = 1.0, top_k = 1;
-  if (top_k <= 0 || top_k >= d.actions) top_k = d.actions;
-  const bool nucleus = top_p < 1.0;
-  if (!(top_p > 0.0)) top_p = 0.0;
-  min_p = min_p > LEAST ? fmin(min_p, 1.0) : LEAST;
+struct Result {
+  int action;
+  double mass;        // of the kept actions, as a share of the largest weight
+};
 
-  float top = -INFINITY;
-  w.row.each([&](float l, int) { top = fmaxf(top, l); });
-  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-  if (w.row.lane == 0) s.top[w.row.wave] = top;
-  if (threadIdx.x == 0) s.index = 0;
-  __syncthreads();
-  for (int i = 0; i < NT / 64; ++i) top = fmaxf(top, s.top[i]);
-  if (top == -INFINITY) {   // no legal action
-    if (threadIdx.x == 0) {
-      action[b] = 0;
-      if (log_prob) log_prob[b] = -INFINITY;
-    }
-    return;
-  }
-  if (top == INFINITY) w.row.only_infinite(), top = 0.0f;
-  w.top = top, w.inv_t = 1.0 / temperature, w.unit = unit;
+__device__ __forceinline__ u64 target_of(float u, u64 total) {
+  u64 target = u > 0.0f ? total : 0;   // (not a number: 0)
+  if (u > 0.0f && u < 1.0f) target = Share((double)u).of(total, false);
+  return target >= total ? total - 1 : target;
+}
 
+// The whole draw over a row.
+template <int NB, typename Row>
+__device__ __forceinline__ Result draw(const Row& row, Shared<Row::THREADS, NB>& s, const Weights& w, const Options& o) {
+  constexpr int NT = Row::THREADS;
   Cut cut = {0, ~0ull};
-  if (top_k < d.actions) {
+  auto ties_of = [&](uint32_t key) {
+    u64 ties = 0, ahead;
+    each(row, [&](float l, int) { ties += key_of(l) == key; });
+    return group_sum<NT>(ties, s, &ahead);
+  };
+  if (o.top_k > 0) {
     Cut c;
-    if (w.template select<false>(top_k, nullptr, 0, 0, &c)) cut = c;
+    if (select<false>(row, s, w, (u64)o.top_k, nullptr, 0, 0, &c)) cut = c;
   }
-  if (nucleus) {
-    u64 less = 0;   // the weight of the ties at the top_k cut that are out
-    if (cut.key) {
-      const uint32_t key = cut.key;
-      u64 ties = 0, ahead;
-      w.row.each([&](float l, int) { ties += key_of(l) == key; });
-      ties = group_sum<NT>(ties, s, &ahead);
-      less = (ties - cut.ties) * w.mass(w.logit_of(key));
-    }
+  if (o.top_p < 1.0) {
+    // the weight of the ties at the top_k cut that are out
+    const u64 less = cut.key && !o.goal ? (ties_of(cut.key) - cut.ties) * w.mass(logit_of(cut.key)) : 0;
+    const Share share(o.top_p);
     Cut c;
-    const Share share(top_p);
-    if (w.template select<true>(0, &share, cut.key, less, &c)) {
+    if (select<true>(row, s, w, o.goal, o.goal ? nullptr : &share, cut.key, less, &c)) {
       if (c.key > cut.key)
         cut = c;
       else if (c.key == cut.key && c.ties < cut.ties)
@@ -378,44 +411,259 @@ __global__ __launch_bounds__(NT) void k_sample(az_sample_desc d, int32_t* action
     }
   }
   int last_tie = 0x7fffffff;
-  if (cut.ties != ~0ull) {
+  if (cut.ties != ~0ull && cut.ties < ties_of(cut.key)) {
     const uint32_t key = cut.key;
-    u64 ties = 0, ahead;
-    w.row.each([&](float l, int) { ties += key_of(l) == key; });
-    ties = group_sum<NT>(ties, s, &ahead);
-    if (cut.ties < ties) last_tie = w.at_sum(cut.ties - 1, [&](float l, int) { return (u64)(key_of(l) == key); });
+    last_tie = at_sum(row, s, cut.ties - 1, [&](float l, int) { return (u64)(key_of(l) == key); });
   }
   auto kept = [&](float l, int i) -> u64 {
     const uint32_t k = key_of(l);
     if (k < cut.key || (k == cut.key && i > last_tie)) return 0;
-    const double x = w.weight(l);
-    return x >= min_p ? (u64)(x * unit + 0.5) : 0;
+    const double x = w(l);
+    return x >= o.min_p ? w.whole(x) : 0;
   };
   u64 mine = 0, ahead;
-  w.row.each([&](float l, int i) { mine += kept(l, i); });
+  each(row, [&](float l, int i) { mine += kept(l, i); });
   const u64 total = group_sum<NT>(mine, s, &ahead);
-  const float u = d.uniform[b];
-  u64 target = u > 0.0f ? total : 0;   // (not a number: 0)
-  if (u > 0.0f && u < 1.0f) target = Share((double)u).of(total, false);
-  if (target >= total) target = total - 1;
-  const int i = w.at_sum(target, kept);
-  if (threadIdx.x == 0) {
-    action[b] = i;
-    if (log_prob) {
-      float l = (float)((const T*)d.logits)[(int64_t)b * d.actions + i];
-      if (l == INFINITY) l = 0.0f;   // (then top is 0 too)
-      log_prob[b] = (float)(((double)l - (double)top) * w.inv_t - log((double)total / unit));
-    }
-  }
+  return {at_sum(row, s, target_of(o.uniform, total), kept), (double)total / w.unit};
 }
 
-template <typename T, int NT, int CHUNKS, bool REGS>
-void launch(const az_sample_desc& d, int32_t* action, float* log_prob, hipStream_t stream) {
-  // weights of up to one unit each sum up below 2^62, and each is exact in float64
-  int bits = 62 - (32 - __builtin_clz((unsigned)d.actions));
-  if (bits > 52) bits = 52;
-  k_sample<T, NT, CHUNKS, REGS>
-      <<<dim3(d.rows), dim3(NT), 0, stream>>>(d, action, log_prob, (double)(1ull << bits));
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ Options options_of(const az_sample_desc& d, int b, double* temperature) {
+  Options o;
+  *temperature = d.temperature_rows ? (double)d.temperature_rows[b] : d.temperature;
+  o.top_k = d.top_k_rows ? d.top_k_rows[b] : d.top_k;
+  o.top_p = d.top_p_rows ? (double)d.top_p_rows[b] : d.top_p;
+  o.min_p = d.min_p_rows ? (double)d.min_p_rows[b] : d.min_p;
+  o.uniform = d.uniform[b];
+  o.goal = 0;
+  if (!(*temperature > 0)) *temperature = 1.0, o.top_k = 1;
+  if (o.top_k <= 0 || o.top_k >= d.actions) o.top_k = 0;
+  o.top_p = o.top_p < 1.0 ? (o.top_p > 0.0 ? o.top_p : 0.0) : 1.0;
+  o.min_p = o.min_p > LEAST ? fmin(o.min_p, 1.0) : LEAST;
+  return o;
+}
+
+template <typename T>
+__device__ __forceinline__ void write(const az_sample_desc& d, int b, const Weights& w, const Result& r, int32_t* action,
+                                      float* log_prob) {
+  action[b] = r.action;
+  if (!log_prob) return;
+  float l = (float)((const T*)d.logits)[(int64_t)b * d.actions + r.action];
+  if (l == INFINITY) l = 0.0f;   // (then the top is 0 too)
+  log_prob[b] = (float)(((double)l - (double)w.top) * w.inv_t - log(r.mass));
+}
+
+__device__ __forceinline__ void write_none(int b, int32_t* action, float* log_prob) {
+  action[b] = 0;
+  if (log_prob) log_prob[b] = -INFINITY;
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+  for (int off = 32; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off));
+  return x;
+}
+
+// Up to MOST actions: a wave a row, WAVES rows a workgroup.
+template <typename T, int MOST, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_sample_wave(az_sample_desc d, int32_t* action, float* log_prob,
+                                                            double unit) {
+  constexpr int V = 16 / sizeof(T), NB = 256;
+  __shared__ Shared<64, NB> shared[WAVES];
+  __shared__ float list[WAVES][MOST];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, b = blockIdx.x * WAVES + wave;
+  if (b >= d.rows) return;
+  double temperature;
+  const Options o = options_of(d, b, &temperature);
+  MemoryRow<T, 64> memory;
+  memory.init((const T*)d.logits + (int64_t)b * d.actions, d.invalid ? d.invalid + (int64_t)b * d.actions : nullptr,
+              d.actions, (d.actions + 64 * V - 1) / (64 * V));
+  memory.start = lane * V;
+  float top = -INFINITY;
+  for (int c = 0; c < memory.chunks; ++c) {
+    float l[V];
+    memory.fetch(c, l);
+    for (int v = 0; v < V; ++v) {
+      top = fmaxf(top, l[v]);
+      if (memory.index(c, v) < d.actions) list[wave][memory.index(c, v)] = l[v];
+    }
+  }
+  top = wave_max(top);
+  if (top == -INFINITY) {
+    if (lane == 0) write_none(b, action, log_prob);
+    return;
+  }
+  sync<64>();
+  if (top == INFINITY) {
+    for (int i = lane; i < d.actions; i += 64) list[wave][i] = list[wave][i] == INFINITY ? 0.0f : -INFINITY;
+    top = 0.0f;
+    sync<64>();
+  }
+  const Weights w = {top, 1.0 / temperature, unit};
+  const ListRow row = {list[wave], nullptr, d.actions, (d.actions + 63) / 64};
+  const Result r = draw<NB>(row, shared[wave], w, o);
+  if (lane == 0) write<T>(d, b, w, r, action, log_prob);
+}
+
+// A row in the registers of a workgroup (CHUNKS > 0) or in memory.
+template <typename T, int NT, int CHUNKS>
+struct FrontRow {
+  static constexpr int V = 16 / sizeof(T);
+  float reg[CHUNKS > 0 ? CHUNKS : 1][V];
+  // f(c, logits) for each chunk
+  template <typename F>
+  __device__ __forceinline__ void chunks(const MemoryRow<T, NT>& m, F&& f) const {
+    if constexpr (CHUNKS > 0) {
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        f(c, reg[c]);
+        __builtin_amdgcn_sched_barrier(0);   // (chunks worked side by side would need the registers of all of them)
+      }
+    } else {
+      for (int c = 0; c < m.chunks; ++c) {
+        float l[V];
+        m.fetch(c, l);
+        f(c, l);
+      }
+    }
+  }
+};
+
+template <typename T, int NT, int CHUNKS>
+__global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_t* action, float* log_prob, double unit) {
+  constexpr int V = 16 / sizeof(T), NW = NT / 64;
+  __shared__ Shared<NT, BINS> s;
+  __shared__ Shared<64, 256> s1;
+  __shared__ float list[LIST];
+  __shared__ int list_at[LIST];
+  __shared__ float tops[NW];
+  __shared__ int counts[NW];
+  const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  double temperature;
+  Options o = options_of(d, b, &temperature);
+  MemoryRow<T, NT> memory;
+  memory.init((const T*)d.logits + (int64_t)b * d.actions, d.invalid ? d.invalid + (int64_t)b * d.actions : nullptr,
+              d.actions, CHUNKS > 0 ? CHUNKS : (d.actions + NT * V - 1) / (NT * V));
+  FrontRow<T, NT, CHUNKS> front;
+  if constexpr (CHUNKS > 0) {
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) memory.fetch(c, front.reg[c]);
+  }
+  float top = -INFINITY;
+  front.chunks(memory, [&](int, const float* l) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) top = fmaxf(top, l[v]);
+  });
+  top = wave_max(top);
+  if (lane == 0) tops[wave] = top;
+  __syncthreads();
+  for (int i = 0; i < NW; ++i) top = fmaxf(top, tops[i]);
+  if (top == -INFINITY) {
+    if (threadIdx.x == 0) write_none(b, action, log_prob);
+    return;
+  }
+  if (top == INFINITY) {
+    memory.infinite = true, top = 0.0f;
+    if constexpr (CHUNKS > 0) {
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+        for (int v = 0; v < V; ++v) front.reg[c][v] = front.reg[c][v] == INFINITY ? 0.0f : -INFINITY;
+    }
+  }
+  const Weights w = {top, 1.0 / temperature, unit};
+  const float scale = w.scale(BINS);
+  // the bin that holds the first cut
+  int bound = BINS;
+  if (o.top_k > 0) {
+    clear(s);
+    front.chunks(memory, [&](int, const float* l) {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (l[v] > -INFINITY) count<false>(s, bin_of(top, l[v], scale, BINS), w, l[v]);
+    });
+    __syncthreads();
+    find(s, 0, (u64)o.top_k, nullptr, 0);
+    bound = s.found;
+    if (bound >= BINS - 1) bound = BINS, o.top_k = 0;   // nothing that could be drawn is cut
+  }
+  if (bound == BINS && o.top_p < 1.0) {
+    clear(s);
+    front.chunks(memory, [&](int, const float* l) {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (l[v] > -INFINITY) count<true>(s, bin_of(top, l[v], scale, BINS), w, l[v]);
+    });
+    __syncthreads();
+    const Share share(o.top_p);
+    o.goal = find(s, 0, 0, &share, 0);
+    bound = s.found;
+  }
+  if (bound == BINS) {
+    // no cut but min_p's: sums over the row, then the one wave that has the action looks for it
+    u64 mine = 0, ahead;
+    auto kept = [&](float l, int) -> u64 {
+      const double x = w(l);
+      return x >= o.min_p ? w.whole(x) : 0;
+    };
+    front.chunks(memory, [&](int, const float* l) {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (l[v] > -INFINITY) mine += kept(l[v], 0);
+    });
+    const u64 in_wave = wave_sum(mine), total = group_sum<NT>(mine, s, &ahead);
+    const u64 target = target_of(o.uniform, total);
+    if (target >= ahead && target < ahead + in_wave) {
+      MemoryRow<T, 64> run;   // the wave's part of the row
+      run.init(memory.logits, memory.invalid, d.actions, memory.chunks);
+      run.start = memory.start, run.infinite = memory.infinite;
+      const int i = at_sum(run, s1, target - ahead, kept);
+      if (lane == 0) write<T>(d, b, w, Result{i, (double)total / w.unit}, action, log_prob);
+    }
+    return;
+  }
+  // the actions up to that bin, in index order, into the list
+  int mine = 0;
+  front.chunks(memory, [&](int, const float* l) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) mine += l[v] > -INFINITY && bin_of(top, l[v], scale, BINS) <= bound;
+  });
+  for (int off = 32; off > 0; off >>= 1) mine += __shfl_xor(mine, off);
+  if (lane == 0) counts[wave] = mine;
+  __syncthreads();
+  int n = 0, at = 0;
+  for (int i = 0; i < NW; ++i) {
+    if (i == wave) at = n;
+    n += counts[i];
+  }
+  if (n > LIST) {
+    const Result r = draw<BINS>(memory, s, w, o);
+    if (threadIdx.x == 0) write<T>(d, b, w, r, action, log_prob);
+    return;
+  }
+  front.chunks(memory, [&](int c, const float* l) {
+    int has = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) has += l[v] > -INFINITY && bin_of(top, l[v], scale, BINS) <= bound;
+    if (__ballot(has) == 0) return;
+    int scan = has;
+    for (int off = 1; off < 64; off <<= 1) {
+      const int y = __shfl_up(scan, off);
+      if (lane >= off) scan += y;
+    }
+    int to = at + scan - has;
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (l[v] > -INFINITY && bin_of(top, l[v], scale, BINS) <= bound) {
+        list[to] = l[v];
+        list_at[to++] = memory.index(c, v);
+      }
+    at += __shfl(scan, 63);
+  });
+  __syncthreads();
+  if (wave > 0) return;
+  const ListRow row = {list, list_at, n, (n + 63) / 64};
+  const Result r = draw<256>(row, s1, w, o);
+  if (lane == 0) write<T>(d, b, w, r, action, log_prob);
 }
 
 }  // namespace
@@ -429,23 +677,24 @@ extern "C" int az_sample_actions(const az_sample_desc* d, int32_t* action, float
   if (d->rows == 0) return AZ_OK;
   if (!d->logits || !d->uniform || !action) return az_fail(AZ_ERR_INVALID, "sample: null logits, uniform or action");
   hipStream_t stream = (hipStream_t)stream_;
+  // weights of up to one unit each sum up below 2^62, and each is exact in float64
+  int bits = 62 - (32 - __builtin_clz((unsigned)d->actions));
+  if (bits > 51) bits = 51;
+  const double unit = (double)(1ull << bits);
   return az_dispatch_type(d->dtype, [&]<typename T>() -> int {
     constexpr int V = 16 / sizeof(T);
     const int n = d->actions;
-    if (n <= 64 * V)
-      launch<T, 64, 1, true>(*d, action, log_prob, stream);
-    else if (n <= 64 * 2 * V)
-      launch<T, 64, 2, true>(*d, action, log_prob, stream);
-    else if (n <= 256 * V * (8 / V))
-      launch<T, 256, 8 / V, true>(*d, action, log_prob, stream);
-    else if (n <= 1024 * 8)
-      launch<T, 1024, 8 / V, true>(*d, action, log_prob, stream);
-    else if (n <= 1024 * 16)
-      launch<T, 1024, 16 / V, true>(*d, action, log_prob, stream);
-    else if (n <= 1024 * 32)
-      launch<T, 1024, 32 / V, true>(*d, action, log_prob, stream);
+    const dim3 rows(d->rows);
+    if (n <= 1024)
+      k_sample_wave<T, 1024, 1><<<rows, dim3(64), 0, stream>>>(*d, action, log_prob, unit);
+    else if (n <= 512 * 16)
+      k_sample_group<T, 512, 16 / V><<<rows, dim3(512), 0, stream>>>(*d, action, log_prob, unit);
+    else if (n <= 512 * 32)
+      k_sample_group<T, 512, 32 / V><<<rows, dim3(512), 0, stream>>>(*d, action, log_prob, unit);
+    else if (n <= 512 * 64)
+      k_sample_group<T, 512, 64 / V><<<rows, dim3(512), 0, stream>>>(*d, action, log_prob, unit);
     else
-      launch<T, 1024, 1, false>(*d, action, log_prob, stream);
+      k_sample_group<T, 512, 0><<<rows, dim3(512), 0, stream>>>(*d, action, log_prob, unit);
     AZ_LAUNCH_CHECK();
     return AZ_OK;
   });
