@@ -163,5 +163,5 @@ def sample_actions(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0
         d.invalid = keep[-1].data_ptr()
     action = torch.empty((B,), dtype=torch.int32, device=logits.device)
     log_prob = torch.empty((B,), dtype=torch.float32, device=logits.device)
-    layers._native(logits.device, nat.lib().az_sample_actions, C.byref(d), nat.ptr(action), nat.ptr(log_prob))
+    layers._native(logits.device, nat.lib().az_sample_actions, C.byref(d), action, log_prob)
     return action, log_prob

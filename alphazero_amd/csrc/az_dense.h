@@ -12,9 +12,20 @@ namespace az_dense {
 
 // ---------------------------------------------------------------------------
 // activations, in float32
+// exp(-z): the exponent's product with log2(e) in two parts, the second one (below 2^-24 of the first) to first
+// order.  Off by three units in the last place where the result is normal.
+__device__ __forceinline__ float exp_minus(float z) {
+  const float hi = -1.44269502f * z;
+  const float lo = fmaf(z, -1.92596303e-8f, fmaf(z, -1.44269502f, -hi));
+  const float e = __builtin_amdgcn_exp2f(hi);
+  return fabsf(lo) < 1.0f ? e * fmaf(0.693147182f, lo, 1.0f) : e;   // (infinite z)
+}
+
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + exp_minus(z)); }
+
 __device__ __forceinline__ float act_value(float z, int act) {
   if (act == AZ_ACT_RELU) return z != z ? z : fmaxf(z, 0.0f);
-  if (act == AZ_ACT_SWISH) return z / (1.0f + expf(-z));
+  if (act == AZ_ACT_SWISH) return z * sigmoid(z);
   if (act == AZ_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
   return z;
 }
@@ -22,11 +33,11 @@ __device__ __forceinline__ float act_value(float z, int act) {
 __device__ __forceinline__ float act_slope(float z, int act) {
   if (act == AZ_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
   if (act == AZ_ACT_SWISH) {
-    const float p = 1.0f / (1.0f + expf(-z));
+    const float p = sigmoid(z);
     return p * (1.0f + z * (1.0f - p));
   }
   if (act == AZ_ACT_GELU)
-    return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * (0.39894228f * expf(-0.5f * z * z));
+    return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * (0.39894228f * exp_minus(0.5f * z * z));
   return 1.0f;
 }
 

@@ -90,9 +90,9 @@ __global__ __launch_bounds__(256) void k_product_tile(Prod p) {
 }
 
 // ---------------------------------------------------------------------------
-// Joins split sums in the order of the splits: 64 groups of four outputs a workgroup, the splits dealt to four
-// waves whose sums are added in their order.  Segment 0 takes the epilogue, segment 1 (the bias' gradient) is
-// stored as it is.
+// Joins split sums in the order of the splits.  Segment 0 (the product; few splits, many outputs) takes the epilogue,
+// 64 groups of four outputs a workgroup and its splits dealt to four threads; segment 1 (the bias' gradient; many
+// splits, few outputs) is stored as it is, 16 groups a workgroup and 16 threads each.
 struct Join {
   const float* part[2];
   int64_t length[2];
@@ -103,31 +103,32 @@ struct Join {
 
 template <typename T, int EPI>
 __global__ __launch_bounds__(256) void k_join(Join q, Prod p) {
-  __shared__ float sums[4][64][4];
+  __shared__ float sums[256][4];
   const int seg = (int64_t)blockIdx.x >= q.blocks0;
   const int64_t L = q.length[seg];
-  const int g = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t at = (((int64_t)blockIdx.x - (seg ? q.blocks0 : 0)) * 64 + g) * 4;
+  const int groups = seg ? 16 : 64, lanes = 256 / groups, g = threadIdx.x % groups, w = threadIdx.x / groups;
+  const int64_t at = (((int64_t)blockIdx.x - (seg ? q.blocks0 : 0)) * groups + g) * 4;
   const int have = (int)max((int64_t)0, min((int64_t)4, L - at));
   float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   if (have > 0) {
     const float* part = q.part[seg] + at;
-    const bool vec = L % 4 == 0;
+    if (L % 4 == 0) {
 #pragma unroll 4
-    for (int i = w; i < q.splits[seg]; i += 4) {
-      const float* r = part + (int64_t)i * L;
-      if (vec) {
-        const float4 x = *reinterpret_cast<const float4*>(r);
+      for (int i = w; i < q.splits[seg]; i += lanes) {
+        const float4 x = *reinterpret_cast<const float4*>(part + (int64_t)i * L);
         s[0] += x.x, s[1] += x.y, s[2] += x.z, s[3] += x.w;
-      } else {
-        for (int e = 0; e < have; ++e) s[e] += r[e];
       }
+    } else {
+#pragma unroll 4
+      for (int i = w; i < q.splits[seg]; i += lanes)
+        for (int e = 0; e < 4; ++e) s[e] += e < have ? part[(int64_t)i * L + e] : 0.0f;
     }
   }
-  for (int e = 0; e < 4; ++e) sums[w][g][e] = s[e];
+  for (int e = 0; e < 4; ++e) sums[threadIdx.x][e] = s[e];
   __syncthreads();
   if (w != 0 || have == 0) return;
-  for (int e = 0; e < 4; ++e) s[e] = ((sums[0][g][e] + sums[1][g][e]) + sums[2][g][e]) + sums[3][g][e];
+  for (int i = 1; i < lanes; ++i)
+    for (int e = 0; e < 4; ++e) s[e] += sums[i * groups + g][e];
   if (seg) {
     for (int e = 0; e < have; ++e) ((T*)q.out1)[at + e] = (T)s[e];
   } else if (p.out_vec) {   // N is a multiple of four: the group is in one row
@@ -146,6 +147,7 @@ __global__ __launch_bounds__(256) void k_join(Join q, Prod p) {
   }
 }
 
+// ---------------------------------------------------------------------------
 // ---------------------------------------------------------------------------
 // The three bfloat16 planes of a float32 value: each the rounding of what is left.  (A value that is not finite has
 // no such planes; the wide kernel works its outputs out again.)
@@ -179,6 +181,7 @@ __global__ __launch_bounds__(256) void k_slope(Slope p) {
   const int m_end = min(p.M, (int)(blockIdx.y + 1) * p.rows_per_chunk);
   float s[V] = {};
   if (n < p.N || ((p.dz || p.planes) && n < p.ld)) {
+#pragma unroll 2
     for (int m = blockIdx.y * p.rows_per_chunk + w; m < m_end; m += 4) {
       const int64_t at = (int64_t)m * p.N + n, to = (int64_t)m * p.ld + n;
       float d[V] = {};
@@ -265,10 +268,11 @@ int splits_of(int64_t tiles, int64_t K) {
   return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 
-// Rows of dz that one workgroup of k_slope takes: 1024 workgroups in all, 64 chunks at most (the join reads them).
+// Chunks of rows that k_slope is dealt in: 2048 workgroups in all, 256 chunks at most (the join reads them), at least
+// 16 rows each.
 int slope_chunks(int64_t rows, int64_t col_tiles) {
-  int64_t c = az_ceil(1024, col_tiles);
-  if (c > 64) c = 64;
+  int64_t c = az_ceil(2048, col_tiles);
+  if (c > 256) c = 256;
   const int64_t most = az_ceil(rows, 16);
   return (int)(c < most ? c : most);
 }
@@ -345,7 +349,7 @@ int product(Prod p, const Plan& plan, float* partial, const Join* extra, hipStre
       j.part[0] = partial, j.length[0] = (int64_t)p.M * p.N, j.splits[0] = splits;
       j.blocks0 = az_ceil(j.length[0], 256);
     }
-    const int64_t blocks = j.blocks0 + az_ceil(j.length[1], 256);
+    const int64_t blocks = j.blocks0 + az_ceil(j.length[1], 64);
     k_join<T, EPI><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(j, p);
     AZ_LAUNCH_CHECK();
   }
@@ -525,7 +529,7 @@ extern "C" int az_dense_backward(int32_t dtype, int32_t act, int32_t rows, int32
       return product<T, false, false, EPI_STORE>(p, l.dw, partial, dbias ? &j : nullptr, stream);
     }
     if (dbias) {
-      k_join<T, EPI_STORE><<<dim3((unsigned)az_ceil(fan_out, 256)), dim3(256), 0, stream>>>(j, Prod{});
+      k_join<T, EPI_STORE><<<dim3((unsigned)az_ceil(fan_out, 64)), dim3(256), 0, stream>>>(j, Prod{});
       AZ_LAUNCH_CHECK();
     }
     return AZ_OK;

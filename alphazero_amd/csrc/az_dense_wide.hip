@@ -184,21 +184,28 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product_wide(Prod p) {
         for (int j = 0; j < FN; ++j) acc[i][j] = mma16<T>(fb[j], fa[i], acc[i][j]);
     }
   }
-  // The outputs leave 16 rows of a wave at a time through LDS, so that a row's columns are written together.
-  constexpr int COLS = FN * 16, PITCH = COLS + 4, QUADS = COLS / 4;
-  static_assert(NW * 16 * PITCH * 4 <= 2 * STAGE);
-  float* out = reinterpret_cast<float*>(lds) + wave * 16 * PITCH;
+  // The outputs leave through LDS, 64 rows of a wave at a time, so that a row's columns are written together; the
+  // sixteen groups of four columns are exchanged by the row, which spreads the rows over the banks.
+  constexpr int ROUND = 4;
+  static_assert(FN == 4 && FM % ROUND == 0 && NW * ROUND * 16 * 64 * 4 <= 2 * STAGE);
+  float* out = reinterpret_cast<float*>(lds) + wave * (ROUND * 16 * 64);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
+  for (int i0 = 0; i0 < FM; i0 += ROUND) {
 #pragma unroll
-    for (int j = 0; j < FN; ++j)
-      *reinterpret_cast<az_f32x4*>(out + (lane & 15) * PITCH + j * 16 + (lane >> 4) * 4) = acc[i][j];
+    for (int i = 0; i < ROUND; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int row = i * 16 + (lane & 15), quad = j * 4 + (lane >> 4);
+        *reinterpret_cast<az_f32x4*>(out + row * 64 + ((quad ^ (row & 15)) * 4)) = acc[i0 + i][j];
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-    for (int q = lane; q < 16 * QUADS; q += 64) {
-      const int m = m0 + wm + i * 16 + q / QUADS, n = n0 + wn + (q % QUADS) * 4;
-      const az_f32x4 x = *reinterpret_cast<const az_f32x4*>(out + (q / QUADS) * PITCH + (q % QUADS) * 4);
+    const int n = n0 + wn + (lane & 15) * 4;
+#pragma unroll 4
+    for (int r = 0; r < ROUND * 16; r += 4) {
+      const int row = r + (lane >> 4), m = m0 + wm + i0 * 16 + row;
+      const az_f32x4 x = *reinterpret_cast<const az_f32x4*>(out + row * 64 + (((lane & 15) ^ (row & 15)) * 4));
       float v[4] = {x[0], x[1], x[2], x[3]};
       if constexpr (SPLIT) {
         for (int e = 0; e < 4; ++e)
@@ -213,6 +220,7 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product_wide(Prod p) {
       }
       finish<TO, EPI>(p, m, n, v);
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
   }
 }

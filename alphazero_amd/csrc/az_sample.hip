@@ -10,9 +10,11 @@
 // Up to 1024 actions a wave takes a row, which it holds in LDS.  Beyond, a workgroup holds the row in registers (up to
 // 32768 actions; wider rows are read from L2 again), takes the first histogram over it, and moves the actions of the bins
 // up to the cut's, in index order, into a list in LDS; one wave ends the draw on the list while the
-// others make room for the next row.  A list that would not fit (ties, a flat distribution) is left, and the
-// workgroup goes on over the row in memory.
+// others make room for the next row.  A row whose list would not fit (ties, a flat distribution) is left to a second
+// kernel that works over the row in memory.
 #include <hip/hip_runtime.h>
+
+#include <cfloat>
 
 #include "az_host.h"
 #include "az_types.h"
@@ -504,6 +506,13 @@ __global__ __launch_bounds__(64 * WAVES) void k_sample_wave(az_sample_desc d, in
   if (lane == 0) write<T>(d, b, w, r, action, log_prob);
 }
 
+// The same value, of which the compiler does not know it: what a pass over the row computes from it is not kept in
+// registers for the next pass.
+__device__ __forceinline__ float anew(float x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // A row in the registers of a workgroup (CHUNKS > 0) or in memory.
 template <typename T, int NT, int CHUNKS>
 struct FrontRow {
@@ -528,13 +537,15 @@ struct FrontRow {
   }
 };
 
-template <typename T, int NT, int CHUNKS>
+// DIRECT: rows that no top_k or top_p truncates.  Otherwise the truncated ones; what does not fit this kernel (a row
+// without a cut, a list that is too long) is left with action -1 for k_sample_rest.
+template <typename T, int NT, int CHUNKS, bool DIRECT>
 __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_t* action, float* log_prob, double unit) {
   constexpr int V = 16 / sizeof(T), NW = NT / 64;
-  __shared__ Shared<NT, BINS> s;
-  __shared__ Shared<64, 256> s1;
-  __shared__ float list[LIST];
-  __shared__ int list_at[LIST];
+  __shared__ Shared<NT, DIRECT ? NT : BINS> s;
+  __shared__ Shared<64, DIRECT ? 64 : 256> s1;
+  __shared__ float list[DIRECT ? 1 : LIST];
+  __shared__ int list_at[DIRECT ? 1 : LIST];
   __shared__ float tops[NW];
   __shared__ int counts[NW];
   const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -557,6 +568,7 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
   if (lane == 0) tops[wave] = top;
   __syncthreads();
   for (int i = 0; i < NW; ++i) top = fmaxf(top, tops[i]);
+  top = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(top)));
   if (top == -INFINITY) {
     if (threadIdx.x == 0) write_none(b, action, log_prob);
     return;
@@ -571,35 +583,8 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
     }
   }
   const Weights w = {top, 1.0 / temperature, unit};
-  const float scale = w.scale(BINS);
-  // the bin that holds the first cut
-  int bound = BINS;
-  if (o.top_k > 0) {
-    clear(s);
-    front.chunks(memory, [&](int, const float* l) {
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (l[v] > -INFINITY) count<false>(s, bin_of(top, l[v], scale, BINS), w, l[v]);
-    });
-    __syncthreads();
-    find(s, 0, (u64)o.top_k, nullptr, 0);
-    bound = s.found;
-    if (bound >= BINS - 1) bound = BINS, o.top_k = 0;   // nothing that could be drawn is cut
-  }
-  if (bound == BINS && o.top_p < 1.0) {
-    clear(s);
-    front.chunks(memory, [&](int, const float* l) {
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (l[v] > -INFINITY) count<true>(s, bin_of(top, l[v], scale, BINS), w, l[v]);
-    });
-    __syncthreads();
-    const Share share(o.top_p);
-    o.goal = find(s, 0, 0, &share, 0);
-    bound = s.found;
-  }
-  if (bound == BINS) {
-    // no cut but min_p's: sums over the row, then the one wave that has the action looks for it
+  if constexpr (DIRECT) {
+    // sums over the row, then the one wave that has the action looks for it
     u64 mine = 0, ahead;
     auto kept = [&](float l, int) -> u64 {
       const double x = w(l);
@@ -607,8 +592,7 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
     };
     front.chunks(memory, [&](int, const float* l) {
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (l[v] > -INFINITY) mine += kept(l[v], 0);
+      for (int v = 0; v < V; ++v) mine += kept(l[v], 0);   // (0 for no action)
     });
     const u64 in_wave = wave_sum(mine), total = group_sum<NT>(mine, s, &ahead);
     const u64 target = target_of(o.uniform, total);
@@ -619,51 +603,128 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
       const int i = at_sum(run, s1, target - ahead, kept);
       if (lane == 0) write<T>(d, b, w, Result{i, (double)total / w.unit}, action, log_prob);
     }
-    return;
-  }
-  // the actions up to that bin, in index order, into the list
-  int mine = 0;
-  front.chunks(memory, [&](int, const float* l) {
+  } else {
+    const float scale = w.scale(BINS);
+    // the bin that holds the first cut
+    int bound = BINS;
+    if (o.top_k > 0) {
+      clear(s);
+      const float none = anew(-INFINITY), scale_ = anew(scale);
+      front.chunks(memory, [&](int, const float* l) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) mine += l[v] > -INFINITY && bin_of(top, l[v], scale, BINS) <= bound;
-  });
-  for (int off = 32; off > 0; off >>= 1) mine += __shfl_xor(mine, off);
-  if (lane == 0) counts[wave] = mine;
-  __syncthreads();
-  int n = 0, at = 0;
-  for (int i = 0; i < NW; ++i) {
-    if (i == wave) at = n;
-    n += counts[i];
+        for (int v = 0; v < V; ++v)
+          if (l[v] > none) count<false>(s, bin_of(top, l[v], scale_, BINS), w, l[v]);
+      });
+      __syncthreads();
+      find(s, 0, (u64)o.top_k, nullptr, 0);
+      bound = s.found;
+      if (bound >= BINS - 1) bound = BINS, o.top_k = 0;   // nothing that could be drawn is cut
+    }
+    if (bound == BINS && o.top_p < 1.0) {
+      clear(s);
+      const float none = anew(-INFINITY), scale_ = anew(scale);
+      front.chunks(memory, [&](int, const float* l) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (l[v] > none) count<true>(s, bin_of(top, l[v], scale_, BINS), w, l[v]);
+      });
+      __syncthreads();
+      const Share share(o.top_p);
+      o.goal = find(s, 0, 0, &share, 0);
+      bound = s.found;
+    }
+    // The actions up to that bin, in index order, into the list.  A few of the next bin may come with them (the draw
+    // over the list finds the same cut): one comparison an action, with a logit that is low enough whatever the
+    // roundings of bin_of.
+    const float reach = (float)(bound + 1) / scale * (1.0f + 0x1p-18f);
+    const float least = anew(fmaxf(top - reach - (fabsf(top) + reach) * 0x1p-20f, -FLT_MAX));   // (finite)
+    int mine = 0;
+    front.chunks(memory, [&](int, const float* l) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) mine += __popcll(__ballot(l[v] >= least));
+    });
+    if (lane == 0) counts[wave] = mine;
+    __syncthreads();
+    int n = 0, at = 0;
+    for (int i = 0; i < NW; ++i) {
+      if (i == wave) at = n;
+      n += counts[i];
+    }
+    if (bound == BINS || n > LIST) {
+      if (threadIdx.x == 0) action[b] = -1;
+      return;
+    }
+    front.chunks(memory, [&](int c, const float* l) {
+      u64 has[V], any = 0;
+#pragma unroll
+      for (int v = 0; v < V; ++v) any |= has[v] = __ballot(l[v] >= least);
+      if (any == 0) return;
+      int to = at;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        to += __builtin_amdgcn_mbcnt_hi((uint32_t)(has[v] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has[v], 0));
+        at += __popcll(has[v]);
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (l[v] >= least) {
+          list[to] = l[v];
+          list_at[to++] = memory.index(c, v);
+        }
+    });
+    __syncthreads();
+    if (wave > 0) return;
+    const ListRow row = {list, list_at, n, (n + 63) / 64};
+    const Result r = draw<256>(row, s1, w, o);
+    if (lane == 0) write<T>(d, b, w, r, action, log_prob);
   }
-  if (n > LIST) {
+}
+
+// The rows that k_sample_group left, over the row in memory: a workgroup looks through PER rows.
+template <typename T, int NT, int PER>
+__global__ __launch_bounds__(NT) void k_sample_rest(az_sample_desc d, int32_t* action, float* log_prob, double unit) {
+  constexpr int V = 16 / sizeof(T), NW = NT / 64;
+  static_assert(PER <= 64);
+  __shared__ Shared<NT, BINS> s;
+  __shared__ float tops[NW];
+  const int64_t first = (int64_t)blockIdx.x * PER;
+  // (every wave reads the flags of its own accord; a row's is overwritten behind a barrier that all of them passed)
+  const int64_t mine = first + (threadIdx.x & 63);
+  u64 left = __ballot((threadIdx.x & 63) < PER && mine < d.rows && action[mine] == -1);
+  __syncthreads();
+  for (; left; left &= left - 1) {
+    const int b = (int)first + __ffsll(left) - 1;
+    double temperature;
+    const Options o = options_of(d, b, &temperature);
+    MemoryRow<T, NT> memory;
+    memory.init((const T*)d.logits + (int64_t)b * d.actions, d.invalid ? d.invalid + (int64_t)b * d.actions : nullptr,
+                d.actions, (d.actions + NT * V - 1) / (NT * V));
+    float top = -INFINITY;
+    each(memory, [&](float l, int) { top = fmaxf(top, l); });
+    top = wave_max(top);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+    for (int i = 0; i < NW; ++i) top = fmaxf(top, tops[i]);
+    if (top == INFINITY) memory.infinite = true, top = 0.0f;
+    const Weights w = {top, 1.0 / temperature, unit};
     const Result r = draw<BINS>(memory, s, w, o);
     if (threadIdx.x == 0) write<T>(d, b, w, r, action, log_prob);
-    return;
+    __syncthreads();
   }
-  front.chunks(memory, [&](int c, const float* l) {
-    int has = 0;
-#pragma unroll
-    for (int v = 0; v < V; ++v) has += l[v] > -INFINITY && bin_of(top, l[v], scale, BINS) <= bound;
-    if (__ballot(has) == 0) return;
-    int scan = has;
-    for (int off = 1; off < 64; off <<= 1) {
-      const int y = __shfl_up(scan, off);
-      if (lane >= off) scan += y;
-    }
-    int to = at + scan - has;
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (l[v] > -INFINITY && bin_of(top, l[v], scale, BINS) <= bound) {
-        list[to] = l[v];
-        list_at[to++] = memory.index(c, v);
-      }
-    at += __shfl(scan, 63);
-  });
-  __syncthreads();
-  if (wave > 0) return;
-  const ListRow row = {list, list_at, n, (n + 63) / 64};
-  const Result r = draw<256>(row, s1, w, o);
-  if (lane == 0) write<T>(d, b, w, r, action, log_prob);
+}
+
+template <typename T, int CHUNKS>
+void launch_group(const az_sample_desc& d, int32_t* action, float* log_prob, double unit, hipStream_t stream) {
+  const bool direct = !d.temperature_rows && !d.top_k_rows && !d.top_p_rows && d.temperature > 0 &&
+                      (d.top_k <= 0 || d.top_k >= d.actions) && !(d.top_p < 1.0);
+  if (direct) {
+    k_sample_group<T, 512, CHUNKS, true><<<dim3(d.rows), dim3(512), 0, stream>>>(d, action, log_prob, unit);
+  } else {
+    constexpr int PER = 8;
+    k_sample_group<T, 512, CHUNKS, false><<<dim3(d.rows), dim3(512), 0, stream>>>(d, action, log_prob, unit);
+    k_sample_rest<T, 512, PER><<<dim3((unsigned)az_ceil(d.rows, PER)), dim3(512), 0, stream>>>(d, action, log_prob, unit);
+  }
 }
 
 }  // namespace
@@ -688,13 +749,13 @@ extern "C" int az_sample_actions(const az_sample_desc* d, int32_t* action, float
     if (n <= 1024)
       k_sample_wave<T, 1024, 1><<<rows, dim3(64), 0, stream>>>(*d, action, log_prob, unit);
     else if (n <= 512 * 16)
-      k_sample_group<T, 512, 16 / V><<<rows, dim3(512), 0, stream>>>(*d, action, log_prob, unit);
+      launch_group<T, 16 / V>(*d, action, log_prob, unit, stream);
     else if (n <= 512 * 32)
-      k_sample_group<T, 512, 32 / V><<<rows, dim3(512), 0, stream>>>(*d, action, log_prob, unit);
+      launch_group<T, 32 / V>(*d, action, log_prob, unit, stream);
     else if (n <= 512 * 64)
-      k_sample_group<T, 512, 64 / V><<<rows, dim3(512), 0, stream>>>(*d, action, log_prob, unit);
+      launch_group<T, 64 / V>(*d, action, log_prob, unit, stream);
     else
-      k_sample_group<T, 512, 0><<<rows, dim3(512), 0, stream>>>(*d, action, log_prob, unit);
+      launch_group<T, 0>(*d, action, log_prob, unit, stream);
     AZ_LAUNCH_CHECK();
     return AZ_OK;
   });

@@ -13,20 +13,21 @@ DTYPES = {torch.float32: nat.TYPE_F32, torch.bfloat16: nat.TYPE_BF16, torch.floa
 ACTIVATIONS = {None: nat.ACT_NONE, "relu": nat.ACT_RELU, "swish": nat.ACT_SWISH, "gelu": nat.ACT_GELU}
 
 
-def _on(device):
-    """Native launches go to the current device's stream: makes `device` current if it is not."""
-    if device.index == torch.cuda.current_device():
-        return None
-    return torch.cuda.device(device)
+# the current stream's handle without the Stream object (a dozen microseconds in the autograd engine's thread)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _native(device, fn, *args):
-    guard = _on(device)
-    if guard is None:
-        nat.check(fn(*args, nat.stream_ptr()))
+    """Calls a native entry point on `device`, which it makes the current one (launches go to the current device's
+    stream).  Tensor arguments are contiguous; they are passed as pointers."""
+    args = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(device.index) if _raw_stream is not None else nat.stream_ptr())
     else:
-        with guard:
-            nat.check(fn(*args, nat.stream_ptr()))
+        with torch.cuda.device(device):
+            rc = fn(*args, nat.stream_ptr())
+    if rc != 0:
+        nat.check(rc)
 
 
 def _checked(op, x, others):
@@ -54,8 +55,8 @@ def _dense_forward(x, kernel, bias, residual, act, keep_z):
     if n < 0:
         nat.check(-2)
     ws = torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
-    _native(x.device, lib.az_dense_forward, code, act, M, K, N, nat.ptr(x), nat.ptr(kernel), nat.ptr(bias),
-            nat.ptr(residual), nat.ptr(y), nat.ptr(z), nat.ptr(ws), n)
+    _native(x.device, lib.az_dense_forward, code, act, M, K, N, x, kernel, bias,
+            residual, y, z, ws, n)
     return y, z
 
 
@@ -76,15 +77,15 @@ class _Dense(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx = torch.empty_like(x) if need[0] else None
         dkernel = torch.empty_like(kernel) if need[1] else None
-        dbias = torch.empty((N,), dtype=x.dtype, device=x.device) if need[2] else None
+        dbias = x.new_empty(N) if need[2] else None
         if need[0] or need[1] or need[2]:
             g = dy.contiguous()
             code = DTYPES[x.dtype]
             lib = nat.lib()
             n = lib.az_dense_workspace_bytes(code, M, K, N, 1)
-            ws = torch.empty((n,), dtype=torch.uint8, device=x.device)
-            _native(x.device, lib.az_dense_backward, code, ctx.act, M, K, N, nat.ptr(x), nat.ptr(kernel), nat.ptr(z),
-                    nat.ptr(g), nat.ptr(dx), nat.ptr(dkernel), nat.ptr(dbias), nat.ptr(ws), n)
+            ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+            _native(x.device, lib.az_dense_backward, code, ctx.act, M, K, N, x, kernel, z,
+                    g, dx, dkernel, dbias, ws, n)
         return dx, dkernel, dbias, dy if need[3] else None, None
 
 
@@ -135,8 +136,8 @@ def _norm_forward(x, scale, bias, eps, keep):
     mean = rstd = None
     if keep:
         mean, rstd = torch.empty((2, M), dtype=torch.float32, device=x.device)
-    _native(x.device, nat.lib().az_layer_norm_forward, code, pcode, M, D, nat.ptr(x), nat.ptr(scale), nat.ptr(bias),
-            eps, nat.ptr(y), nat.ptr(mean), nat.ptr(rstd))
+    _native(x.device, nat.lib().az_layer_norm_forward, code, pcode, M, D, x, scale, bias,
+            eps, y, mean, rstd)
     return y, mean, rstd
 
 
@@ -163,8 +164,8 @@ class _LayerNorm(torch.autograd.Function):
         lib = nat.lib()
         n = lib.az_layer_norm_workspace_bytes(M, D) if need[1] or need[2] else 0
         ws = torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
-        _native(x.device, lib.az_layer_norm_backward, code, DTYPES[ptype], M, D, nat.ptr(x), nat.ptr(scale),
-                nat.ptr(mean), nat.ptr(rstd), nat.ptr(g), nat.ptr(dx), nat.ptr(dscale), nat.ptr(dbias), nat.ptr(ws),
+        _native(x.device, lib.az_layer_norm_backward, code, DTYPES[ptype], M, D, x, scale,
+                mean, rstd, g, dx, dscale, dbias, ws,
                 n)
         return dx, dscale, dbias, None
 
