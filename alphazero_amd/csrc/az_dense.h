@@ -85,9 +85,10 @@ struct Prod {
   int64_t lda32, ldb32;
 };
 
-// Four consecutive outputs of row m from column n.
+// Four consecutive outputs of row m from column n.  `early`: the caller has loaded their residual.
 template <typename T, int EPI>
-__device__ __forceinline__ void finish(const Prod& p, int m, int n, const float* v) {
+__device__ __forceinline__ void finish(const Prod& p, int m, int n, const float* v, bool early = false,
+                                       AzVec<T, 4> loaded = {}) {
   if (m >= p.M || n >= p.N) return;
   const int64_t at = (int64_t)m * p.N + n;
   const int have = p.N - n < 4 ? p.N - n : 4;
@@ -117,7 +118,8 @@ __device__ __forceinline__ void finish(const Prod& p, int m, int n, const float*
         AzVec<T, 4> o, r, b;
         AzVec<Z, 4> zz;
         if (bias) b = az_loadv<T, 4>(bias + n);
-        if (res) r = az_loadv<T, 4>(res);
+        r = loaded;
+        if (res && !early) r = az_loadv<T, 4>(res);
         for (int i = 0; i < 4; ++i) {
           const float s = v[i] + (bias ? (float)b.v[i] : 0.0f);
           keep(&zz.v[i], s);

@@ -18,34 +18,48 @@ using namespace az_dense;
 namespace {
 
 // ---------------------------------------------------------------------------
-// Any sizes and alignments: 64 x 64 outputs a workgroup, four waves of 32 x 32, 64 bytes of reduction a step.
-// Operands go through registers (one step ahead, every element guarded, zero outside) into LDS, each row's reduction
-// contiguous, rows 80 bytes apart so that the 16 rows of an operand read fall on different banks.
-constexpr int TILE = 64, ROW_BYTES = 80;
+// Any sizes and alignments: 64 x 64 outputs a workgroup, four waves of 32 x 32, 256 bytes of reduction a step (64
+// float32 elements, 128 of 16 bits).  Operands go through registers (one step ahead, every element guarded, zero outside)
+// into LDS, each row's reduction contiguous, rows 272 bytes apart so that the 16 rows of an operand read fall on
+// different banks.  A step this long keeps the loads of the next one in flight for two thousand cycles of matrix
+// instructions; with 64 bytes a step the loop waited for memory.
+constexpr int TILE = 64, ROW_BYTES = 272, PACKS = 4;
 
 template <typename T, bool KC>
 struct Stage {
-  static constexpr int E = AzPack<T>::N, BK = 4 * E;
-  AzPack<T> r;
-  // row / first reduction index (KC) or first row / reduction index (not KC) of this thread's 16 bytes
-  __device__ static int row(int t) { return KC ? t / 4 : (t % (TILE / E)) * E; }
-  __device__ static int red(int t) { return KC ? (t % 4) * E : t / (TILE / E); }
+  static constexpr int E = AzPack<T>::N, BK = 4 * PACKS * E;
+  AzPack<T> r[PACKS];
+  // row / first reduction index (KC) or first row / reduction index (not KC) of this thread's pack q
+  __device__ static int row(int q) {
+    return KC ? threadIdx.x / (4 * PACKS) + q * (TILE / PACKS) : (threadIdx.x % (TILE / E)) * E;
+  }
+  __device__ static int red(int q) {
+    return KC ? (threadIdx.x % (4 * PACKS)) * E : threadIdx.x / (TILE / E) + q * (BK / PACKS);
+  }
   __device__ void load(const T* p, int64_t ld, int rows, int r0, int k0, int k1, bool vec) {
-    const int r_ = r0 + row(threadIdx.x), k_ = k0 + red(threadIdx.x);
-    const int cont = KC ? k_ : r_, cont_end = KC ? k1 : rows;
-    const bool line = KC ? r_ < rows : k_ < k1;
-    const T* q = p + (KC ? (int64_t)r_ * ld + k_ : (int64_t)k_ * ld + r_);
-    if (line && vec && cont + E <= cont_end) {
-      r = az_load16(q);
-    } else {
-      for (int e = 0; e < E; ++e) r.v[e] = line && cont + e < cont_end ? q[e] : (T)0.0f;
+#pragma unroll
+    for (int q = 0; q < PACKS; ++q) {
+      const int r_ = r0 + row(q), k_ = k0 + red(q);
+      const int cont = KC ? k_ : r_, cont_end = KC ? k1 : rows;
+      const bool line = KC ? r_ < rows : k_ < k1;
+      const T* at = p + (KC ? (int64_t)r_ * ld + k_ : (int64_t)k_ * ld + r_);
+      if (line && vec && cont + E <= cont_end) {
+        r[q] = az_load16(at);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) r[q].v[e] = line && cont + e < cont_end ? at[e] : (T)0.0f;
+      }
     }
   }
   __device__ void store(char* lds) const {
-    if constexpr (KC) {
-      az_store16((T*)(lds + row(threadIdx.x) * ROW_BYTES) + red(threadIdx.x), r);
-    } else {
-      for (int e = 0; e < E; ++e) ((T*)(lds + (row(threadIdx.x) + e) * ROW_BYTES))[red(threadIdx.x)] = r.v[e];
+#pragma unroll
+    for (int q = 0; q < PACKS; ++q) {
+      if constexpr (KC) {
+        az_store16((T*)(lds + row(q) * ROW_BYTES) + red(q), r[q]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) ((T*)(lds + (row(q) + e) * ROW_BYTES))[red(q)] = r[q].v[e];
+      }
     }
   }
 };
@@ -72,15 +86,22 @@ __global__ __launch_bounds__(256) void k_product_tile(Prod p) {
       sa.load((const T*)p.a, p.lda, p.M, m0, k + BK, k_end, p.a_vec);
       sb.load((const T*)p.b, p.ldb, p.N, n0, k + BK, k_end, p.b_vec);
     }
-    AzPack<T> fa[2], fb[2];
-    for (int i = 0; i < 2; ++i) {
-      const int off = (lane & 15) * ROW_BYTES + (lane >> 4) * 16;
-      fa[i] = az_load16((const T*)(lds[buf][0] + (wm + i * 16) * ROW_BYTES + off));
-      fb[i] = az_load16((const T*)(lds[buf][1] + (wn + i * 16) * ROW_BYTES + off));
+#pragma unroll
+    for (int q = 0; q < PACKS; ++q) {
+      if (k + q * (BK / PACKS) >= k_end) break;   // zeros from here on
+      AzPack<T> fa[2], fb[2];
+      const int off = (lane & 15) * ROW_BYTES + q * 64 + (lane >> 4) * 16;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        fa[i] = az_load16((const T*)(lds[buf][0] + (wm + i * 16) * ROW_BYTES + off));
+        fb[i] = az_load16((const T*)(lds[buf][1] + (wn + i * 16) * ROW_BYTES + off));
+      }
+      // operands exchanged: a lane then holds four consecutive columns of one output row
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
     }
-    // operands exchanged: a lane then holds four consecutive columns of one output row
-    for (int i = 0; i < 2; ++i)
-      for (int j = 0; j < 2; ++j) acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
   }
   for (int i = 0; i < 2; ++i)
     for (int j = 0; j < 2; ++j) {
@@ -260,14 +281,6 @@ __global__ void k_zero(T* p, int64_t n) {
 int size_of(int dtype) { return dtype == AZ_TYPE_F32 ? 4 : 2; }
 int64_t round16(int64_t n) { return (n + 15) & ~(int64_t)15; }
 
-// Splits of a reduction of K for tiles x splits workgroups: enough to give every compute unit two, at least 128
-// elements each.
-int splits_of(int64_t tiles, int64_t K) {
-  const int64_t want = az_ceil(512, tiles), most = az_ceil(K, 128);
-  int64_t s = want < most ? want : most;
-  return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
-}
-
 // Chunks of rows that k_slope is dealt in: 2048 workgroups in all, 256 chunks at most (the join reads them), at least
 // 16 rows each.
 int slope_chunks(int64_t rows, int64_t col_tiles) {
@@ -285,19 +298,39 @@ struct Plan {
   int splits;
 };
 
-Plan plan_of(int dtype, int64_t M, int64_t N, int64_t K) {
+// As many splits as bring `tiles` tiles to `want` workgroups, each at least `least` steps of the reduction long.
+int64_t splits_for(int64_t tiles, int64_t want, int64_t K, int64_t least) {
+  const int64_t s = az_ceil(want, tiles), most = K / least;
+  return s < most ? s : most;
+}
+
+// Measured over layers of 64 to 16384 rows and 256 to 4096 columns, in microseconds (wide / 64 x 64 tiles):
+//   16 bits: 4096 x 1024 x 1024 19 / 53, 64 x 1024 x 1024 9 / 9, 8192 x 256 x 256 10 / 10, 8 x 4096 x 4096 11 / 19; operands
+//     that have to be copied first: 1003 x 401 x 517 23 / 19
+//   float32: 4096 x 1024 x 1024 83 / 114, 1024 x 1024 x 1024 38 / 40, 256 x 2048 x 2048 43 / 38
+// 256 x 256 tiles pay from one for each compute unit on: 16384 x 512 x 2048 59 against 62 with 128 x 128 (512 tiles),
+// its dx 57 against 37 (128 tiles).
+// in_place: a 16-bit operand need not be copied for the wide kernel.
+Plan plan_of(int dtype, int64_t M, int64_t N, int64_t K, bool in_place) {
   Plan p = {};
   const double work = (double)M * N * K;
-  p.wide = work >= (dtype == AZ_TYPE_F32 ? 0x1p31 : 0x1p27) && M >= 128 && N >= 64 && K >= 128;
+  const bool f32 = dtype == AZ_TYPE_F32;
+  p.wide = work >= (f32 ? 0x1p31 : in_place ? 0x1p25 : 0x1p29);
+  int64_t s = 1;
   if (!p.wide) {
-    p.splits = splits_of(az_ceil(M, TILE) * az_ceil(N, TILE), K);
-    return p;
+    // two workgroups a compute unit for a long reduction, one otherwise; a few tiles are split down to 32 steps
+    const int64_t tiles = az_ceil(M, TILE) * az_ceil(N, TILE);
+    s = splits_for(tiles, K >= 1024 ? 512 : 256, K, tiles <= 16 ? 32 : 128);
+  } else {
+    const int64_t large = az_ceil(M, 256) * az_ceil(N, 256), steps = f32 ? 6 * K : K;
+    p.big = large >= 256;
+    if (!p.big) {
+      const int64_t tiles = az_ceil(M, 128) * az_ceil(N, 128);
+      const int64_t one = splits_for(tiles, 256, steps, 512), two = splits_for(tiles, 512, steps, 2048);
+      s = one > two ? one : two;
+      if (s > K / 64) s = K / 64;
+    }
   }
-  const int64_t large = az_ceil(M, 256) * az_ceil(N, 256), small = az_ceil(M, 128) * az_ceil(N, 128);
-  p.big = large >= 128 || (large >= 16 && K >= 256 * 64 / large);
-  const int64_t tiles = p.big ? large : small, want = p.big ? 256 : 512, most = az_ceil(K, 512);
-  int64_t s = tiles >= want / 2 ? 1 : want / tiles;
-  if (s > most) s = most;
   p.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
   return p;
 }
@@ -374,11 +407,11 @@ Layout layout_of(int dtype, int64_t M, int64_t K, int64_t N, int pass) {
     return here;
   };
   if (pass == 0) {
-    l.y = plan_of(dtype, M, N, K);
+    l.y = plan_of(dtype, M, N, K, K % 64 == 0 && N % 8 == 0);
     if (l.y.wide) l.x = room(M * Kp * each), l.kernel = room(K * Np * each);
     if (l.y.splits > 1) l.partial = room(l.y.splits * M * N * 4);
   } else {
-    l.dx = plan_of(dtype, M, K, N), l.dw = plan_of(dtype, K, N, M);
+    l.dx = plan_of(dtype, M, K, N, N % 64 == 0), l.dw = plan_of(dtype, K, N, M, K % 8 == 0 && N % 8 == 0);
     l.chunks = slope_chunks(M, az_ceil(N, 64 * (N % 4 == 0 ? 4 : 1)));
     l.dz = room(M * Np * size_of(dtype));
     if (dtype == AZ_TYPE_F32 && (l.dx.wide || l.dw.wide)) l.dz_planes = room(M * Np * 6);

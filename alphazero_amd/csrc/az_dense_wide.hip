@@ -202,23 +202,44 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product_wide(Prod p) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
     const int n = n0 + wn + (lane & 15) * 4;
-#pragma unroll 4
-    for (int r = 0; r < ROUND * 16; r += 4) {
-      const int row = r + (lane >> 4), m = m0 + wm + i0 * 16 + row;
-      const az_f32x4 x = *reinterpret_cast<const az_f32x4*>(out + row * 64 + (((lane & 15) ^ (row & 15)) * 4));
-      float v[4] = {x[0], x[1], x[2], x[3]};
-      if constexpr (SPLIT) {
-        for (int e = 0; e < 4; ++e)
-          if (!(fabsf(v[e]) < INFINITY) && m < p.M && n + e < p.N) {
-            float sum = 0.0f;
-            const int k1 = min(p.K, t1 * STEP);
-            for (int k = t0 * STEP; k < k1; ++k)
-              sum = fmaf(p.a32[AKC ? m * p.lda32 + k : k * p.lda32 + m],
-                         p.b32[BKC ? (n + e) * p.ldb32 + k : k * p.ldb32 + n + e], sum);
-            v[e] = sum;
-          }
+    // the residual of the next four rows is loaded while these four are worked on
+    constexpr int AHEAD = 4;
+    AzVec<TO, 4> next[AHEAD];
+    const bool early = EPI == EPI_FORWARD && p.residual && p.out_vec;
+    auto fetch = [&](int r0) {
+      if (!early) return;
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int m = m0 + wm + i0 * 16 + r0 + k * 4 + (lane >> 4);
+        if (m < p.M && n < p.N) next[k] = az_loadv<TO, 4>((const TO*)p.residual + (int64_t)m * p.N + n);
       }
-      finish<TO, EPI>(p, m, n, v);
+    };
+    fetch(0);
+#pragma unroll 1
+    for (int r0 = 0; r0 < ROUND * 16; r0 += 4 * AHEAD) {
+      AzVec<TO, 4> res[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) res[k] = next[k];
+      if (r0 + 4 * AHEAD < ROUND * 16) fetch(r0 + 4 * AHEAD);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int row = r0 + 4 * k + (lane >> 4), m = m0 + wm + i0 * 16 + row;
+        const az_f32x4 x = *reinterpret_cast<const az_f32x4*>(out + row * 64 + (((lane & 15) ^ (row & 15)) * 4));
+        float v[4] = {x[0], x[1], x[2], x[3]};
+        if constexpr (SPLIT) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(fabsf(v[e]) < INFINITY) && m < p.M && n + e < p.N) {
+              float sum = 0.0f;
+              const int k1 = min(p.K, t1 * STEP);
+              for (int j = t0 * STEP; j < k1; ++j)
+                sum = fmaf(p.a32[AKC ? m * p.lda32 + j : j * p.lda32 + m],
+                           p.b32[BKC ? (n + e) * p.ldb32 + j : j * p.ldb32 + n + e], sum);
+              v[e] = sum;
+            }
+        }
+        finish<TO, EPI>(p, m, n, v, early, res[k]);
+      }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();

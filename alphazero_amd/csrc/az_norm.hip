@@ -25,15 +25,26 @@ struct Norm {
   int rows, width;
 };
 
-// V elements of a row from column c; 0 beyond its end.
-template <typename T, int V>
-__device__ __forceinline__ void load_row(const T* row, int c, int width, float* v) {
-  if (c + V <= width) {
-    const AzVec<T, V> r = az_loadu<T, V>(row + c);
-    for (int i = 0; i < V; ++i) v[i] = (float)r.v[i];
+// V elements of a row from column c as they are, 0 beyond its end.  EXACT: the width is a multiple of V; the load
+// is then made by every thread, without a branch (behind which the compiler would wait for it).
+template <typename T, int V, bool EXACT>
+__device__ __forceinline__ AzVec<T, V> fetch_row(const T* row, int c, int width) {
+  AzVec<T, V> r;
+  if constexpr (EXACT) {
+    r = az_loadu<T, V>(row + (c < width ? c : 0));
+    for (int i = 0; i < V; ++i) r.v[i] = c < width ? r.v[i] : (T)0.0f;
+  } else if (c + V <= width) {
+    r = az_loadu<T, V>(row + c);
   } else {
-    for (int i = 0; i < V; ++i) v[i] = c + i < width ? (float)row[c + i] : 0.0f;
+    for (int i = 0; i < V; ++i) r.v[i] = c + i < width ? row[c + i] : (T)0.0f;
   }
+  return r;
+}
+
+template <typename T, int V, bool EXACT>
+__device__ __forceinline__ void load_row(const T* row, int c, int width, float* v) {
+  const AzVec<T, V> r = fetch_row<T, V, EXACT>(row, c, width);
+  for (int i = 0; i < V; ++i) v[i] = (float)r.v[i];
 }
 
 template <typename T, int V>
@@ -68,7 +79,7 @@ constexpr int vec_of() {
 }
 
 // NT threads a row, R 16-byte loads a thread; workgroups of max(NT, 256) threads.
-template <typename T, typename P, int NT, int R>
+template <typename T, typename P, int NT, int R, bool EXACT>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm_forward(Norm p) {
   constexpr int V = vec_of<T>(), ROWS = NT < 256 ? 256 / NT : 1;
   __shared__ float scratch[2][NT / 64];
@@ -79,7 +90,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm_forward(Norm p) {
   float v[R][V];
   float s = 0.0f;
   for (int r = 0; r < R; ++r) {
-    load_row<T, V>(x, (r * NT + t) * V, p.width, v[r]);
+    load_row<T, V, EXACT>(x, (r * NT + t) * V, p.width, v[r]);
     for (int i = 0; i < V; ++i) s += v[r][i];
   }
   const float mean = row_sum<NT>(s, scratch[0]) / p.width;
@@ -94,8 +105,8 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm_forward(Norm p) {
   for (int r = 0; r < R; ++r) {
     const int c = (r * NT + t) * V;
     float g[V], b[V];
-    if (p.scale) load_row<P, V>((const P*)p.scale, c, p.width, g);
-    if (p.bias) load_row<P, V>((const P*)p.bias, c, p.width, b);
+    if (p.scale) load_row<P, V, EXACT>((const P*)p.scale, c, p.width, g);
+    if (p.bias) load_row<P, V, EXACT>((const P*)p.bias, c, p.width, b);
     for (int i = 0; i < V; ++i) {
       float o = v[r][i] * rstd;
       if (p.scale) o *= g[i];
@@ -107,41 +118,65 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm_forward(Norm p) {
   if (t == 0 && p.mean) p.mean[m] = mean, p.rstd[m] = rstd;
 }
 
-template <typename T, typename P, int NT, int R>
+// A row's x and dy are loaded while the row before is worked on (not with 1024 threads a row, which have 128 registers
+// each).  16384 x 4096 bfloat16: 80 us, 402 MB; 138 us while the loads waited for each other and for the barriers.
+template <typename T, typename P, int NT, int R, bool EXACT>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm_backward(Norm p) {
   constexpr int V = vec_of<T>(), ROWS = NT < 256 ? 256 / NT : 1, W = NT * V * R;
-  __shared__ float scratch[4][NT / 64];
+  __shared__ float scratch[2][2 * (NT / 64)];
   __shared__ float joined[ROWS > 1 ? 2 * W : 1];
   const int t = threadIdx.x % NT, g = threadIdx.x / NT;
-  float ds[R][V] = {}, db[R][V] = {}, gain[R][V];
+  float ds[R][V] = {}, db[R][V] = {};
+  AzVec<P, V> gain[R];
   for (int r = 0; r < R; ++r) {
     if (p.scale)
-      load_row<P, V>((const P*)p.scale, (r * NT + t) * V, p.width, gain[r]);
+      gain[r] = fetch_row<P, V, EXACT>((const P*)p.scale, (r * NT + t) * V, p.width);
     else
-      for (int i = 0; i < V; ++i) gain[r][i] = 1.0f;
+      for (int i = 0; i < V; ++i) gain[r].v[i] = (P)1.0f;
   }
-  int phase = 0;
-  for (int m = blockIdx.x * ROWS + g; m < p.rows; m += gridDim.x * ROWS, phase ^= 2) {
+  AzVec<T, V> next_x[R], next_h[R];
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  auto fetch = [&](int m) {
+    m = min(m, p.rows - 1);   // (beyond the last row: loaded, not used)
     const int64_t at = (int64_t)m * p.width;
-    const float mean = p.mean[m], rstd = p.rstd[m];
-    float x[R][V], h[R][V], s1 = 0.0f, s2 = 0.0f;
+    next_mean = p.mean[m], next_rstd = p.rstd[m];
     for (int r = 0; r < R; ++r) {
-      load_row<T, V>((const T*)p.x + at, (r * NT + t) * V, p.width, x[r]);
-      load_row<T, V>((const T*)p.dy + at, (r * NT + t) * V, p.width, h[r]);
+      next_x[r] = fetch_row<T, V, EXACT>((const T*)p.x + at, (r * NT + t) * V, p.width);
+      next_h[r] = fetch_row<T, V, EXACT>((const T*)p.dy + at, (r * NT + t) * V, p.width);
     }
+  };
+  constexpr bool AHEAD = NT < 1024;
+  const int stride = gridDim.x * ROWS;
+  int phase = 0;
+  if (AHEAD) fetch(blockIdx.x * ROWS + g);
+  for (int64_t m64 = blockIdx.x * ROWS + g; m64 < p.rows; m64 += stride, phase ^= 1) {
+    const int m = (int)m64;
+    if (!AHEAD) fetch(m);
+    const float mean = next_mean, rstd = next_rstd;
+    float x[R][V], h[R][V], s1 = 0.0f, s2 = 0.0f;
+    for (int r = 0; r < R; ++r)
+      for (int i = 0; i < V; ++i) x[r][i] = (float)next_x[r].v[i], h[r][i] = (float)next_h[r].v[i];
+    if (AHEAD) fetch(m + stride);
     for (int r = 0; r < R; ++r)
       for (int i = 0; i < V; ++i) {
         x[r][i] = (x[r][i] - mean) * rstd;
         ds[r][i] += h[r][i] * x[r][i];
         db[r][i] += h[r][i];
-        h[r][i] *= gain[r][i];
+        h[r][i] *= (float)gain[r].v[i];
         s1 += h[r][i];          // (beyond the row's end h is 0)
         s2 += h[r][i] * x[r][i];
       }
     if (!p.out) continue;
-    // (two sets of scratch in turn: a set is written again only behind the other set's barrier)
-    s1 = row_sum<NT>(s1, scratch[phase]) / p.width;
-    s2 = row_sum<NT>(s2, scratch[phase + 1]) / p.width;
+    for (int off = 32; off > 0; off >>= 1) s1 += __shfl_xor(s1, off), s2 += __shfl_xor(s2, off);
+    if constexpr (NT > 64) {
+      // (two scratches in turn: one is written again only behind the other's barrier)
+      if ((t & 63) == 0) scratch[phase][2 * (t >> 6)] = s1, scratch[phase][2 * (t >> 6) + 1] = s2;
+      az_lds_barrier();
+      s1 = s2 = 0.0f;
+      for (int i = 0; i < NT / 64; ++i) s1 += scratch[phase][2 * i], s2 += scratch[phase][2 * i + 1];
+    }
+    s1 /= p.width, s2 /= p.width;
+    const int64_t at = (int64_t)m * p.width;
     for (int r = 0; r < R; ++r) {
       for (int i = 0; i < V; ++i) h[r][i] = rstd * (h[r][i] - s1 - x[r][i] * s2);
       store_row<T, V>((T*)p.out + at, (r * NT + t) * V, p.width, h[r]);
@@ -272,22 +307,28 @@ int backward_blocks(int64_t rows, int width) {
   return (int)(n < most ? n : most);
 }
 
-// Calls f.operator()<T, P, NT, R>() for the row's threads and loads.
+// Calls f.operator()<NT, R, EXACT>() for the row's threads and loads.
 template <typename T, typename P, typename F>
 void with_shape(int width, F&& f) {
   constexpr int V = vec_of<T>(), FULL = 16 / V;   // 16 elements a thread
   const int nt = threads_of(width);
+  auto with = [&]<int NT, int R>() {
+    if (width % V == 0)
+      f.template operator()<NT, R, true>();
+    else
+      f.template operator()<NT, R, false>();
+  };
   if (nt == 64) {
-    if (width <= 64 * V) return f.template operator()<64, 1>();
+    if (width <= 64 * V) return with.template operator()<64, 1>();
     if constexpr (FULL > 2)
-      if (width <= 128 * V) return f.template operator()<64, 2>();
-    return f.template operator()<64, FULL>();
+      if (width <= 128 * V) return with.template operator()<64, 2>();
+    return with.template operator()<64, FULL>();
   }
   if (nt == 256) {
-    if (width <= 256 * 2 * V && FULL > 2) return f.template operator()<256, 2>();
-    return f.template operator()<256, FULL>();
+    if (width <= 256 * 2 * V && FULL > 2) return with.template operator()<256, 2>();
+    return with.template operator()<256, FULL>();
   }
-  return f.template operator()<1024, FULL>();
+  return with.template operator()<1024, FULL>();
 }
 
 int check(int dtype, int param_dtype, int64_t rows, int64_t width) {
@@ -324,9 +365,9 @@ extern "C" int az_layer_norm_forward(int32_t dtype, int32_t param_dtype, int32_t
     if (width > IN_REGISTERS) {
       k_norm_forward_wide<T, P><<<dim3(rows), dim3(1024), 0, stream>>>(p);
     } else {
-      with_shape<T, P>(width, [&]<int NT, int R>() {
+      with_shape<T, P>(width, [&]<int NT, int R, bool EXACT>() {
         constexpr int ROWS = NT < 256 ? 256 / NT : 1;
-        k_norm_forward<T, P, NT, R><<<dim3((unsigned)az_ceil(rows, ROWS)), dim3(NT < 256 ? 256 : NT), 0, stream>>>(p);
+        k_norm_forward<T, P, NT, R, EXACT><<<dim3((unsigned)az_ceil(rows, ROWS)), dim3(NT < 256 ? 256 : NT), 0, stream>>>(p);
       });
     }
     AZ_LAUNCH_CHECK();
@@ -368,8 +409,8 @@ extern "C" int az_layer_norm_backward(int32_t dtype, int32_t param_dtype, int32_
       if (columns)
         k_norm_columns_wide<T><<<dim3((unsigned)az_ceil(width, 256), blocks), dim3(256), 0, stream>>>(p);
     } else {
-      with_shape<T, P>(width, [&]<int NT, int R>() {
-        k_norm_backward<T, P, NT, R><<<dim3(blocks), dim3(NT < 256 ? 256 : NT), 0, stream>>>(p);
+      with_shape<T, P>(width, [&]<int NT, int R, bool EXACT>() {
+        k_norm_backward<T, P, NT, R, EXACT><<<dim3(blocks), dim3(NT < 256 ? 256 : NT), 0, stream>>>(p);
       });
     }
     AZ_LAUNCH_CHECK();

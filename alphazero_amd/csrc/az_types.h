@@ -13,6 +13,14 @@ typedef __bf16 az_bf16;
 typedef _Float16 az_f16;
 typedef float az_f32x4 __attribute__((ext_vector_type(4)));
 
+// A workgroup barrier that orders LDS accesses alone: __syncthreads also waits for the global loads in flight, the
+// ones that run ahead among them.
+static __device__ __forceinline__ void az_lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // sixteen bytes of T
 template <typename T>
 struct alignas(16) AzPack {

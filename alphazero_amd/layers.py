@@ -40,6 +40,11 @@ def _checked(op, x, others):
         raise NotImplementedError(f"{op}: tensors must be on the GPU (there is no CPU path)")
 
 
+def _rows(x):
+    """x as contiguous [rows, width] (x itself where it is: a view would be a node of the autograd graph)."""
+    return (x if x.dim() == 2 else x.reshape(-1, x.shape[-1])).contiguous()
+
+
 # ---------------------------------------------------------------- dense
 def _dense_forward(x, kernel, bias, residual, act, keep_z):
     """(y, z): x [M, K] and residual [M, N] contiguous."""
@@ -113,10 +118,9 @@ def dense(x, kernel, bias=None, activation=None, residual=None):
             raise TypeError(f"dense: {name} is {t.dtype}, x {x.dtype}")
     _checked("dense", x, others)
     act = ACTIVATIONS[activation]
-    x2 = x.reshape(-1, kernel.shape[0]).contiguous()
+    x2, r2 = _rows(x), None if residual is None else _rows(residual)
     kernel = kernel.contiguous()
     bias = None if bias is None else bias.contiguous()
-    r2 = None if residual is None else residual.reshape(-1, shape[-1]).contiguous()
     if torch.is_grad_enabled() and (x2.requires_grad or kernel.requires_grad or
                                     (bias is not None and bias.requires_grad) or
                                     (r2 is not None and r2.requires_grad)):
@@ -192,7 +196,7 @@ def layer_norm(x, scale=None, bias=None, eps=1e-6):
     if not 0.0 <= eps < float("inf"):
         raise ValueError(f"layer_norm: eps {eps}")
     _checked("layer_norm", x, (("scale", scale), ("bias", bias)))
-    x2 = x.reshape(-1, D).contiguous()
+    x2 = _rows(x)
     scale = None if scale is None else scale.contiguous()
     bias = None if bias is None else bias.contiguous()
     if torch.is_grad_enabled() and (x2.requires_grad or (scale is not None and scale.requires_grad) or
