@@ -12,9 +12,9 @@ from .action_selection import (GumbelMuZeroExtraData, gumbel_muzero_interior_act
 from .base import (ChanceRecurrentFnOutput, DecisionRecurrentFnOutput, PolicyOutput, RecurrentFnOutput,
                    RootFnOutput, StochasticRecurrentState)
 from .layers import dense, layer_norm
-from .networks import FusedModel, FusedRecurrentFn, init_mlp
-from .policies import (actor_post, gumbel_muzero_policy, muzero_policy, sampled_muzero_policy,
-                       stochastic_muzero_policy)
+from .networks import FusedModel, FusedRecurrentFn, ResidualNetworks, init_mlp
+from .policies import (actor_post, gumbel_muzero_policy, muzero_policy, prior_policy,
+                       sampled_muzero_policy, stochastic_muzero_policy)
 from .qtransforms import (qtransform_by_min_max, qtransform_by_parent_and_siblings,
                           qtransform_completed_by_mix_value)
 from .search import InjectedRecurrentFn, search
@@ -37,4 +37,5 @@ __all__ = [
     "sampled_muzero_action_selection", "sampled_muzero_policy", "search",
     "ChanceRecurrentFnOutput", "DecisionRecurrentFnOutput", "StochasticRecurrentState",
     "stochastic_muzero_policy", "minatar", "dense", "layer_norm", "sample_actions",
+    "ResidualNetworks", "prior_policy",
 ]

@@ -13,6 +13,7 @@ import torch
 import torch.distributed as dist
 import torch.nn.functional as F
 
+from . import layers as layers_lib
 from . import prng
 
 
@@ -81,8 +82,14 @@ def mse_value_loss(values, targets):
     return (e * e * 0.5).squeeze()
 
 
-def mlp_apply(layers, x):
-    """networks/networks.py:25-48: Dense + swish on all but the last layer."""
+def mlp_apply(layers, x, native=False):
+    """networks/networks.py:25-48: Dense + swish on all but the last layer.
+    native: every layer is one layers.dense (one launch forward, four backward) instead of library
+    calls; the same sums in another order."""
+    if native:
+        for i, (w, b) in enumerate(layers):
+            x = layers_lib.dense(x, w, b, "swish" if i + 1 < len(layers) else None)
+        return x
     for i, (w, b) in enumerate(layers):
         x = x @ w + b
         if i + 1 < len(layers):
@@ -90,7 +97,7 @@ def mlp_apply(layers, x):
     return x
 
 
-def forward_networks(policy_layers, value_layers, mean, std, obs):
+def forward_networks(policy_layers, value_layers, mean, std, obs, native=False):
     """alphazero.py:208-216 (differentiable twin of FusedModel.forward).  With value_layers None,
     `policy_layers` is a networks object with forward(obs, mean, std) and leaves() of its own
     (the shared convolutional torso with its two heads, alphazero.py:246-267): the normaliser is
@@ -98,7 +105,7 @@ def forward_networks(policy_layers, value_layers, mean, std, obs):
     if value_layers is None:
         return policy_layers.forward(obs, mean, std)
     x = (obs - mean) / std
-    return mlp_apply(policy_layers, x), mlp_apply(value_layers, x)
+    return mlp_apply(policy_layers, x, native), mlp_apply(value_layers, x, native)
 
 
 # columns of a flat MCTSTransition row (envs/transition.py:18-34 in ravel order; extras is
@@ -143,13 +150,15 @@ def unpack_rows(layout, rows):
 
 
 def compute_muzero_loss(policy_layers, value_layers, mean, std, data, num_atoms, qr_kappa=1.0,
-                        vf_cost=0.5, l2_coef=1e-4, per_importance_sampling=True, l2_outside_graph=False):
+                        vf_cost=0.5, l2_coef=1e-4, per_importance_sampling=True, l2_outside_graph=False,
+                        native_dense=False):
     """alphazero.py:723-807 on a dict of batch fields; returns (total_loss, metrics).
     l2_outside_graph: the L2 penalty enters the reported losses only, computed without autograd
     in three launches; the caller adds its gradient, l2_coef * parameter, itself
     (minibatch_step) -- the differentiable form costs about a hundred launches of a few
-    microseconds per minibatch for the 22 parameter leaves."""
-    logits, baseline = forward_networks(policy_layers, value_layers, mean, std, data["observation"])
+    microseconds per minibatch for the 22 parameter leaves.
+    native_dense: the MLPs' layers run as layers.dense (mlp_apply)."""
+    logits, baseline = forward_networks(policy_layers, value_layers, mean, std, data["observation"], native_dense)
     lsm = F.log_softmax(logits, -1)
     policy_loss = -(data["target_policy_probs"].detach() * lsm).sum(-1).mean()
     vs = (data["value_prefix_target"].unsqueeze(-1) +

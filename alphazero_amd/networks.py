@@ -5,6 +5,8 @@ the last layer, lecun_uniform kernels, zero biases), alphazero.py:208-216
 (forward = normalise, policy MLP, value MLP) and alphazero.py:317-339 (the
 recurrent_fn = environment step + forward).  PyTorch only owns the parameter
 storage; every forward pass runs in the HIP kernels of libaz_mcts.so.
+`ResidualNetworks` (not in the reference) is a shared torso of pre-norm residual
+blocks with the two heads, on the layer operators of `layers`.
 """
 import math
 
@@ -13,6 +15,7 @@ import torch
 from . import _native as nat
 from . import base
 from . import envs as envs_lib
+from . import layers as layers_lib
 
 
 def init_mlp(layer_sizes, generator=None, device="cuda"):
@@ -140,3 +143,58 @@ class FusedRecurrentFn:
         out = base.RecurrentFnOutput(reward=reward, discount=discount, prior_logits=logits,
                                      value=value)
         return out, {"state": state, "time": time}
+
+
+class ResidualNetworks:
+    """A shared torso of `blocks` pre-norm residual blocks, `width` wide, and one dense layer each for the
+    policy logits and the value atoms:
+
+        h = dense(x);  per block  h = h + dense(swish(dense(layer_norm(h))));  heads on layer_norm(h)
+
+    Takes the networks' place in the learner's functions, as minatar.AtariNetworks does (forward(obs, mean,
+    std) and leaves()); observations [..., *obs_shape] or flattened.  Kernels are lecun_uniform (the second one of
+    a block scaled by 1 / sqrt(2 blocks)), biases zero, scales one.  dtype: of the parameters and the products
+    (float32, bfloat16 or float16); logits and value come back as float32."""
+
+    def __init__(self, obs_size, num_actions, num_atoms=1, width=256, blocks=2, hidden=None, generator=None,
+                 device="cuda", dtype=torch.float32):
+        hidden = width if hidden is None else int(hidden)
+        self.obs_size = int(obs_size)
+
+        def kernel(fan_in, fan_out, gain=1.0):
+            (w, b), = init_mlp((fan_in, fan_out), generator, device)
+            return (w * gain).to(dtype), b.to(dtype)
+
+        def norm():
+            return (torch.ones(width, device=device, dtype=dtype), torch.zeros(width, device=device, dtype=dtype))
+
+        self.inlet = kernel(self.obs_size, width)
+        self.blocks = [(norm(), kernel(width, hidden), kernel(hidden, width, (2 * blocks) ** -0.5))
+                       for _ in range(blocks)]
+        self.norm = norm()
+        self.policy = kernel(width, num_actions)
+        self.value = kernel(width, num_atoms)
+
+    def leaves(self):
+        pairs = [self.inlet] + [p for block in self.blocks for p in block] + [self.norm, self.policy, self.value]
+        return [t for p in pairs for t in p]
+
+    def forward(self, obs, mean=None, std=None):
+        """(prior logits [..., A], value [..., K]); mean / std: the running-statistics normaliser."""
+        if obs.shape[-1] != self.obs_size:
+            lead = obs.dim()
+            size = 1
+            while lead > 0 and size < self.obs_size:
+                lead -= 1
+                size *= obs.shape[lead]
+            if size != self.obs_size:
+                raise ValueError(f"observations {tuple(obs.shape)} do not hold {self.obs_size} values each")
+            obs = obs.reshape(tuple(obs.shape[:lead]) + (self.obs_size,))
+        if mean is not None:
+            obs = (obs - mean) / std
+        h = layers_lib.dense(obs.to(self.inlet[0].dtype), *self.inlet)
+        for norm, up, down in self.blocks:
+            u = layers_lib.dense(layers_lib.layer_norm(h, *norm), *up, activation="swish")
+            h = layers_lib.dense(u, *down, residual=h)
+        h = layers_lib.layer_norm(h, *self.norm)
+        return layers_lib.dense(h, *self.policy).float(), layers_lib.dense(h, *self.value).float()

@@ -284,6 +284,28 @@ def gumbel_muzero_policy(params, rng_key, root, recurrent_fn, num_simulations,
     return base.PolicyOutput(action=action, action_weights=weights, search_tree=search_tree)
 
 
+def prior_policy(params, rng_key, root, invalid_actions=None, *, temperature=1.0, top_k=0, top_p=1.0,
+                 min_p=0.0, uniform=None):
+    """Acts from the network's prior alone, without a search (not in the reference): a draw from the
+    truncated root logits (action_selection.sample_actions; temperature 0 takes the likeliest action).
+    The PolicyOutput has the prior's probabilities over the legal actions as action_weights and no
+    search_tree.  uniform [B] (optional) injects the random numbers; otherwise they are
+    jax.random.uniform's under rng_key."""
+    logits = root.prior_logits.detach()
+    if uniform is None:
+        uniform = torch.empty((logits.shape[0],), dtype=torch.int64, device=logits.device)
+        nat.check(nat.lib().az_random_sort_keys(_key_words(prng.as_key(rng_key)), logits.shape[0], nat.ptr(uniform),
+                                                nat.stream_ptr()))
+        # 32 random bits, of which jax's uniform takes the upper 23
+        uniform = ((uniform & 0xFFFFFFFF) >> 9).to(torch.float32) * 2.0 ** -23
+    action, _ = action_selection.sample_actions(logits, uniform, temperature, top_k, top_p, min_p, invalid_actions)
+    weights = logits.float()
+    if invalid_actions is not None:
+        weights = weights.masked_fill(invalid_actions != 0, -torch.inf)
+    weights = torch.nan_to_num(torch.softmax(weights, -1))   # (a row without a legal action: zeros)
+    return base.PolicyOutput(action=action, action_weights=weights, search_tree=None)
+
+
 def actor_post(search_tree, action_weights, sampled_action, prior_logits, deterministic=False):
     """alphazero.py:367-379: (actions, search_value, prior_log_prob) after a policy call."""
     d, tp = search_tree._desc_and_ptrs()

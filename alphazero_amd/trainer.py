@@ -72,6 +72,13 @@ class Config:
     # not in the reference: with one process the minibatch update (loss, gradient, clip + Adam)
     # is captured once in a HIP graph and replayed (learner.GraphedMinibatchStep)
     graph_sgd: bool = True
+    # not in the reference: the learner's MLP layers run as layers.dense instead of library calls
+    native_dense: bool = False
+    # not in the reference: the shared torso for Breakout-MinAtar, "conv" (alphazero.py:246-267) or
+    # "residual" (networks.ResidualNetworks on the flattened observation)
+    torso: str = "conv"
+    residual_width: int = 256
+    residual_blocks: int = 2
 
 
 class Trainer:
@@ -96,8 +103,14 @@ class Trainer:
             obs, act = minatar.OBS, minatar.ACTIONS
             self.stats = L.RunningStatistics(obs, device=self.device)
             # the learner's functions take the networks object in the policy slot (learner.forward_networks)
-            self.policy_layers = minatar.AtariNetworks(act, cfg.num_atoms, tuple(cfg.atari_dense_layer_sizes),
-                                                       generator=g, device=self.device)
+            if cfg.torso == "residual":
+                self.policy_layers = networks.ResidualNetworks(
+                    obs, act, cfg.num_atoms, cfg.residual_width, cfg.residual_blocks, generator=g, device=self.device)
+            elif cfg.torso == "conv":
+                self.policy_layers = minatar.AtariNetworks(act, cfg.num_atoms, tuple(cfg.atari_dense_layer_sizes),
+                                                           generator=g, device=self.device)
+            else:
+                raise ValueError(f"Config.torso {cfg.torso!r} is neither 'conv' nor 'residual'")
             self.value_layers = None
             self.model = None
             self.recurrent_fn = minatar.recurrent_fn(self.env, self.policy_layers, cfg.n_step_gamma,
@@ -250,10 +263,10 @@ class Trainer:
         batch = L.unpack_rows(self.layout, rows)
         metrics = []
         loss_kw = dict(qr_kappa=cfg.qr_kappa, vf_cost=cfg.vf_cost, l2_coef=cfg.l2_coef,
-                       per_importance_sampling=cfg.per_importance_sampling)
-        # (the torso's convolutions stay outside graph capture: eager minibatches for Breakout)
+                       per_importance_sampling=cfg.per_importance_sampling, native_dense=cfg.native_dense)
+        # (the torso's convolutions stay outside graph capture: eager minibatches for Breakout with them)
         if cfg.graph_sgd and self.world == 1 and self.device.type == "cuda" and self._graphed is None \
-                and not self.atari:
+                and not (self.atari and cfg.torso == "conv"):
             self._graphed = L.GraphedMinibatchStep(
                 self.policy_layers, self.value_layers, self.optimizer, self.layout,
                 rows.shape[0] // cfg.num_minibatches, cfg.num_atoms, self.device, **loss_kw)
@@ -261,10 +274,7 @@ class Trainer:
             metrics += L.sgd_step(self.policy_layers, self.value_layers, mean, std, batch,
                                   self.optimizer, cfg.num_atoms, cfg.num_minibatches,
                                   generator=self._perm_gen, rows=rows, layout=self.layout,
-                                  graphed=self._graphed, key=key_sgd,
-                                  qr_kappa=cfg.qr_kappa, vf_cost=cfg.vf_cost,
-                                  l2_coef=cfg.l2_coef,
-                                  per_importance_sampling=cfg.per_importance_sampling)
+                                  graphed=self._graphed, key=key_sgd, **loss_kw)
             if key_sgd is not None:
                 key_sgd = prng.split(key_sgd, 3)[0]   # the carry of sgd_step (:1076, :1089)
         # refresh the priorities of the sampled rows with the PRE-update networks (:1177-1180)
@@ -296,12 +306,23 @@ class Trainer:
             self._refresh_model()
         return steps
 
-    def evaluate(self, key=None, num_eval_envs=None, episode_length=None):
+    def prior_step(self, key, deterministic, state):
+        """An environment step without a search: actions from the networks' prior (policies.prior_policy), the
+        likeliest one if deterministic; the next state."""
+        _, _, key = prng.split(key, 3)   # as actor_step
+        logits, value = self._forward(state.obs)
+        root = RootFnOutput(prior_logits=logits, value=value, embedding=state.embedding)
+        out = policies.prior_policy((), key, root, temperature=0.0 if deterministic else 1.0)
+        return self.env.step(state, out.action)
+
+    def evaluate(self, key=None, num_eval_envs=None, episode_length=None, search=True):
         """alphazero.py:433-508 (Evaluator.run_evaluation) with the accumulation of EvalWrapper
         (envs/brax_wrappers.py:153-197): `num_eval_envs` fresh environments run one unroll of
         `episode_length` actor steps (greedy actions when Config.deterministic_eval); every lane
         adds up the rewards of its FIRST episode and records that episode's length.  Runs on
-        this rank's device only, like the reference's evaluator (process 0, one device)."""
+        this rank's device only, like the reference's evaluator (process 0, one device).
+        search=False plays the raw policy instead (prior_step): what the search adds to it is the
+        difference of the two."""
         cfg = self.cfg
         n = cfg.num_eval_envs if num_eval_envs is None else int(num_eval_envs)
         length = cfg.episode_length if episode_length is None else int(episode_length)
@@ -314,7 +335,10 @@ class Trainer:
         episode_steps = torch.zeros_like(st.reward)
         for _ in range(length):
             sub, key = prng.split(key, 2)                                # generate_unroll (:422)
-            st, _ = self.actor_step(sub, deterministic=cfg.deterministic_eval, state=st)
+            if search:
+                st, _ = self.actor_step(sub, deterministic=cfg.deterministic_eval, state=st)
+            else:
+                st = self.prior_step(sub, cfg.deterministic_eval, st)
             episode_steps = torch.where(active != 0, st.steps, episode_steps)
             episode_reward = episode_reward + st.reward * active
             active = active * (1 - st.done)

@@ -590,3 +590,138 @@ def test_two_calls_at_once_on_two_streams():
     torch.cuda.synchronize()
     for o in outs:
         assert torch.equal(o[0], want[0]) and torch.equal(o[1], want[1])
+
+
+# ---------------------------------------------------------------- the operators together, as the package uses them
+def plain_forward(nets, obs, mean=None, std=None):
+    """ResidualNetworks.forward in the leaves' type, by elementary operations."""
+    def norm(h, s, b):
+        d = h - h.mean(1, keepdim=True)
+        return d / ((d * d).mean(1, keepdim=True) + 1e-6).sqrt() * s + b
+    it = iter(nets)
+    obs = obs if mean is None else (obs - mean) / std
+    h = obs @ next(it) + next(it)
+    for _ in range((len(nets) - 8) // 6):
+        u = norm(h, next(it), next(it)) @ next(it) + next(it)
+        h = h + (u * torch.sigmoid(u)) @ next(it) + next(it)
+    h = norm(h, next(it), next(it))
+    return h @ next(it) + next(it), h @ next(it) + next(it)
+
+
+@pytest.mark.parametrize("T,tol", [(torch.float32, 2e-5), (torch.bfloat16, 0.06), (torch.float16, 0.008)], ids=str)
+def test_residual_networks_and_gradients(T, tol):
+    """Forward and gradients of a whole network against 64 bits.  Tolerances (of the tensors' norms): the network is
+    eleven layers deep and normalised, and an error travels on by the residual path unchanged; each layer adds some
+    half steps of its type (float32: sums of up to 400 terms), 11 layers x 2 directions x half a step, some
+    of them doubled by a slope: 22 x 2^-24 x 8, 22 x 2^-8 x 0.7, 22 x 2^-11 x 0.7."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    nets = mctx.ResidualNetworks(400, 3, num_atoms=5, width=192, blocks=3, generator=g, dtype=T)
+    leaves = [p.requires_grad_() for p in nets.leaves()]
+    obs = rand((130, 10, 10, 4), torch.float32, 1)
+    cl, cv = rand((130, 3), torch.float32, 2), rand((130, 5), torch.float32, 3)
+    logits, value = nets.forward(obs)
+    assert logits.dtype == value.dtype == torch.float32 and logits.shape == (130, 3) and value.shape == (130, 5)
+    grads = torch.autograd.grad((logits * cl).sum() + (value * cv).sum(), leaves)
+    ref = [p.detach().double().cpu().requires_grad_() for p in leaves]
+    rl, rv = plain_forward(ref, obs.to(T).double().cpu().reshape(130, 400))
+    rgrads = torch.autograd.grad((rl * cl.double().cpu()).sum() + (rv * cv.double().cpu()).sum(), ref)
+    for got, want in zip((logits, value) + grads, (rl, rv) + rgrads):
+        want = want.detach()
+        off = torch.linalg.vector_norm(got.detach().double().cpu() - want) / torch.linalg.vector_norm(want)
+        assert float(off) <= tol, (tuple(want.shape), float(off))
+
+
+def test_native_learner_step_against_library_calls():
+    """One minibatch update of the MLP learner with layers.dense and with library calls: the same losses and, up to
+    float32 sums in another order, the same gradients; the default is the library's."""
+    from alphazero_amd import learner as L
+    from alphazero_amd import networks
+    g = torch.Generator(device="cuda").manual_seed(3)
+    N, obs, A, K = 257, 6, 3, 4
+    layout = L.row_layout(obs, A, K)
+    rows = torch.rand((N, layout["_width"]), generator=g, device="cuda")
+    rows[:, layout["raw_action"][0]] = 1
+    data = L.unpack_rows(layout, rows)
+    mean, std = torch.zeros(obs, device="cuda"), torch.ones(obs, device="cuda")
+    pol = networks.init_mlp((obs, 64, 64, A), g)
+    val = networks.init_mlp((obs, 256, 256, 256, K), g)
+    leaves = [p.requires_grad_() for p in L.flat_leaves(pol, val)]
+    out = {}
+    for native in (False, True):
+        total, metrics = L.compute_muzero_loss(pol, val, mean, std, data, K, native_dense=native)
+        out[native] = (total, torch.autograd.grad(total, leaves))
+    # a loss is a mean of sums through 4 layers of up to 256 terms: 4 x 256 roundings at the very most
+    assert abs(float(out[True][0] - out[False][0])) <= 1024 * U * abs(float(out[False][0]))
+    for a, b in zip(out[True][1], out[False][1]):
+        # both sides' sums of up to 257 rows x 256 terms; 2e-5 of the norm is 300 half steps
+        assert float(torch.linalg.vector_norm(a - b)) <= 2e-5 * float(torch.linalg.vector_norm(b)) + 1e-9
+
+
+def test_prior_policy():
+    B, A = 64, 18
+    logits = rand((B, A), torch.float32, 1, 2.0)
+    inv = (torch.rand((B, A), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") < 0.3).float()
+    inv[5] = 1
+    root = mctx.RootFnOutput(prior_logits=logits, value=torch.zeros(B, device="cuda"), embedding=None)
+    out = mctx.prior_policy((), 7, root, invalid_actions=inv, temperature=0.0)
+    assert out.search_tree is None and out.action.dtype == torch.int32
+    masked = logits.masked_fill(inv != 0, -math.inf)
+    want = masked.argmax(1)
+    want[5] = 0
+    assert torch.equal(out.action.long(), want)
+    p = torch.nan_to_num(torch.softmax(masked.double(), 1))
+    assert bool(((out.action_weights.double() - p).abs() <= 64 * U * p + 1e-12).all()) and bool((p[5] == 0).all())
+    # the same key, the same draw; the random numbers are jax.random.uniform's
+    from alphazero_amd import prng
+    a, b = (mctx.prior_policy((), 7, root, top_p=0.9) for _ in range(2))
+    u = torch.from_numpy((prng.random_bits32(prng.as_key(7), B) >> 9).astype("float32")).cuda() * 2.0 ** -23
+    assert torch.equal(a.action, b.action)
+    assert torch.equal(a.action, mctx.sample_actions(logits, u, top_p=0.9)[0])
+
+
+@pytest.mark.parametrize("kw", [dict(env_id="CartPole-v1", native_dense=True),
+                                dict(env_id="Breakout-MinAtar", torso="residual", residual_width=64)],
+                         ids=["native_dense", "residual_torso"])
+@pytest.mark.parametrize("graph", [True, False], ids=["graph", "eager"])
+def test_trainer_runs_on_the_operators(kw, graph):
+    from alphazero_amd.trainer import Config, Trainer
+    cfg = Config(num_envs=32, unroll_length=4, num_simulations=8, policy="gumbel", use_gae=False, max_replay_size=512,
+                 min_replay_size=0, replay_buffer_batch_size=32, num_minibatches=4, value_hidden=(64, 64),
+                 policy_hidden=(32, 32), graph_sgd=graph, **kw)
+    tr = Trainer(cfg, device="cuda")
+    before = [p.clone() for p in tr.optimizer.params]
+    m = tr.train(3)
+    assert all(math.isfinite(v) for v in m.values()), m
+    assert (tr._graphed is not None) == graph
+    assert all(not torch.equal(a, b) for a, b in zip(before, tr.optimizer.params))
+    for search in (True, False):
+        ev = tr.evaluate(num_eval_envs=8, episode_length=6, search=search)
+        assert math.isfinite(ev["eval/episode_reward"]) and ev["eval/avg_episode_length"] > 0
+
+
+def test_graphed_learner_equals_the_eager_one():
+    """Captured minibatch updates on the operators, replayed, against eager ones on the same rows: bit by bit."""
+    from alphazero_amd import learner as L
+    obs, A, K, n = 400, 3, 1, 96
+    layout = L.row_layout(obs, A, K)
+    results = []
+    for graphed in (False, True):
+        g = torch.Generator(device="cuda").manual_seed(3)
+        nets = mctx.ResidualNetworks(obs, A, K, width=64, blocks=2, generator=g)
+        opt = L.ClipAdam(L.flat_leaves(nets, None), 1e-3, total_timesteps=100)
+        mean, std = torch.zeros(obs, device="cuda"), torch.ones(obs, device="cuda")
+        step = L.GraphedMinibatchStep(nets, None, opt, layout, n, K, "cuda") if graphed else None
+        losses = []
+        for i in range(5):
+            rows = torch.rand((n, layout["_width"]), generator=g, device="cuda")
+            rows[:, layout["raw_action"][0]] = 1
+            if graphed:
+                m = step(rows, mean, std)
+            else:
+                m = L.minibatch_step(nets, None, mean, std, L.unpack_rows(layout, rows), opt, K)
+            losses.append(float(m["total_loss"]))
+        results.append((losses, [p.detach().clone() for p in opt.params]))
+    # (the learning rate comes from the device in the graph: a float32 of the same double expression)
+    assert results[0][0] == pytest.approx(results[1][0], rel=1e-5)
+    for a, b in zip(results[0][1], results[1][1]):
+        assert torch.allclose(a, b, rtol=1e-5, atol=1e-6)

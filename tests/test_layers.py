@@ -131,3 +131,24 @@ def test_native_refusals():
     assert lib.az_sample_actions(C.byref(d), some, some, None) == -1
     d.rows = 0
     assert lib.az_sample_actions(C.byref(d), None, None, None) == 0
+
+
+def test_prior_policy_and_networks_refusals():
+    from alphazero_amd import networks, trainer
+    root = mctx.RootFnOutput(prior_logits=t(4, 3), value=t(4), embedding=None)
+    with pytest.raises(NotImplementedError):       # no CPU path
+        mctx.prior_policy((), 0, root, uniform=t(4))
+    with pytest.raises(ValueError):
+        mctx.prior_policy((), 0, root, uniform=t(3))
+    nets = networks.ResidualNetworks(12, 3, width=8, blocks=2, device="cpu")
+    assert len(nets.leaves()) == 2 + 2 * 6 + 2 + 2 + 2
+    with pytest.raises(ValueError):
+        nets.forward(t(4, 5))
+    with pytest.raises(ValueError):
+        nets.forward(t(3, 3, 5))                   # 15 values, not 12
+    with pytest.raises(NotImplementedError):
+        nets.forward(t(4, 3, 4))
+    with pytest.raises(ValueError):
+        trainer.Trainer(trainer.Config(env_id="Breakout-MinAtar", torso="transformer"), device="cpu")
+    # what the learner computes without the operators is what it computed before
+    assert trainer.Config().native_dense is False and trainer.Config().torso == "conv"
