@@ -12,7 +12,10 @@ import dataclasses
 import math
 from typing import Any
 
+import torch
+
 from . import _native as nat
+from . import layers
 from . import qtransforms as qt
 
 _MSG = ("action selection runs inside the search kernels; pass this function (or a "
@@ -124,35 +127,38 @@ def sample_actions(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     negative or NaN temperature counts as 0, top_k <= 0 as all, and top_p, min_p beyond [0, 1] as the nearer end).
     -inf and NaN logits are illegal; a row without a legal action gives action 0 and log_prob -inf.
     """
-    import torch
-    from . import layers
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"sample_actions: logits {tuple(logits.shape)} must be [B, A] with A >= 1")
     B, A = logits.shape
-    if logits.dtype not in layers.DTYPES:
+    code = layers.DTYPES.get(logits.dtype)
+    if code is None:
         raise TypeError(f"sample_actions: float32, bfloat16 or float16 logits, got {logits.dtype}")
-    if tuple(uniform.shape) != (B,) or uniform.dtype != torch.float32:
+    if uniform.shape != (B,) or uniform.dtype != torch.float32:
         raise ValueError(f"sample_actions: uniform must be float32 [{B}], got {uniform.dtype} {tuple(uniform.shape)}")
-    if invalid_actions is not None and tuple(invalid_actions.shape) != (B, A):
+    if invalid_actions is not None and invalid_actions.shape != (B, A):
         raise ValueError(f"sample_actions: invalid_actions {tuple(invalid_actions.shape)} must be {(B, A)}")
-    d = nat.SampleDesc(dtype=layers.DTYPES[logits.dtype], rows=B, actions=A)
+    d = nat.SampleDesc(code, B, A)
     keep = []
-    for name, value, dtype, ok in (
-            ("temperature", temperature, torch.float32, lambda v: 0.0 <= v < math.inf),
-            ("top_k", top_k, torch.int32, lambda v: 0 <= v < 2 ** 31 and v == int(v)),
-            ("top_p", top_p, torch.float32, lambda v: 0.0 <= v <= 1.0),
-            ("min_p", min_p, torch.float32, lambda v: 0.0 <= v <= 1.0)):
-        if torch.is_tensor(value) and value.dim() > 0:
-            if tuple(value.shape) != (B,):
+    values = (temperature, top_k, top_p, min_p)
+    if any(isinstance(v, torch.Tensor) for v in values):
+        values = list(values)
+        for i, (name, dtype) in enumerate((("temperature", torch.float32), ("top_k", torch.int32),
+                                           ("top_p", torch.float32), ("min_p", torch.float32))):
+            value = values[i]
+            if not isinstance(value, torch.Tensor) or value.dim() == 0:
+                continue
+            if value.shape != (B,):
                 raise ValueError(f"sample_actions: {name} {tuple(value.shape)} must be a number or [{B}]")
             if value.device != logits.device:
                 raise ValueError(f"sample_actions: {name} is on {value.device}, logits on {logits.device}")
             keep.append(value.to(dtype).contiguous())
             setattr(d, name + "_rows", keep[-1].data_ptr())
-        else:
-            if not ok(value):
-                raise ValueError(f"sample_actions: {name}={value}")
-            setattr(d, name, int(value) if name == "top_k" else float(value))
+            values[i] = 0
+    temperature, top_k, top_p, min_p = values
+    if not (0.0 <= temperature < math.inf and 0.0 <= top_p <= 1.0 and 0.0 <= min_p <= 1.0 and
+            0 <= top_k < 2 ** 31 and top_k == int(top_k)):
+        raise ValueError(f"sample_actions: temperature={temperature} top_k={top_k} top_p={top_p} min_p={min_p}")
+    d.temperature, d.top_k, d.top_p, d.min_p = temperature, int(top_k), top_p, min_p
     layers._checked("sample_actions", logits, (("uniform", uniform), ("invalid_actions", invalid_actions)))
     logits, uniform = logits.detach().contiguous(), uniform.contiguous()
     d.logits, d.uniform = logits.data_ptr(), uniform.data_ptr()

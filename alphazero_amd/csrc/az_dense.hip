@@ -111,6 +111,50 @@ __global__ __launch_bounds__(256) void k_product_tile(Prod p) {
 }
 
 // ---------------------------------------------------------------------------
+// Few outputs: 16 x 16 a workgroup, whose waves share the reduction (each takes every WAVES-th piece of 64 bytes) and
+// whose sums are added in the waves' order.  One launch where splitting over workgroups needs two; operands go straight
+// into registers, element by element where the reduction is not contiguous.
+constexpr int WAVES = 16;
+
+template <typename T, bool KC>
+__device__ __forceinline__ AzPack<T> piece(const T* p, int64_t ld, int rows, int K, int r, int k, bool vec) {
+  constexpr int E = AzPack<T>::N;
+  AzPack<T> x;
+  if constexpr (KC) {
+    const T* at = p + (int64_t)r * ld + k;
+    if (vec && r < rows && k + E <= K) return az_load16(at);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x.v[e] = r < rows && k + e < K ? at[e] : (T)0.0f;
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) x.v[e] = r < rows && k + e < K ? p[(int64_t)(k + e) * ld + r] : (T)0.0f;
+  }
+  return x;
+}
+
+template <typename T, bool AKC, bool BKC, int EPI>
+__global__ __launch_bounds__(WAVES * 64) void k_product_few(Prod p) {
+  constexpr int E = AzPack<T>::N;
+  __shared__ az_f32x4 sums[WAVES][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int m0 = (blockIdx.x % p.tiles_m) * 16, n0 = (blockIdx.x / p.tiles_m) * 16;
+  az_f32x4 acc = {};
+#pragma unroll 2
+  for (int k = wave * 4 * E; k < p.K; k += WAVES * 4 * E) {
+    const int at = k + (lane >> 4) * E;
+    const AzPack<T> a = piece<T, AKC>((const T*)p.a, p.lda, p.M, p.K, m0 + (lane & 15), at, p.a_vec);
+    const AzPack<T> b = piece<T, BKC>((const T*)p.b, p.ldb, p.N, p.K, n0 + (lane & 15), at, p.b_vec);
+    acc = mma(b, a, acc);
+  }
+  sums[wave][lane] = acc;
+  __syncthreads();
+  if (wave > 0) return;
+  for (int w = 1; w < WAVES; ++w) acc += sums[w][lane];
+  const float v[4] = {acc[0], acc[1], acc[2], acc[3]};
+  finish<T, EPI>(p, m0 + (lane & 15), n0 + (lane >> 4) * 4, v);
+}
+
+// ---------------------------------------------------------------------------
 // Joins split sums in the order of the splits.  Segment 0 (the product; few splits, many outputs) takes the epilogue,
 // 64 groups of four outputs a workgroup and its splits dealt to four threads; segment 1 (the bias' gradient; many
 // splits, few outputs) is stored as it is, 16 groups a workgroup and 16 threads each.
@@ -294,7 +338,7 @@ int64_t round64(int64_t n) { return (n + 63) & ~(int64_t)63; }
 
 // How one product C[M, N] over K runs.
 struct Plan {
-  bool wide, big;
+  bool wide, big, few;
   int splits;
 };
 
@@ -310,18 +354,25 @@ int64_t splits_for(int64_t tiles, int64_t want, int64_t K, int64_t least) {
 //   float32: 4096 x 1024 x 1024 83 / 114, 1024 x 1024 x 1024 38 / 40, 256 x 2048 x 2048 43 / 38
 // 256 x 256 tiles pay from one for each compute unit on: 16384 x 512 x 2048 59 against 62 with 128 x 128 (512 tiles),
 // its dx 57 against 37 (128 tiles).
-// in_place: a 16-bit operand need not be copied for the wide kernel.
-Plan plan_of(int dtype, int64_t M, int64_t N, int64_t K, bool in_place) {
+// Few outputs, up to 1024 tiles of 16 x 16, as long as the reduction is not too long for the waves of one workgroup
+// (k_product_few / the best other form): 64 x 256 x 256 float32 3.4 / 7.3, bfloat16 3.2 / 7.0, 512 x 512 x 512 float32
+// 9.4 / 12.2, 1 x 4096 x 4096 float32 20.7 / 35, bfloat16 dx 8.4 / 10.2 but y (whose second operand it reads element by
+// element) 23 / 11.
+// in_place: a 16-bit operand need not be copied for the wide kernel.  contiguous: operands with a contiguous reduction.
+Plan plan_of(int dtype, int64_t M, int64_t N, int64_t K, bool in_place, int contiguous) {
   Plan p = {};
   const double work = (double)M * N * K;
   const bool f32 = dtype == AZ_TYPE_F32;
-  p.wide = work >= (f32 ? 0x1p31 : in_place ? 0x1p25 : 0x1p29);
+  p.few = az_ceil(M, 16) * az_ceil(N, 16) <= 1024 &&
+          K <= (contiguous == 2 ? 4096 : contiguous == 1 ? (f32 ? 4096 : 2048) : 1024);
+  p.wide = !p.few && work >= (f32 ? 0x1p31 : in_place ? 0x1p25 : 0x1p29);
   int64_t s = 1;
-  if (!p.wide) {
-    // two workgroups a compute unit for a long reduction, one otherwise; a few tiles are split down to 32 steps
+  if (!p.few && !p.wide) {
+    // two workgroups a compute unit for a long reduction, one otherwise, of two steps at least; a few tiles are split
+    // further
     const int64_t tiles = az_ceil(M, TILE) * az_ceil(N, TILE);
-    s = splits_for(tiles, K >= 1024 ? 512 : 256, K, tiles <= 16 ? 32 : 128);
-  } else {
+    s = splits_for(tiles, K >= 1024 ? 512 : 256, K, tiles <= 16 ? 32 : f32 ? 128 : 256);
+  } else if (p.wide) {
     const int64_t large = az_ceil(M, 256) * az_ceil(N, 256), steps = f32 ? 6 * K : K;
     p.big = large >= 256;
     if (!p.big) {
@@ -357,7 +408,7 @@ int product(Prod p, const Plan& plan, float* partial, const Join* extra, hipStre
   p.b_vec = p.ldb % E == 0 && az_aligned16(p.b);
   auto four = [](const void* q) { return ((uintptr_t)q & (4 * sizeof(T) - 1)) == 0; };
   p.out_vec = p.N % 4 == 0 && four(p.out) && four(p.bias) && four(p.residual) && az_aligned16(p.z);
-  const int tile = !plan.wide ? TILE : plan.big ? 256 : 128;
+  const int tile = plan.wide ? (plan.big ? 256 : 128) : plan.few ? 16 : TILE;
   p.tiles_m = (int)az_ceil(p.M, tile), p.tiles_n = (int)az_ceil(p.N, tile);
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
   if (tiles > 0x7fffffff) return az_fail(AZ_ERR_UNSUPPORTED, "dense: too many output tiles");
@@ -368,6 +419,9 @@ int product(Prod p, const Plan& plan, float* partial, const Join* extra, hipStre
   if (splits > 1) q.partial = partial, q.out_vec = p.N % 4 == 0;
   if (plan.wide) {
     if (int rc = az_product_wide(dtype, pass, splits > 1, plan.big, &q, splits, stream)) return rc;
+  } else if (plan.few) {
+    k_product_few<T, AKC, BKC, EPI><<<dim3((unsigned)tiles), dim3(WAVES * 64), 0, stream>>>(q);
+    AZ_LAUNCH_CHECK();
   } else {
     const dim3 grid((unsigned)tiles, 1, splits), block(256);
     if (splits == 1)
@@ -407,11 +461,11 @@ Layout layout_of(int dtype, int64_t M, int64_t K, int64_t N, int pass) {
     return here;
   };
   if (pass == 0) {
-    l.y = plan_of(dtype, M, N, K, K % 64 == 0 && N % 8 == 0);
+    l.y = plan_of(dtype, M, N, K, K % 64 == 0 && N % 8 == 0, 1);
     if (l.y.wide) l.x = room(M * Kp * each), l.kernel = room(K * Np * each);
     if (l.y.splits > 1) l.partial = room(l.y.splits * M * N * 4);
   } else {
-    l.dx = plan_of(dtype, M, K, N, N % 64 == 0), l.dw = plan_of(dtype, K, N, M, K % 8 == 0 && N % 8 == 0);
+    l.dx = plan_of(dtype, M, K, N, N % 64 == 0, 2), l.dw = plan_of(dtype, K, N, M, K % 8 == 0 && N % 8 == 0, 0);
     l.chunks = slope_chunks(M, az_ceil(N, 64 * (N % 4 == 0 ? 4 : 1)));
     l.dz = room(M * Np * size_of(dtype));
     if (dtype == AZ_TYPE_F32 && (l.dx.wide || l.dw.wide)) l.dz_planes = room(M * Np * 6);

@@ -7,7 +7,8 @@
 // evenly, then over the order-preserving integer of the logit within the bin that holds the cut, until that bin is a
 // single logit.  Weights are summed as 64-bit integers: the order of the LDS atomics does not matter.
 //
-// Up to 1024 actions a wave takes a row, which it holds in LDS.  Beyond, a workgroup holds the row in registers (up to
+// Up to 1024 actions a wave takes a row, which it holds in LDS.  Of up to 128 candidates every one is compared with
+// every other: that gives each its place in the descending order and the weight ahead of it at once.  Beyond, a workgroup holds the row in registers (up to
 // 32768 actions; wider rows are read from L2 again), takes the first histogram over it, and moves the actions of the bins
 // up to the cut's, in index order, into a list in LDS; one wave ends the draw on the list while the
 // others make room for the next row.  A row whose list would not fit (ties, a flat distribution) is left to a second
@@ -214,10 +215,11 @@ struct Cut {
 struct Share {
   u64 m;
   int shift;
-  __device__ __forceinline__ explicit Share(double x) {
-    int e;
-    m = (u64)ldexp(frexp(x, &e), 53);
-    shift = x > 0.0 ? 53 - e : 53;
+  __device__ __forceinline__ explicit Share(double x) {   // (subnormal numbers count as 0)
+    const u64 bits = (u64)__double_as_longlong(x);
+    const int e = (int)(bits >> 52);
+    m = e ? (bits & 0xfffffffffffffull) | 1ull << 52 : 0;
+    shift = 1075 - e;
   }
   // n times it, rounded down or up
   __device__ __forceinline__ u64 of(u64 n, bool up) const {
@@ -429,6 +431,65 @@ __device__ __forceinline__ Result draw(const Row& row, Shared<Row::THREADS, NB>&
   return {at_sum(row, s, target_of(o.uniform, total), kept), (double)total / w.unit};
 }
 
+// The whole draw over at most FEW actions in LDS (their indices `at`, or their places), by one wave.
+constexpr int FEW = 128;
+
+__device__ __forceinline__ Result draw_few(const float* l, const int* at, int n, u64* scratch, const Weights& w,
+                                           const Options& o) {
+  constexpr int E = FEW / 64;
+  const int lane = threadIdx.x & 63;
+  u64* masses = scratch;                                        // [FEW]
+  uint32_t* keys = reinterpret_cast<uint32_t*>(scratch + FEW);  // [FEW]
+  uint32_t key[E], rank[E];
+  u64 m[E], ahead[E];
+  double x[E];
+  bool in[E];
+  for (int e = 0; e < E; ++e) {
+    const int i = e * 64 + lane;
+    const float v = i < n ? l[i] : -INFINITY;
+    in[e] = v > -INFINITY;
+    key[e] = key_of(v);
+    x[e] = in[e] ? w(v) : 0.0;
+    m[e] = w.whole(x[e]);
+    rank[e] = 0, ahead[e] = 0;
+    masses[i] = m[e], keys[i] = key[e];
+  }
+  sync<64>();
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) {
+    const uint32_t k = keys[j];
+    const u64 mass = masses[j];
+    for (int e = 0; e < E; ++e) {
+      const bool first = k > key[e] || (k == key[e] && j < e * 64 + lane);
+      rank[e] += first;
+      ahead[e] += first ? mass : 0;
+    }
+  }
+  u64 sum = 0;
+  for (int e = 0; e < E; ++e) {
+    in[e] = in[e] && (o.top_k <= 0 || rank[e] < (uint32_t)o.top_k);
+    sum += in[e] ? m[e] : 0;
+  }
+  u64 goal = o.goal;
+  if (o.top_p < 1.0 && !goal) {
+    goal = Share(o.top_p).of(wave_sum(sum), true);
+    if (goal == 0) goal = 1;
+  }
+  u64 scan[E], total = 0;
+  for (int e = 0; e < E; ++e) {
+    in[e] = in[e] && (o.top_p >= 1.0 || ahead[e] < goal) && x[e] >= o.min_p;
+    scan[e] = total + wave_scan(in[e] ? m[e] : 0);
+    total = (u64)__shfl((uint32_t)(scan[e] >> 32), 63) << 32 | (u64)(uint32_t)__shfl((uint32_t)scan[e], 63);
+  }
+  const u64 target = target_of(o.uniform, total);
+  int found = 0;
+  for (int e = E - 1; e >= 0; --e) {
+    const u64 over = __ballot(target < scan[e]);
+    if (over) found = e * 64 + __ffsll(over) - 1;
+  }
+  return {at ? at[found] : found, (double)total / w.unit};
+}
+
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ Options options_of(const az_sample_desc& d, int b, double* temperature) {
   Options o;
@@ -460,6 +521,13 @@ __device__ __forceinline__ void write_none(int b, int32_t* action, float* log_pr
   if (log_prob) log_prob[b] = -INFINITY;
 }
 
+// A logit that is at most that of every action in the bins up to `bound`, whatever the roundings of bin_of: taking the
+// actions from it on may take some of the next bin along, in which the draw over them finds the same cut.
+__device__ __forceinline__ float least_of(float top, float scale, int bound) {
+  const float reach = (float)(bound + 1) / scale * (1.0f + 0x1p-18f);
+  return fmaxf(top - reach - (fabsf(top) + reach) * 0x1p-20f, -FLT_MAX);   // (finite: above what stands for no action)
+}
+
 __device__ __forceinline__ float wave_max(float x) {
   for (int off = 32; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off));
   return x;
@@ -472,10 +540,12 @@ __global__ __launch_bounds__(64 * WAVES) void k_sample_wave(az_sample_desc d, in
   constexpr int V = 16 / sizeof(T), NB = 256;
   __shared__ Shared<64, NB> shared[WAVES];
   __shared__ float list[WAVES][MOST];
+  __shared__ float few[WAVES][FEW];
+  __shared__ int few_at[WAVES][FEW];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, b = blockIdx.x * WAVES + wave;
   if (b >= d.rows) return;
   double temperature;
-  const Options o = options_of(d, b, &temperature);
+  Options o = options_of(d, b, &temperature);
   MemoryRow<T, 64> memory;
   memory.init((const T*)d.logits + (int64_t)b * d.actions, d.invalid ? d.invalid + (int64_t)b * d.actions : nullptr,
               d.actions, (d.actions + 64 * V - 1) / (64 * V));
@@ -501,8 +571,48 @@ __global__ __launch_bounds__(64 * WAVES) void k_sample_wave(az_sample_desc d, in
     sync<64>();
   }
   const Weights w = {top, 1.0 / temperature, unit};
-  const ListRow row = {list[wave], nullptr, d.actions, (d.actions + 63) / 64};
-  const Result r = draw<NB>(row, shared[wave], w, o);
+  const float* l = list[wave];
+  Result r;
+  if (d.actions <= FEW) {
+    r = draw_few(l, nullptr, d.actions, shared[wave].bins, w, o);
+  } else {
+    const ListRow row = {l, nullptr, d.actions, (d.actions + 63) / 64};
+    Shared<64, NB>& s = shared[wave];
+    // the bin that holds the first cut, and the actions up to it (k_sample_group has the same, over more threads)
+    const float scale = w.scale(NB);
+    int bound = NB;
+    if (o.top_k > 0) {
+      clear(s);
+      each(row, [&](float x, int) { count<false>(s, bin_of(top, x, scale, NB), w, x); });
+      sync<64>();
+      find(s, 0, (u64)o.top_k, nullptr, 0);
+      bound = s.found;
+      if (bound >= NB - 1) bound = NB, o.top_k = 0;   // nothing that could be drawn is cut
+    }
+    if (bound == NB && o.top_p < 1.0) {
+      clear(s);
+      each(row, [&](float x, int) { count<true>(s, bin_of(top, x, scale, NB), w, x); });
+      sync<64>();
+      const Share share(o.top_p);
+      o.goal = find(s, 0, 0, &share, 0);
+      bound = s.found;
+    }
+    int n = FEW + 1;
+    if (bound < NB) {
+      const float least = least_of(top, scale, bound);
+      n = 0;
+      for (int c = 0; c < row.chunks; ++c) {
+        float x;
+        row.fetch(c, &x);
+        const u64 has = __ballot(x >= least);
+        const int to = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(has >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)has, 0));
+        if (x >= least && to < FEW) few[wave][to] = x, few_at[wave][to] = c * 64 + lane;
+        n += __popcll(has);
+      }
+      sync<64>();
+    }
+    r = n <= FEW ? draw_few(few[wave], few_at[wave], n, s.bins, w, o) : draw<NB>(row, s, w, o);
+  }
   if (lane == 0) write<T>(d, b, w, r, action, log_prob);
 }
 
@@ -633,11 +743,8 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
       o.goal = find(s, 0, 0, &share, 0);
       bound = s.found;
     }
-    // The actions up to that bin, in index order, into the list.  A few of the next bin may come with them (the draw
-    // over the list finds the same cut): one comparison an action, with a logit that is low enough whatever the
-    // roundings of bin_of.
-    const float reach = (float)(bound + 1) / scale * (1.0f + 0x1p-18f);
-    const float least = anew(fmaxf(top - reach - (fabsf(top) + reach) * 0x1p-20f, -FLT_MAX));   // (finite)
+    // the actions up to that bin, in index order, into the list
+    const float least = anew(least_of(top, scale, bound));
     int mine = 0;
     front.chunks(memory, [&](int, const float* l) {
 #pragma unroll
@@ -675,7 +782,7 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
     __syncthreads();
     if (wave > 0) return;
     const ListRow row = {list, list_at, n, (n + 63) / 64};
-    const Result r = draw<256>(row, s1, w, o);
+    const Result r = n <= FEW ? draw_few(list, list_at, n, s1.bins, w, o) : draw<256>(row, s1, w, o);
     if (lane == 0) write<T>(d, b, w, r, action, log_prob);
   }
 }

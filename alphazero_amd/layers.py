@@ -21,8 +21,9 @@ def _native(device, fn, *args):
     """Calls a native entry point on `device`, which it makes the current one (launches go to the current device's
     stream).  Tensor arguments are contiguous; they are passed as pointers."""
     args = [a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args]
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, _raw_stream(device.index) if _raw_stream is not None else nat.stream_ptr())
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index) if _raw_stream is not None else nat.stream_ptr())
     else:
         with torch.cuda.device(device):
             rc = fn(*args, nat.stream_ptr())
@@ -30,13 +31,19 @@ def _native(device, fn, *args):
         nat.check(rc)
 
 
-def _checked(op, x, others):
+def _checked(op, x, others, same_type=False):
+    """Refuses tensors of other types or devices than the kernels take."""
     if x.dtype not in DTYPES:
         raise TypeError(f"{op}: float32, bfloat16 or float16 tensors, got {x.dtype}")
+    at = x.get_device()
     for name, t in others:
-        if t is not None and t.device != x.device:
+        if t is None:
+            continue
+        if same_type and t.dtype != x.dtype:
+            raise TypeError(f"{op}: {name} is {t.dtype}, x {x.dtype}")
+        if t.get_device() != at or (at < 0 and t.device != x.device):
             raise ValueError(f"{op}: {name} is on {t.device}, x on {x.device}")
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise NotImplementedError(f"{op}: tensors must be on the GPU (there is no CPU path)")
 
 
@@ -52,17 +59,38 @@ def _dense_forward(x, kernel, bias, residual, act, keep_z):
     N = kernel.shape[1]
     code = DTYPES[x.dtype]
     lib = nat.lib()
-    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    y = x.new_empty((M, N))
     z = None
     if keep_z and act != nat.ACT_NONE:
         z = torch.empty((M, N), dtype=torch.float32 if x.dtype == torch.float32 else torch.float16, device=x.device)
     n = lib.az_dense_workspace_bytes(code, M, K, N, 0)
     if n < 0:
         nat.check(-2)
-    ws = torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
-    _native(x.device, lib.az_dense_forward, code, act, M, K, N, x, kernel, bias,
-            residual, y, z, ws, n)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    _native(x.device, lib.az_dense_forward, code, act, M, K, N, x, kernel, bias, residual, y, z, ws, n)
     return y, z
+
+
+def _dense_backward(ctx, dy):
+    x, kernel, z = ctx.saved_tensors
+    M, K = x.shape
+    N = kernel.shape[1]
+    need = ctx.needs_input_grad
+    dx = torch.empty_like(x) if need[0] else None
+    dkernel = torch.empty_like(kernel) if need[1] else None
+    dbias = x.new_empty(N) if need[2] else None
+    if need[0] or need[1] or need[2]:
+        g = dy.contiguous()
+        code = DTYPES[x.dtype]
+        lib = nat.lib()
+        n = lib.az_dense_workspace_bytes(code, M, K, N, 1)
+        ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+        _native(x.device, lib.az_dense_backward, code, ctx.act, M, K, N, x, kernel, z, g, dx, dkernel, dbias, ws, n)
+    return dx, dkernel, dbias, dy if need[3] else None, None
+
+
+# (the wrapper makes a second differentiation an error; it is only needed where one is being recorded)
+_dense_backward_once = torch.autograd.function.once_differentiable(_dense_backward)
 
 
 class _Dense(torch.autograd.Function):
@@ -74,24 +102,8 @@ class _Dense(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, kernel, z = ctx.saved_tensors
-        M, K = x.shape
-        N = kernel.shape[1]
-        need = ctx.needs_input_grad
-        dx = torch.empty_like(x) if need[0] else None
-        dkernel = torch.empty_like(kernel) if need[1] else None
-        dbias = x.new_empty(N) if need[2] else None
-        if need[0] or need[1] or need[2]:
-            g = dy.contiguous()
-            code = DTYPES[x.dtype]
-            lib = nat.lib()
-            n = lib.az_dense_workspace_bytes(code, M, K, N, 1)
-            ws = torch.empty(n, dtype=torch.uint8, device=x.device)
-            _native(x.device, lib.az_dense_backward, code, ctx.act, M, K, N, x, kernel, z,
-                    g, dx, dkernel, dbias, ws, n)
-        return dx, dkernel, dbias, dy if need[3] else None, None
+        return (_dense_backward_once if torch.is_grad_enabled() else _dense_backward)(ctx, dy)
 
 
 def dense(x, kernel, bias=None, activation=None, residual=None):
@@ -101,23 +113,13 @@ def dense(x, kernel, bias=None, activation=None, residual=None):
     (float32, bfloat16 or float16) on one GPU; strided tensors are copied first.
     activation: None, "relu", "swish" (z * sigmoid(z), networks/networks.py:25-48) or "gelu" (erf form).
     """
-    if activation not in ACTIVATIONS:
-        raise ValueError(f"dense: activation {activation!r} is not one of {list(ACTIVATIONS)}")
-    if kernel.dim() != 2 or x.dim() < 1 or x.shape[-1] != kernel.shape[0]:
-        raise ValueError(f"dense: x {tuple(x.shape)} and kernel {tuple(kernel.shape)} do not match")
-    shape = tuple(x.shape[:-1]) + (kernel.shape[1],)
-    if kernel.shape[0] < 1 or kernel.shape[1] < 1:
-        raise ValueError(f"dense: empty kernel {tuple(kernel.shape)}")
-    if bias is not None and tuple(bias.shape) != shape[-1:]:
-        raise ValueError(f"dense: bias {tuple(bias.shape)} does not match kernel {tuple(kernel.shape)}")
-    if residual is not None and tuple(residual.shape) != shape:
-        raise ValueError(f"dense: residual {tuple(residual.shape)} is not of the output's shape {shape}")
-    others = (("kernel", kernel), ("bias", bias), ("residual", residual))
-    for name, t in others:
-        if t is not None and t.dtype != x.dtype:
-            raise TypeError(f"dense: {name} is {t.dtype}, x {x.dtype}")
-    _checked("dense", x, others)
-    act = ACTIVATIONS[activation]
+    act = ACTIVATIONS.get(activation, -1)
+    N = kernel.shape[1] if kernel.dim() == 2 else 0
+    if act < 0 or N < 1 or x.dim() < 1 or x.shape[-1] != kernel.shape[0] or not x.shape[-1] or \
+            (bias is not None and bias.shape != (N,)) or \
+            (residual is not None and (residual.shape[-1:] != (N,) or residual.shape[:-1] != x.shape[:-1])):
+        _refuse_dense(x, kernel, bias, activation, residual)
+    _checked("dense", x, (("kernel", kernel), ("bias", bias), ("residual", residual)), True)
     x2, r2 = _rows(x), None if residual is None else _rows(residual)
     kernel = kernel.contiguous()
     bias = None if bias is None else bias.contiguous()
@@ -127,7 +129,20 @@ def dense(x, kernel, bias=None, activation=None, residual=None):
         y = _Dense.apply(x2, kernel, bias, r2, act)
     else:
         y, _ = _dense_forward(x2, kernel, bias, r2, act, False)
-    return y if x.dim() == 2 else y.view(shape)
+    return y if x.dim() == 2 else y.view(x.shape[:-1] + (N,))
+
+
+def _refuse_dense(x, kernel, bias, activation, residual):
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"dense: activation {activation!r} is not one of {list(ACTIVATIONS)}")
+    if kernel.dim() != 2 or x.dim() < 1 or x.shape[-1] != kernel.shape[0]:
+        raise ValueError(f"dense: x {tuple(x.shape)} and kernel {tuple(kernel.shape)} do not match")
+    if 0 in kernel.shape:
+        raise ValueError(f"dense: empty kernel {tuple(kernel.shape)}")
+    shape = tuple(x.shape[:-1]) + (kernel.shape[1],)
+    if bias is not None and tuple(bias.shape) != shape[-1:]:
+        raise ValueError(f"dense: bias {tuple(bias.shape)} does not match kernel {tuple(kernel.shape)}")
+    raise ValueError(f"dense: residual {tuple(residual.shape)} is not of the output's shape {shape}")
 
 
 # ---------------------------------------------------------------- layer norm
@@ -145,6 +160,26 @@ def _norm_forward(x, scale, bias, eps, keep):
     return y, mean, rstd
 
 
+def _norm_backward(ctx, dy):
+    x, scale, mean, rstd = ctx.saved_tensors
+    M, D = x.shape
+    need = ctx.needs_input_grad
+    code = DTYPES[x.dtype]
+    ptype = scale.dtype if scale is not None else ctx.bias_dtype or x.dtype
+    dx = torch.empty_like(x) if need[0] else None
+    dscale = torch.empty(D, dtype=ptype, device=x.device) if need[1] else None
+    dbias = torch.empty(D, dtype=ptype, device=x.device) if need[2] else None
+    lib = nat.lib()
+    n = lib.az_layer_norm_workspace_bytes(M, D) if need[1] or need[2] else 0
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    _native(x.device, lib.az_layer_norm_backward, code, DTYPES[ptype], M, D, x, scale, mean, rstd, dy.contiguous(), dx,
+            dscale, dbias, ws, n)
+    return dx, dscale, dbias, None
+
+
+_norm_backward_once = torch.autograd.function.once_differentiable(_norm_backward)
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, scale, bias, eps):
@@ -154,24 +189,8 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, scale, mean, rstd = ctx.saved_tensors
-        M, D = x.shape
-        need = ctx.needs_input_grad
-        code = DTYPES[x.dtype]
-        ptype = scale.dtype if scale is not None else ctx.bias_dtype or x.dtype
-        dx = torch.empty_like(x) if need[0] else None
-        dscale = torch.empty((D,), dtype=ptype, device=x.device) if need[1] else None
-        dbias = torch.empty((D,), dtype=ptype, device=x.device) if need[2] else None
-        g = dy.contiguous()
-        lib = nat.lib()
-        n = lib.az_layer_norm_workspace_bytes(M, D) if need[1] or need[2] else 0
-        ws = torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
-        _native(x.device, lib.az_layer_norm_backward, code, DTYPES[ptype], M, D, x, scale,
-                mean, rstd, g, dx, dscale, dbias, ws,
-                n)
-        return dx, dscale, dbias, None
+        return (_norm_backward_once if torch.is_grad_enabled() else _norm_backward)(ctx, dy)
 
 
 def layer_norm(x, scale=None, bias=None, eps=1e-6):
@@ -187,7 +206,7 @@ def layer_norm(x, scale=None, bias=None, eps=1e-6):
     for name, t in (("scale", scale), ("bias", bias)):
         if t is None:
             continue
-        if tuple(t.shape) != (D,):
+        if t.shape != (D,):
             raise ValueError(f"layer_norm: {name} {tuple(t.shape)} does not match x {tuple(x.shape)}")
         if t.dtype not in (x.dtype, torch.float32) or (ptype is not None and t.dtype != ptype):
             raise TypeError(f"layer_norm: scale and bias must share a type, x's ({x.dtype}) or float32")

@@ -23,6 +23,7 @@ import torch
 from . import _native as nat
 from . import action_selection
 from . import base
+from . import layers
 from . import prng
 from . import qtransforms
 from . import search as search_lib
@@ -293,9 +294,11 @@ def prior_policy(params, rng_key, root, invalid_actions=None, *, temperature=1.0
     jax.random.uniform's under rng_key."""
     logits = root.prior_logits.detach()
     if uniform is None:
-        uniform = torch.empty((logits.shape[0],), dtype=torch.int64, device=logits.device)
-        nat.check(nat.lib().az_random_sort_keys(_key_words(prng.as_key(rng_key)), logits.shape[0], nat.ptr(uniform),
-                                                nat.stream_ptr()))
+        layers._checked("prior_policy", logits, (("invalid_actions", invalid_actions),))
+        uniform = torch.zeros((logits.shape[0],), dtype=torch.int64, device=logits.device)
+        if uniform.shape[0]:
+            layers._native(logits.device, nat.lib().az_random_sort_keys, _key_words(prng.as_key(rng_key)),
+                           uniform.shape[0], uniform)
         # 32 random bits, of which jax's uniform takes the upper 23
         uniform = ((uniform & 0xFFFFFFFF) >> 9).to(torch.float32) * 2.0 ** -23
     action, _ = action_selection.sample_actions(logits, uniform, temperature, top_k, top_p, min_p, invalid_actions)

@@ -91,7 +91,8 @@ def check_dense(x, w, b, r, dy, act, y, grads):
 
 SIZES = [(1, 1, 1), (1, 64, 64), (2, 3, 5), (17, 33, 65), (64, 256, 256), (63, 100, 36), (65, 128, 129),
          (130, 72, 200), (257, 64, 8), (300, 520, 264), (1, 1000, 7), (5, 2048, 3), (1025, 40, 24), (256, 256, 256),
-         (512, 320, 384), (700, 192, 256)]
+         (512, 320, 384), (700, 192, 256), (1100, 72, 300), (1027, 131, 517), (600, 1500, 700), (500, 1001, 600),
+         (5000, 20, 100), (3, 5000, 40), (40, 3, 5000)]
 
 
 @pytest.mark.parametrize("M,K,N", SIZES)

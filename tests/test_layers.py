@@ -108,11 +108,11 @@ def test_native_refusals():
     assert dense(0, 9, 4, 4, 4, some, some, None, None, some, None, some, 1 << 30, None) == -1
     assert dense(0, 0, 4, 4, 4, None, some, None, None, some, None, some, 1 << 30, None) == -1
     assert dense(0, 0, 0, 4, 4, None, None, None, None, None, None, None, 0, None) == 0      # no rows
-    n = lib.az_dense_workspace_bytes(0, 1, 4096, 64, 0)
+    n = lib.az_dense_workspace_bytes(0, 256, 4096, 4096, 0)
     assert n > 0
-    assert dense(0, 0, 1, 4096, 64, some, some, None, None, some, None, some, n - 1, None) == -1
-    assert dense(0, 0, 1, 4096, 64, some, some, None, None, some, None, None, n, None) == -1
-    assert dense(0, 0, 1, 4096, 64, some, some, None, None, some, None, C.c_void_p(4100), n, None) == -1
+    assert dense(0, 0, 256, 4096, 4096, some, some, None, None, some, None, some, n - 1, None) == -1
+    assert dense(0, 0, 256, 4096, 4096, some, some, None, None, some, None, None, n, None) == -1
+    assert dense(0, 0, 256, 4096, 4096, some, some, None, None, some, None, C.c_void_p(4100), n, None) == -1
     back = lib.az_dense_backward
     assert back(0, 1, 4, 4, 4, some, some, None, some, some, some, some, some, 1 << 30, None) == -1   # z is missing
     assert back(0, 0, 4, 4, 4, None, some, None, some, some, some, some, some, 1 << 30, None) == -1
