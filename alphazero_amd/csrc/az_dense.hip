@@ -116,25 +116,31 @@ __global__ __launch_bounds__(256) void k_product_tile(Prod p) {
 // into registers, element by element where the reduction is not contiguous.
 constexpr int WAVES = 16;
 
-template <typename T, bool KC>
-__device__ __forceinline__ AzPack<T> piece(const T* p, int64_t ld, int rows, int K, int r, int k, bool vec) {
-  constexpr int E = AzPack<T>::N;
-  AzPack<T> x;
+// C: the type that the matrix instructions take, S: the operand's in memory.
+template <typename C, typename S, bool KC>
+__device__ __forceinline__ AzPack<C> piece(const S* p, int64_t ld, int rows, int K, int r, int k, bool vec) {
+  constexpr int E = AzPack<C>::N;
+  AzPack<C> x;
   if constexpr (KC) {
-    const T* at = p + (int64_t)r * ld + k;
-    if (vec && r < rows && k + E <= K) return az_load16(at);
+    const S* at = p + (int64_t)r * ld + k;
+    if (vec && r < rows && k + E <= K) {
+      const AzVec<S, E> v = az_loadv<S, E>(at);
 #pragma unroll
-    for (int e = 0; e < E; ++e) x.v[e] = r < rows && k + e < K ? at[e] : (T)0.0f;
+      for (int e = 0; e < E; ++e) x.v[e] = (C)v.v[e];
+      return x;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) x.v[e] = r < rows && k + e < K ? (C)at[e] : (C)0.0f;
   } else {
 #pragma unroll
-    for (int e = 0; e < E; ++e) x.v[e] = r < rows && k + e < K ? p[(int64_t)(k + e) * ld + r] : (T)0.0f;
+    for (int e = 0; e < E; ++e) x.v[e] = r < rows && k + e < K ? (C)p[(int64_t)(k + e) * ld + r] : (C)0.0f;
   }
   return x;
 }
 
-template <typename T, bool AKC, bool BKC, int EPI>
+template <typename C, typename SA, typename SB, typename TO, bool AKC, bool BKC, int EPI>
 __global__ __launch_bounds__(WAVES * 64) void k_product_few(Prod p) {
-  constexpr int E = AzPack<T>::N;
+  constexpr int E = AzPack<C>::N;
   __shared__ az_f32x4 sums[WAVES][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m0 = (blockIdx.x % p.tiles_m) * 16, n0 = (blockIdx.x / p.tiles_m) * 16;
@@ -142,8 +148,8 @@ __global__ __launch_bounds__(WAVES * 64) void k_product_few(Prod p) {
 #pragma unroll 2
   for (int k = wave * 4 * E; k < p.K; k += WAVES * 4 * E) {
     const int at = k + (lane >> 4) * E;
-    const AzPack<T> a = piece<T, AKC>((const T*)p.a, p.lda, p.M, p.K, m0 + (lane & 15), at, p.a_vec);
-    const AzPack<T> b = piece<T, BKC>((const T*)p.b, p.ldb, p.N, p.K, n0 + (lane & 15), at, p.b_vec);
+    const AzPack<C> a = piece<C, SA, AKC>((const SA*)p.a, p.lda, p.M, p.K, m0 + (lane & 15), at, p.a_vec);
+    const AzPack<C> b = piece<C, SB, BKC>((const SB*)p.b, p.ldb, p.N, p.K, n0 + (lane & 15), at, p.b_vec);
     acc = mma(b, a, acc);
   }
   sums[wave][lane] = acc;
@@ -151,7 +157,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_product_few(Prod p) {
   if (wave > 0) return;
   for (int w = 1; w < WAVES; ++w) acc += sums[w][lane];
   const float v[4] = {acc[0], acc[1], acc[2], acc[3]};
-  finish<T, EPI>(p, m0 + (lane & 15), n0 + (lane >> 4) * 4, v);
+  finish<TO, EPI>(p, m0 + (lane & 15), n0 + (lane >> 4) * 4, v);
 }
 
 // ---------------------------------------------------------------------------
@@ -230,6 +236,7 @@ struct Slope {
   const void* dy;
   const void* z;
   void* dz;            // may be null (no activation: dy itself is dz)
+  float* dz32;         // dz before the rounding, may be null
   az_bf16* planes;     // float32 only: dz as planes, may be null
   int64_t plane;
   float* partial;      // [chunks][N], may be null
@@ -245,7 +252,7 @@ __global__ __launch_bounds__(256) void k_slope(Slope p) {
   const int n = (blockIdx.x * 64 + g) * V;
   const int m_end = min(p.M, (int)(blockIdx.y + 1) * p.rows_per_chunk);
   float s[V] = {};
-  if (n < p.N || ((p.dz || p.planes) && n < p.ld)) {
+  if (n < p.N || ((p.dz || p.planes) && n < p.ld)) {   // (dz32: ld is N)
 #pragma unroll 2
     for (int m = blockIdx.y * p.rows_per_chunk + w; m < m_end; m += 4) {
       const int64_t at = (int64_t)m * p.N + n, to = (int64_t)m * p.ld + n;
@@ -258,6 +265,9 @@ __global__ __launch_bounds__(256) void k_slope(Slope p) {
           d[i] = p.act == AZ_ACT_NONE ? (float)dy.v[i] : (float)dy.v[i] * act_slope((float)z.v[i], p.act);
           s[i] += d[i];
         }
+      }
+      if (p.dz32) {
+        for (int i = 0; i < V; ++i) p.dz32[to + i] = d[i];
       }
       if (p.dz) {
         AzVec<T, V> o;
@@ -398,14 +408,20 @@ int check(int dtype, int act, int64_t rows, int64_t fan_in, int64_t fan_out) {
   return AZ_OK;
 }
 
-// One product (and, with `extra`, the join of the bias' gradient).  `partial` holds splits x M x N floats.
-template <typename T, bool AKC, bool BKC, int EPI>
+// 16-byte aligned rows, of S elements
+template <typename S>
+bool rows_aligned(const void* p, int64_t ld) {
+  return ld % AzPack<S>::N == 0 && az_aligned16(p);
+}
+
+// One product (and, with `extra`, the join of the bias' gradient).  `partial` holds splits x M x N floats.  SA, SB: the
+// operands' types where they are not T's (few outputs in float32 arithmetic).
+template <typename T, bool AKC, bool BKC, int EPI, typename SA = T, typename SB = T>
 int product(Prod p, const Plan& plan, float* partial, const Join* extra, hipStream_t stream) {
-  const int E = AzPack<T>::N;
   const int pass = EPI == EPI_FORWARD ? PASS_Y : AKC ? PASS_DX : PASS_DW;
   const int dtype = sizeof(T) == 4 ? AZ_TYPE_F32 : std::is_same_v<T, az_bf16> ? AZ_TYPE_BF16 : AZ_TYPE_F16;
-  p.a_vec = p.lda % E == 0 && az_aligned16(p.a);
-  p.b_vec = p.ldb % E == 0 && az_aligned16(p.b);
+  p.a_vec = rows_aligned<SA>(p.a, p.lda);
+  p.b_vec = rows_aligned<SB>(p.b, p.ldb);
   auto four = [](const void* q) { return ((uintptr_t)q & (4 * sizeof(T) - 1)) == 0; };
   p.out_vec = p.N % 4 == 0 && four(p.out) && four(p.bias) && four(p.residual) && az_aligned16(p.z);
   const int tile = plan.wide ? (plan.big ? 256 : 128) : plan.few ? 16 : TILE;
@@ -417,10 +433,13 @@ int product(Prod p, const Plan& plan, float* partial, const Join* extra, hipStre
   const int splits = (int)az_ceil(p.K, p.k_chunk);
   Prod q = p;
   if (splits > 1) q.partial = partial, q.out_vec = p.N % 4 == 0;
-  if (plan.wide) {
+  if constexpr (!std::is_same_v<SA, SB>) {
+    k_product_few<float, SA, SB, T, AKC, BKC, EPI><<<dim3((unsigned)tiles), dim3(WAVES * 64), 0, stream>>>(q);
+    AZ_LAUNCH_CHECK();
+  } else if (plan.wide) {
     if (int rc = az_product_wide(dtype, pass, splits > 1, plan.big, &q, splits, stream)) return rc;
   } else if (plan.few) {
-    k_product_few<T, AKC, BKC, EPI><<<dim3((unsigned)tiles), dim3(WAVES * 64), 0, stream>>>(q);
+    k_product_few<T, T, T, T, AKC, BKC, EPI><<<dim3((unsigned)tiles), dim3(WAVES * 64), 0, stream>>>(q);
     AZ_LAUNCH_CHECK();
   } else {
     const dim3 grid((unsigned)tiles, 1, splits), block(256);
@@ -447,6 +466,7 @@ int product(Prod p, const Plan& plan, float* partial, const Join* extra, hipStre
 // (always room for them), dz, the partial sums of the bias' gradient, the partial sums of a split product.
 struct Layout {
   Plan y, dx, dw;
+  bool whole;       // dz is not rounded to 16 bits
   int chunks;
   int64_t x, kernel, dz, dz_planes, bias, partial, total;
 };
@@ -466,8 +486,12 @@ Layout layout_of(int dtype, int64_t M, int64_t K, int64_t N, int pass) {
     if (l.y.splits > 1) l.partial = room(l.y.splits * M * N * 4);
   } else {
     l.dx = plan_of(dtype, M, K, N, N % 64 == 0, 2), l.dw = plan_of(dtype, K, N, M, K % 8 == 0 && N % 8 == 0, 0);
+    // Few values of dz would not average out what rounding them to 16 bits takes from the gradients' sums: they stay
+    // float32 (and the products over them, which cost next to nothing, run in float32).
+    l.whole = dtype != AZ_TYPE_F32 && (M * N <= 512 || (M * N <= 16384 && l.dx.few && l.dw.few));
+    if (l.whole) l.dx = l.dw = Plan{false, false, true, 1};
     l.chunks = slope_chunks(M, az_ceil(N, 64 * (N % 4 == 0 ? 4 : 1)));
-    l.dz = room(M * Np * size_of(dtype));
+    l.dz = room(M * Np * (l.whole ? 4 : size_of(dtype)));
     if (dtype == AZ_TYPE_F32 && (l.dx.wide || l.dw.wide)) l.dz_planes = room(M * Np * 6);
     l.bias = room((int64_t)l.chunks * N * 4);
     if (l.dw.wide) l.x = room(M * Kp * each);
@@ -574,9 +598,10 @@ extern "C" int az_dense_backward(int32_t dtype, int32_t act, int32_t rows, int32
     Source sdz = {dy, fan_out, 0}, sdzw = sdz;
     if (copy) sdz = sdzw = {ws + l.dz, ld, 0};
     if (F32 && wide) sdzw = {ws + l.dz_planes, ld, rows * ld};
+    const bool whole = l.whole && copy;   // (without an activation dz is dy, which has 16 bits)
     if (copy || dbias || (F32 && wide)) {
       Slope s = {};
-      s.dy = dy, s.z = z, s.dz = copy ? ws + l.dz : nullptr;
+      s.dy = dy, s.z = z, s.dz = copy && !whole ? ws + l.dz : nullptr, s.dz32 = whole ? (float*)(ws + l.dz) : nullptr;
       if (F32 && wide) s.planes = (az_bf16*)(ws + l.dz_planes), s.plane = rows * ld;
       s.partial = dbias ? (float*)(ws + l.bias) : nullptr;
       s.M = rows, s.N = fan_out, s.act = act, s.rows_per_chunk = (int)az_ceil(rows, l.chunks), s.ld = (int)ld;
@@ -601,7 +626,9 @@ extern "C" int az_dense_backward(int32_t dtype, int32_t act, int32_t rows, int32
       operand_a(p, wide_dx ? sdzw : sdz, dz32, ld32);
       operand_b(p, sk, kernel, fan_out);
       p.M = rows, p.N = fan_in, p.K = fan_out, p.out = dx;
-      if (int rc = product<T, true, true, EPI_STORE>(p, l.dx, partial, nullptr, stream)) return rc;
+      if (int rc = whole ? product<T, true, true, EPI_STORE, float, T>(p, l.dx, partial, nullptr, stream)
+                         : product<T, true, true, EPI_STORE>(p, l.dx, partial, nullptr, stream))
+        return rc;
     }
     Join j = {};
     j.part[1] = (const float*)(ws + l.bias), j.length[1] = fan_out, j.splits[1] = l.chunks, j.out1 = dbias;
@@ -613,7 +640,8 @@ extern "C" int az_dense_backward(int32_t dtype, int32_t act, int32_t rows, int32
       operand_a(p, sx, x, fan_in);
       operand_b(p, wide_dw ? sdzw : sdz, dz32, ld32);
       p.M = fan_in, p.N = fan_out, p.K = rows, p.out = dkernel;
-      return product<T, false, false, EPI_STORE>(p, l.dw, partial, dbias ? &j : nullptr, stream);
+      return whole ? product<T, false, false, EPI_STORE, T, float>(p, l.dw, partial, dbias ? &j : nullptr, stream)
+                   : product<T, false, false, EPI_STORE>(p, l.dw, partial, dbias ? &j : nullptr, stream);
     }
     if (dbias) {
       k_join<T, EPI_STORE><<<dim3((unsigned)az_ceil(fan_out, 64)), dim3(256), 0, stream>>>(j, Prod{});
