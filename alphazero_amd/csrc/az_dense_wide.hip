@@ -163,45 +163,70 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product_wide(Prod p) {
     b.load(t, pb, lds_at + buf * STAGE + OpA::BYTES, wave);
   };
   az_f32x4 acc[FM][FN] = {};
-  load(0, 0);
-  for (int s = 0; s < stages; ++s) {
-    const int buf = s & 1;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();   // this stage is in LDS, and the other buffer's readers are done
-    if (s + 1 < stages) load(s + 1, buf ^ 1);
-    const char* la = lds + buf * STAGE;
-    const char* lb = la + OpA::BYTES;
+  // Two sets of fragments: while one half of a stage is multiplied, the next half (of this stage, or of the next one
+  // behind the barrier) is read.
+  uint4 fa[2][FM], fb[2][FN];
+  auto read = [&](int s, int sub) {
+    const char* la = lds + (s & 1) * STAGE;
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-      uint4 fa[FM], fb[FN];
+    for (int j = 0; j < FN; ++j) fb[sub][j] = fragment<BKC, BN>(la + OpA::BYTES, wn + j * 16, sub, lane);
 #pragma unroll
-      for (int j = 0; j < FN; ++j) fb[j] = fragment<BKC, BN>(lb, wn + j * 16, sub, lane);
+    for (int i = 0; i < FM; ++i) fa[sub][i] = fragment<AKC, BM>(la, wm + i * 16, sub, lane);
+  };
+  auto multiply = [&](int sub) {
 #pragma unroll
-      for (int i = 0; i < FM; ++i) fa[i] = fragment<AKC, BM>(la, wm + i * 16, sub, lane);
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
+      for (int j = 0; j < FN; ++j) acc[i][j] = mma16<T>(fb[sub][j], fa[sub][i], acc[i][j]);
+  };
+  // one LDS read, then its share of the matrix instructions: left to itself the compiler puts each read in front of its
+  // use and waits for it (16384 x 4096 x 4096, three products and the rest of a step: 1.52 ms, 1.46 ms this way)
+  auto interleave = [&] {
+    constexpr int READS = FM * (AKC ? 1 : 2) + FN * (BKC ? 1 : 2), PER = FM * FN / READS;
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = mma16<T>(fb[j], fa[i], acc[i][j]);
+    for (int i = 0; i < READS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, PER, 0);
     }
+    __builtin_amdgcn_sched_group_barrier(0x8, FM * FN - READS * PER, 0);
+  };
+  load(0, 0);
+  if (stages > 1) load(1, 1);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  read(0, 0);
+  for (int s = 0; s < stages; ++s) {
+    read(s, 1);
+    multiply(0);
+    interleave();
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();   // the next stage is in LDS, and this one's readers are done
+    if (s + 2 < stages) load(s + 2, s & 1);
+    read(s + 1, 0);    // (behind the last stage: read, not used)
+    multiply(1);
+    interleave();
+    __builtin_amdgcn_sched_barrier(0);
   }
   // The outputs leave through LDS, 64 rows of a wave at a time, so that a row's columns are written together; the
   // sixteen groups of four columns are exchanged by the row, which spreads the rows over the banks.
   constexpr int ROUND = 4;
-  static_assert(FN == 4 && FM % ROUND == 0 && NW * ROUND * 16 * 64 * 4 <= 2 * STAGE);
+  static_assert(FN % 4 == 0 && FM % ROUND == 0 && NW * ROUND * 16 * 64 * 4 <= 2 * STAGE);
   float* out = reinterpret_cast<float*>(lds) + wave * (ROUND * 16 * 64);
   __syncthreads();
 #pragma unroll
-  for (int i0 = 0; i0 < FM; i0 += ROUND) {
+  for (int part = 0; part < FM / ROUND * (FN / 4); ++part) {
+    const int i0 = part / (FN / 4) * ROUND, j0 = part % (FN / 4) * 4;
 #pragma unroll
     for (int i = 0; i < ROUND; ++i)
 #pragma unroll
-      for (int j = 0; j < FN; ++j) {
+      for (int j = 0; j < 4; ++j) {
         const int row = i * 16 + (lane & 15), quad = j * 4 + (lane >> 4);
-        *reinterpret_cast<az_f32x4*>(out + row * 64 + ((quad ^ (row & 15)) * 4)) = acc[i0 + i][j];
+        *reinterpret_cast<az_f32x4*>(out + row * 64 + ((quad ^ (row & 15)) * 4)) = acc[i0 + i][j0 + j];
       }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
-    const int n = n0 + wn + (lane & 15) * 4;
+    const int n = n0 + wn + j0 * 16 + (lane & 15) * 4;
     // the residual of the next four rows is loaded while these four are worked on
     constexpr int AHEAD = 4;
     AzVec<TO, 4> next[AHEAD];
