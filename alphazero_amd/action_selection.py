@@ -130,6 +130,8 @@ def sample_actions(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"sample_actions: logits {tuple(logits.shape)} must be [B, A] with A >= 1")
     B, A = logits.shape
+    if B > layers.MAX_ROWS or A > layers.MAX_ROWS:
+        raise NotImplementedError(f"sample_actions: logits {tuple(logits.shape)}")
     code = layers.DTYPES.get(logits.dtype)
     if code is None:
         raise TypeError(f"sample_actions: float32, bfloat16 or float16 logits, got {logits.dtype}")

@@ -327,8 +327,7 @@ __global__ __launch_bounds__(256) void k_pack(const T* src, int rows, int cols, 
 
 template <typename T>
 __global__ void k_zero(T* p, int64_t n) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i < n) p[i] = (T)0.0f;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) p[i] = (T)0.0f;
 }
 
 // ---------------------------------------------------------------------------
@@ -427,7 +426,8 @@ int product(Prod p, const Plan& plan, float* partial, const Join* extra, hipStre
   const int tile = plan.wide ? (plan.big ? 256 : 128) : plan.few ? 16 : TILE;
   p.tiles_m = (int)az_ceil(p.M, tile), p.tiles_n = (int)az_ceil(p.N, tile);
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-  if (tiles > 0x7fffffff) return az_fail(AZ_ERR_UNSUPPORTED, "dense: too many output tiles");
+  if (!az_grid_fits(tiles, plan.few ? WAVES * 64 : 512) || !az_grid_fits(az_ceil((int64_t)p.M * p.N, 256), 256))
+    return az_fail(AZ_ERR_UNSUPPORTED, "dense: %d x %d outputs are too many for one launch", p.M, p.N);
   const int step = plan.wide ? 64 : Stage<T, true>::BK;
   p.k_chunk = (int)(az_ceil(az_ceil(p.K, plan.splits), step) * step);
   const int splits = (int)az_ceil(p.K, p.k_chunk);
@@ -517,7 +517,7 @@ int source(const void* src, int64_t rows, int64_t cols, bool along, void* to, hi
     return AZ_OK;
   }
   const int64_t ld = round64(cols), threads = rows * (ld / 8);
-  if (az_ceil(threads, 256) > 0x7fffffff) return az_fail(AZ_ERR_UNSUPPORTED, "dense: operand too large");
+  if (!az_grid_fits(az_ceil(threads, 256), 256)) return az_fail(AZ_ERR_UNSUPPORTED, "dense: operand too large");
   *out = {to, ld, rows * ld};
   k_pack<T><<<dim3((unsigned)az_ceil(threads, 256)), dim3(256), 0, stream>>>((const T*)src, (int)rows, (int)cols,
                                                                              (int)ld, to, rows * ld);
@@ -576,7 +576,7 @@ extern "C" int az_dense_backward(int32_t dtype, int32_t act, int32_t rows, int32
   return az_dispatch_type(dtype, [&]<typename T>() -> int {
     if (rows == 0) {
       const int64_t n = (int64_t)fan_in * fan_out;
-      if (dkernel) k_zero<T><<<dim3((unsigned)az_ceil(n, 256)), dim3(256), 0, stream>>>((T*)dkernel, n);
+      if (dkernel) k_zero<T><<<dim3((unsigned)(n < 1 << 20 ? az_ceil(n, 256) : 4096)), dim3(256), 0, stream>>>((T*)dkernel, n);
       if (dbias) k_zero<T><<<dim3((unsigned)az_ceil(fan_out, 256)), dim3(256), 0, stream>>>((T*)dbias, fan_out);
       AZ_LAUNCH_CHECK();
       return AZ_OK;

@@ -82,40 +82,40 @@ constexpr int vec_of() {
 template <typename T, typename P, int NT, int R, bool EXACT>
 __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm_forward(Norm p) {
   constexpr int V = vec_of<T>(), ROWS = NT < 256 ? 256 / NT : 1;
-  __shared__ float scratch[2][NT / 64];
+  __shared__ float scratch[2][NT / 64];   // (each is written again behind the other's barrier)
   const int t = threadIdx.x % NT;
-  const int m = blockIdx.x * ROWS + threadIdx.x / NT;
-  if (m >= p.rows) return;   // (whole waves; with NT > 64 a workgroup has one row)
-  const T* x = (const T*)p.x + (int64_t)m * p.width;
-  float v[R][V];
-  float s = 0.0f;
-  for (int r = 0; r < R; ++r) {
-    load_row<T, V, EXACT>(x, (r * NT + t) * V, p.width, v[r]);
-    for (int i = 0; i < V; ++i) s += v[r][i];
-  }
-  const float mean = row_sum<NT>(s, scratch[0]) / p.width;
-  s = 0.0f;
-  for (int r = 0; r < R; ++r)
-    for (int i = 0; i < V; ++i) {
-      v[r][i] -= mean;
-      if ((r * NT + t) * V + i < p.width) s += v[r][i] * v[r][i];
+  for (int64_t m = (int64_t)blockIdx.x * ROWS + threadIdx.x / NT; m < p.rows; m += (int64_t)gridDim.x * ROWS) {
+    const T* x = (const T*)p.x + m * p.width;
+    float v[R][V];
+    float s = 0.0f;
+    for (int r = 0; r < R; ++r) {
+      load_row<T, V, EXACT>(x, (r * NT + t) * V, p.width, v[r]);
+      for (int i = 0; i < V; ++i) s += v[r][i];
     }
-  const float rstd = 1.0f / sqrtf(row_sum<NT>(s, scratch[1]) / p.width + p.eps);
-  T* y = (T*)p.out + (int64_t)m * p.width;
-  for (int r = 0; r < R; ++r) {
-    const int c = (r * NT + t) * V;
-    float g[V], b[V];
-    if (p.scale) load_row<P, V, EXACT>((const P*)p.scale, c, p.width, g);
-    if (p.bias) load_row<P, V, EXACT>((const P*)p.bias, c, p.width, b);
-    for (int i = 0; i < V; ++i) {
-      float o = v[r][i] * rstd;
-      if (p.scale) o *= g[i];
-      if (p.bias) o += b[i];
-      v[r][i] = o;
+    const float mean = row_sum<NT>(s, scratch[0]) / p.width;
+    s = 0.0f;
+    for (int r = 0; r < R; ++r)
+      for (int i = 0; i < V; ++i) {
+        v[r][i] -= mean;
+        if ((r * NT + t) * V + i < p.width) s += v[r][i] * v[r][i];
+      }
+    const float rstd = 1.0f / sqrtf(row_sum<NT>(s, scratch[1]) / p.width + p.eps);
+    T* y = (T*)p.out + m * p.width;
+    for (int r = 0; r < R; ++r) {
+      const int c = (r * NT + t) * V;
+      float g[V], b[V];
+      if (p.scale) load_row<P, V, EXACT>((const P*)p.scale, c, p.width, g);
+      if (p.bias) load_row<P, V, EXACT>((const P*)p.bias, c, p.width, b);
+      for (int i = 0; i < V; ++i) {
+        float o = v[r][i] * rstd;
+        if (p.scale) o *= g[i];
+        if (p.bias) o += b[i];
+        v[r][i] = o;
+      }
+      store_row<T, V>(y, c, p.width, v[r]);
     }
-    store_row<T, V>(y, c, p.width, v[r]);
+    if (t == 0 && p.mean) p.mean[m] = mean, p.rstd[m] = rstd;
   }
-  if (t == 0 && p.mean) p.mean[m] = mean, p.rstd[m] = rstd;
 }
 
 // A row's x and dy are loaded while the row before is worked on (not with 1024 threads a row, which have 128 registers
@@ -209,46 +209,50 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_norm_backward(Norm p) {
 template <typename T, typename P>
 __global__ __launch_bounds__(1024) void k_norm_forward_wide(Norm p) {
   __shared__ float scratch[2][16];
-  const int64_t at = (int64_t)blockIdx.x * p.width;
-  const T* x = (const T*)p.x + at;
-  float s = 0.0f;
-  for (int c = threadIdx.x; c < p.width; c += 1024) s += (float)x[c];
-  const float mean = row_sum<1024>(s, scratch[0]) / p.width;
-  s = 0.0f;
-  for (int c = threadIdx.x; c < p.width; c += 1024) {
-    const float d = (float)x[c] - mean;
-    s += d * d;
+  for (int64_t m = blockIdx.x; m < p.rows; m += gridDim.x) {
+    const int64_t at = m * p.width;
+    const T* x = (const T*)p.x + at;
+    float s = 0.0f;
+    for (int c = threadIdx.x; c < p.width; c += 1024) s += (float)x[c];
+    const float mean = row_sum<1024>(s, scratch[0]) / p.width;
+    s = 0.0f;
+    for (int c = threadIdx.x; c < p.width; c += 1024) {
+      const float d = (float)x[c] - mean;
+      s += d * d;
+    }
+    const float rstd = 1.0f / sqrtf(row_sum<1024>(s, scratch[1]) / p.width + p.eps);
+    for (int c = threadIdx.x; c < p.width; c += 1024) {
+      float o = ((float)x[c] - mean) * rstd;
+      if (p.scale) o *= (float)((const P*)p.scale)[c];
+      if (p.bias) o += (float)((const P*)p.bias)[c];
+      ((T*)p.out)[at + c] = (T)o;
+    }
+    if (threadIdx.x == 0 && p.mean) p.mean[m] = mean, p.rstd[m] = rstd;
   }
-  const float rstd = 1.0f / sqrtf(row_sum<1024>(s, scratch[1]) / p.width + p.eps);
-  for (int c = threadIdx.x; c < p.width; c += 1024) {
-    float o = ((float)x[c] - mean) * rstd;
-    if (p.scale) o *= (float)((const P*)p.scale)[c];
-    if (p.bias) o += (float)((const P*)p.bias)[c];
-    ((T*)p.out)[at + c] = (T)o;
-  }
-  if (threadIdx.x == 0 && p.mean) p.mean[blockIdx.x] = mean, p.rstd[blockIdx.x] = rstd;
 }
 
 template <typename T, typename P>
 __global__ __launch_bounds__(1024) void k_norm_backward_wide(Norm p) {
   __shared__ float scratch[2][16];
-  const int64_t at = (int64_t)blockIdx.x * p.width;
-  const float mean = p.mean[blockIdx.x], rstd = p.rstd[blockIdx.x];
-  auto h_of = [&](int c) {
-    const float d = (float)((const T*)p.dy)[at + c];
-    return p.scale ? d * (float)((const P*)p.scale)[c] : d;
-  };
-  auto x_of = [&](int c) { return ((float)((const T*)p.x)[at + c] - mean) * rstd; };
-  float s1 = 0.0f, s2 = 0.0f;
-  for (int c = threadIdx.x; c < p.width; c += 1024) {
-    const float h = h_of(c);
-    s1 += h;
-    s2 += h * x_of(c);
+  for (int64_t m = blockIdx.x; m < p.rows; m += gridDim.x) {
+    const int64_t at = m * p.width;
+    const float mean = p.mean[m], rstd = p.rstd[m];
+    auto h_of = [&](int c) {
+      const float d = (float)((const T*)p.dy)[at + c];
+      return p.scale ? d * (float)((const P*)p.scale)[c] : d;
+    };
+    auto x_of = [&](int c) { return ((float)((const T*)p.x)[at + c] - mean) * rstd; };
+    float s1 = 0.0f, s2 = 0.0f;
+    for (int c = threadIdx.x; c < p.width; c += 1024) {
+      const float h = h_of(c);
+      s1 += h;
+      s2 += h * x_of(c);
+    }
+    s1 = row_sum<1024>(s1, scratch[0]) / p.width;
+    s2 = row_sum<1024>(s2, scratch[1]) / p.width;
+    for (int c = threadIdx.x; c < p.width; c += 1024)
+      ((T*)p.out)[at + c] = (T)(rstd * (h_of(c) - s1 - x_of(c) * s2));
   }
-  s1 = row_sum<1024>(s1, scratch[0]) / p.width;
-  s2 = row_sum<1024>(s2, scratch[1]) / p.width;
-  for (int c = threadIdx.x; c < p.width; c += 1024)
-    ((T*)p.out)[at + c] = (T)(rstd * (h_of(c) - s1 - x_of(c) * s2));
 }
 
 template <typename T>
@@ -299,6 +303,9 @@ __global__ void k_norm_zero(P* a, P* b, int n) {
 constexpr int IN_REGISTERS = 16384;   // widest row of the register form: 1024 threads x 16 elements
 
 int threads_of(int width) { return width <= 1024 ? 64 : width <= 4096 ? 256 : 1024; }
+
+// Workgroups of a forward pass: one a row (or four rows) as long as a launch holds them, then they go on to further rows.
+int64_t few(int64_t blocks) { return blocks < (1 << 20) ? blocks : 1 << 20; }
 
 // Workgroups of the backward pass, each of which leaves a row of partial column sums.
 int backward_blocks(int64_t rows, int width) {
@@ -363,11 +370,11 @@ extern "C" int az_layer_norm_forward(int32_t dtype, int32_t param_dtype, int32_t
   p.rows = rows, p.width = width;
   return with_types(dtype, param_dtype, [&]<typename T, typename P>() -> int {
     if (width > IN_REGISTERS) {
-      k_norm_forward_wide<T, P><<<dim3(rows), dim3(1024), 0, stream>>>(p);
+      k_norm_forward_wide<T, P><<<dim3((unsigned)few(rows)), dim3(1024), 0, stream>>>(p);
     } else {
       with_shape<T, P>(width, [&]<int NT, int R, bool EXACT>() {
         constexpr int ROWS = NT < 256 ? 256 / NT : 1;
-        k_norm_forward<T, P, NT, R, EXACT><<<dim3((unsigned)az_ceil(rows, ROWS)), dim3(NT < 256 ? 256 : NT), 0, stream>>>(p);
+        k_norm_forward<T, P, NT, R, EXACT><<<dim3((unsigned)few(az_ceil(rows, ROWS))), dim3(NT < 256 ? 256 : NT), 0, stream>>>(p);
       });
     }
     AZ_LAUNCH_CHECK();
@@ -405,7 +412,7 @@ extern "C" int az_layer_norm_backward(int32_t dtype, int32_t param_dtype, int32_
     p.rstd = const_cast<float*>(rstd), p.partial = columns ? (float*)workspace : nullptr;
     p.rows = rows, p.width = width;
     if (width > IN_REGISTERS) {
-      if (dx) k_norm_backward_wide<T, P><<<dim3(rows), dim3(1024), 0, stream>>>(p);
+      if (dx) k_norm_backward_wide<T, P><<<dim3((unsigned)few(rows)), dim3(1024), 0, stream>>>(p);
       if (columns)
         k_norm_columns_wide<T><<<dim3((unsigned)az_ceil(width, 256), blocks), dim3(256), 0, stream>>>(p);
     } else {

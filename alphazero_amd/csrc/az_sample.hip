@@ -499,7 +499,7 @@ __device__ __forceinline__ Options options_of(const az_sample_desc& d, int b, do
   o.min_p = d.min_p_rows ? (double)d.min_p_rows[b] : d.min_p;
   o.uniform = d.uniform[b];
   o.goal = 0;
-  if (!(*temperature > 0)) *temperature = 1.0, o.top_k = 1;
+  if (!(*temperature > 1e-300)) *temperature = 1.0, o.top_k = 1;
   if (o.top_k <= 0 || o.top_k >= d.actions) o.top_k = 0;
   o.top_p = o.top_p < 1.0 ? (o.top_p > 0.0 ? o.top_p : 0.0) : 1.0;
   o.min_p = o.min_p > LEAST ? fmin(o.min_p, 1.0) : LEAST;
@@ -823,7 +823,7 @@ __global__ __launch_bounds__(NT) void k_sample_rest(az_sample_desc d, int32_t* a
 
 template <typename T, int CHUNKS>
 void launch_group(const az_sample_desc& d, int32_t* action, float* log_prob, double unit, hipStream_t stream) {
-  const bool direct = !d.temperature_rows && !d.top_k_rows && !d.top_p_rows && d.temperature > 0 &&
+  const bool direct = !d.temperature_rows && !d.top_k_rows && !d.top_p_rows && d.temperature > 1e-300 &&
                       (d.top_k <= 0 || d.top_k >= d.actions) && !(d.top_p < 1.0);
   if (direct) {
     k_sample_group<T, 512, CHUNKS, true><<<dim3(d.rows), dim3(512), 0, stream>>>(d, action, log_prob, unit);
@@ -843,6 +843,8 @@ extern "C" int az_sample_actions(const az_sample_desc* d, int32_t* action, float
   if (d->actions > AZ_SAMPLE_MAX_ACTIONS)
     return az_fail(AZ_ERR_UNSUPPORTED, "sample: up to %d actions", AZ_SAMPLE_MAX_ACTIONS);
   if (d->rows == 0) return AZ_OK;
+  if (!az_grid_fits(d->rows, d->actions <= 1024 ? 64 : 512))
+    return az_fail(AZ_ERR_UNSUPPORTED, "sample: %d rows are too many for one launch", d->rows);
   if (!d->logits || !d->uniform || !action) return az_fail(AZ_ERR_INVALID, "sample: null logits, uniform or action");
   hipStream_t stream = (hipStream_t)stream_;
   // weights of up to one unit each sum up below 2^62, and each is exact in float64

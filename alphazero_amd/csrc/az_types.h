@@ -74,6 +74,9 @@ static inline bool az_aligned16(const void* p) { return ((uintptr_t)p & 15) == 0
 
 static inline int64_t az_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// A launch holds fewer than 2^32 threads along an axis.
+static inline bool az_grid_fits(int64_t blocks, int threads) { return blocks * threads <= 0xffffffffll; }
+
 // f.template operator()<T>() for an AZ_TYPE_ code
 template <typename F>
 static int az_dispatch_type(int dtype, F&& f) {

@@ -10,6 +10,7 @@ import torch
 from . import _native as nat
 
 DTYPES = {torch.float32: nat.TYPE_F32, torch.bfloat16: nat.TYPE_BF16, torch.float16: nat.TYPE_F16}
+MAX_ROWS = 0x7fff0000   # rows and widths are 32-bit numbers in the C ABI
 ACTIVATIONS = {None: nat.ACT_NONE, "relu": nat.ACT_RELU, "swish": nat.ACT_SWISH, "gelu": nat.ACT_GELU}
 
 
@@ -49,6 +50,8 @@ def _checked(op, x, others, same_type=False):
 
 def _rows(x):
     """x as contiguous [rows, width] (x itself where it is: a view would be a node of the autograd graph)."""
+    if x.numel() > MAX_ROWS and (x.shape[-1] > MAX_ROWS or x.numel() // x.shape[-1] > MAX_ROWS):
+        raise NotImplementedError(f"{tuple(x.shape)} holds more than {MAX_ROWS} rows or columns")
     return (x if x.dim() == 2 else x.reshape(-1, x.shape[-1])).contiguous()
 
 

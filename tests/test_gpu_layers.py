@@ -267,6 +267,29 @@ def test_dense_slope_beyond_the_kept_range(T):
     assert float(db[1]) == 1.0               # z = 1e-7 * 2^-14, positive
 
 
+@pytest.mark.parametrize("T", TYPES, ids=str)
+@pytest.mark.parametrize("M,K,N", [(20, 48, 40), (1100, 72, 300), (600, 1500, 700), (1024, 512, 1024)])
+def test_dense_writes_over_its_residual(T, M, K, N):
+    """C ABI: y may be the residual itself, in every form of the product."""
+    x, w, r = rand((M, K), T, 1), rand((K, N), T, 2, K ** -0.5), rand((M, N), T, 3)
+    want = mctx.dense(x, w, None, "swish", r)
+    lib, code = nat.lib(), {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[T]
+    n = lib.az_dense_workspace_bytes(code, M, K, N, 0)
+    ws = torch.empty(n + 16, dtype=torch.uint8, device="cuda")
+    nat.check(lib.az_dense_forward(code, nat.ACT_SWISH, M, K, N, nat.ptr(x), nat.ptr(w), None, nat.ptr(r), nat.ptr(r), None,
+                                   nat.ptr(ws), n, nat.stream_ptr()))
+    torch.cuda.synchronize()
+    assert torch.equal(r, want)
+
+
+def test_second_derivatives_are_refused():
+    x, w = rand((5, 6), torch.float32, 1).requires_grad_(), rand((6, 7), torch.float32, 2).requires_grad_()
+    for y in (mctx.dense(x, w, None, "swish"), mctx.layer_norm(x)):
+        (g,) = torch.autograd.grad(y.sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), x)
+
+
 # ---------------------------------------------------------------- layer norm
 def check_norm(x, scale, bias, eps, dy, y, grads):
     T = x.dtype
@@ -328,7 +351,7 @@ def test_layer_norm_and_gradients(T, M, D):
 @pytest.mark.parametrize("T", TYPES, ids=str)
 def test_layer_norm_many_rows(T):
     """More rows than the backward pass has workgroups, a ragged last one."""
-    for M, D in ((5003, 96), (2501, 1200), (777, 5000)):
+    for M, D in ((5003, 96), (2501, 1200), (777, 5000), (300, 17000)):
         x, s, b = rand((M, D), T, 1).requires_grad_(), rand((D,), T, 2).requires_grad_(), rand((D,), T, 3).requires_grad_()
         dy = rand((M, D), T, 4)
         y = mctx.layer_norm(x, s, b, eps=1e-3)
@@ -507,6 +530,10 @@ def test_sample_actions_parameters_by_row_and_extremes():
     min_p = torch.tensor([0.0, 0.0, 0.0, 0.0, 0.0, 0.5, 0.0, 0.0625, 0.0, 2.0, 0.0, -1.0], device=dev)
     for seed in range(4):
         check_sample(logits, uniforms(B, seed), temperature, top_k, top_p, min_p)
+    check_sample(logits, uniforms(B, 9), temperature=1e-310)
+    check_sample(logits, uniforms(B, 9), temperature=1e-290)
+    check_sample(logits, uniforms(B, 9), temperature=1e-30, top_p=0.5)
+    check_sample(logits, uniforms(B, 9), temperature=1e300, top_p=0.5, top_k=300)
     # uniforms outside [0, 1) take the nearest end
     u = torch.tensor([-1.0, math.nan, 1.0, 2.0], device=dev)
     a, lp = mctx.sample_actions(logits[:4], u, top_k=1)

@@ -152,3 +152,23 @@ def test_prior_policy_and_networks_refusals():
         trainer.Trainer(trainer.Config(env_id="Breakout-MinAtar", torso="transformer"), device="cpu")
     # what the learner computes without the operators is what it computed before
     assert trainer.Config().native_dense is False and trainer.Config().torso == "conv"
+
+
+def test_sizes_beyond_the_abi_are_refused():
+    """Rows and widths are 32-bit numbers there: tensors (without storage here) that would wrap."""
+    big = torch.empty((1,), dtype=H).expand(2 ** 32 + 5, 1)
+    with pytest.raises(NotImplementedError):
+        mctx.dense(big, t(1, 1, dtype=H))
+    with pytest.raises(NotImplementedError):
+        mctx.layer_norm(big)
+    with pytest.raises(NotImplementedError):
+        mctx.sample_actions(big, torch.empty((1,)).expand(2 ** 32 + 5))
+    from alphazero_amd import layers
+    with pytest.raises(NotImplementedError, match="rows or columns"):
+        layers._rows(big)
+    lib = nat.lib()
+    some = C.c_void_p(4096)
+    # more outputs or rows than a launch has threads for
+    assert lib.az_dense_forward(1, 0, 2 ** 31 - 2 ** 16, 1, 2 ** 20, some, some, None, None, some, None, some, 1 << 62, None) == -2
+    d = nat.SampleDesc(dtype=0, rows=2 ** 31 - 1, actions=2, logits=4096, uniform=4096)
+    assert lib.az_sample_actions(C.byref(d), some, some, None) == -2
