@@ -7,7 +7,7 @@
 // evenly, then over the order-preserving integer of the logit within the bin that holds the cut, until that bin is a
 // single logit.  Weights are summed as 64-bit integers: the order of the LDS atomics does not matter.
 //
-// Up to 1024 actions a wave takes a row, which it holds in LDS.  Of up to 128 candidates every one is compared with
+// Up to 1024 actions a wave takes a row, which it holds in LDS.  Of up to 256 candidates every one is compared with
 // every other: that gives each its place in the descending order and the weight ahead of it at once.  Beyond, a workgroup holds the row in registers (up to
 // 32768 actions; wider rows are read from L2 again), takes the first histogram over it, and moves the actions of the bins
 // up to the cut's, in index order, into a list in LDS; one wave ends the draw on the list while the
@@ -234,10 +234,10 @@ struct Share {
 };
 
 // Scans the bins: the first whose inclusive sum, with `before`, reaches the goal is left in s.found (NB: none),
-// the sum ahead of it in s.found_before.  With `share` the goal is that share of the bins' total but `less` (of the
-// first one at least).
+// the sum ahead of it in s.found_before.  With a `share` below 1 the goal is that share of the bins' total but `less` (of
+// the first one at least).
 template <int NT, int NB>
-__device__ __forceinline__ u64 find(Shared<NT, NB>& s, u64 before, u64 goal, const Share* share, u64 less) {
+__device__ __forceinline__ u64 find(Shared<NT, NB>& s, u64 before, u64 goal, double share = 1.0, u64 less = 0) {
   constexpr int PER = NB / NT;
   const int t = threadIdx.x & (NT - 1);
   u64 mine = 0, ahead, h[PER];
@@ -246,8 +246,8 @@ __device__ __forceinline__ u64 find(Shared<NT, NB>& s, u64 before, u64 goal, con
   const u64 total = group_sum<NT>(mine, s, &ahead);
   if (t == 0) s.found = NB;
   sync<NT>();
-  if (share) {
-    goal = share->of(total - less, true);
+  if (share < 1.0) {
+    goal = Share(share).of(total - less, true);
     if (goal == 0) goal = 1;
   }
   u64 cum = before + ahead + scan - mine;
@@ -278,7 +278,7 @@ __device__ __forceinline__ void count(Shared<NT, NB>& s, int bin, const Weights&
 // The shortest prefix of the descending order, among logits with a key >= `least`, whose counts (MASS: weights) sum up
 // to the goal; false if there is none (no cut).
 template <bool MASS, int NB, typename Row>
-__device__ __forceinline__ bool select(const Row& row, Shared<Row::THREADS, NB>& s, const Weights& w, u64 goal, const Share* share,
+__device__ __forceinline__ bool select(const Row& row, Shared<Row::THREADS, NB>& s, const Weights& w, u64 goal, double share,
                        uint32_t least, u64 less, Cut* cut) {
   constexpr int NT = Row::THREADS;
   const float scale = w.scale(NB);
@@ -310,7 +310,7 @@ __device__ __forceinline__ bool select(const Row& row, Shared<Row::THREADS, NB>&
       if (k >= lo && k <= hi) count<MASS>(s, (hi - k) >> shift, w, l);
     });
     sync<NT>();
-    find(s, before, goal, nullptr, 0);
+    find(s, before, goal);
     // (the sums over these keys are those of the bin that crossed, so one of its bins crosses)
     if (s.found >= NB) break;
     const uint32_t b = s.found;
@@ -400,14 +400,13 @@ __device__ __forceinline__ Result draw(const Row& row, Shared<Row::THREADS, NB>&
   };
   if (o.top_k > 0) {
     Cut c;
-    if (select<false>(row, s, w, (u64)o.top_k, nullptr, 0, 0, &c)) cut = c;
+    if (select<false>(row, s, w, (u64)o.top_k, 1.0, 0, 0, &c)) cut = c;
   }
   if (o.top_p < 1.0) {
     // the weight of the ties at the top_k cut that are out
     const u64 less = cut.key && !o.goal ? (ties_of(cut.key) - cut.ties) * w.mass(logit_of(cut.key)) : 0;
-    const Share share(o.top_p);
     Cut c;
-    if (select<true>(row, s, w, o.goal, o.goal ? nullptr : &share, cut.key, less, &c)) {
+    if (select<true>(row, s, w, o.goal, o.goal ? 1.0 : o.top_p, cut.key, less, &c)) {
       if (c.key > cut.key)
         cut = c;
       else if (c.key == cut.key && c.ties < cut.ties)
@@ -431,36 +430,38 @@ __device__ __forceinline__ Result draw(const Row& row, Shared<Row::THREADS, NB>&
   return {at_sum(row, s, target_of(o.uniform, total), kept), (double)total / w.unit};
 }
 
-// The whole draw over at most FEW actions in LDS (their indices `at`, or their places), by one wave.
-constexpr int FEW = 128;
+// The whole draw over at most FEW actions in LDS (their indices `at`, or their places), by one wave: E a lane.
+constexpr int FEW = 256;
 
-__device__ __forceinline__ Result draw_few(const float* l, const int* at, int n, u64* scratch, const Weights& w,
-                                           const Options& o) {
-  constexpr int E = FEW / 64;
+struct FewScratch {
+  u64 order[FEW];    // key, then the place from behind: greater is earlier in the descending order
+  u64 mass[FEW];
+};
+
+template <int E>
+__device__ __forceinline__ Result draw_ranked(const float* l, const int* at, int n, FewScratch& s, const Weights& w,
+                                              const Options& o) {
   const int lane = threadIdx.x & 63;
-  u64* masses = scratch;                                        // [FEW]
-  uint32_t* keys = reinterpret_cast<uint32_t*>(scratch + FEW);  // [FEW]
-  uint32_t key[E], rank[E];
-  u64 m[E], ahead[E];
+  uint32_t rank[E];
+  u64 order[E], m[E], ahead[E];
   double x[E];
   bool in[E];
   for (int e = 0; e < E; ++e) {
     const int i = e * 64 + lane;
     const float v = i < n ? l[i] : -INFINITY;
     in[e] = v > -INFINITY;
-    key[e] = key_of(v);
+    order[e] = (u64)key_of(v) << 32 | (uint32_t)~i;
     x[e] = in[e] ? w(v) : 0.0;
     m[e] = w.whole(x[e]);
     rank[e] = 0, ahead[e] = 0;
-    masses[i] = m[e], keys[i] = key[e];
+    s.mass[i] = m[e], s.order[i] = order[e];
   }
   sync<64>();
 #pragma unroll 4
   for (int j = 0; j < n; ++j) {
-    const uint32_t k = keys[j];
-    const u64 mass = masses[j];
+    const u64 other = s.order[j], mass = s.mass[j];
     for (int e = 0; e < E; ++e) {
-      const bool first = k > key[e] || (k == key[e] && j < e * 64 + lane);
+      const bool first = other > order[e];
       rank[e] += first;
       ahead[e] += first ? mass : 0;
     }
@@ -488,6 +489,14 @@ __device__ __forceinline__ Result draw_few(const float* l, const int* at, int n,
     if (over) found = e * 64 + __ffsll(over) - 1;
   }
   return {at ? at[found] : found, (double)total / w.unit};
+}
+
+__device__ __forceinline__ Result draw_few(const float* l, const int* at, int n, FewScratch& s, const Weights& w,
+                                           const Options& o) {
+  if (n <= 64) return draw_ranked<1>(l, at, n, s, w, o);
+  if (n <= 128) return draw_ranked<2>(l, at, n, s, w, o);
+  if (n <= 192) return draw_ranked<3>(l, at, n, s, w, o);
+  return draw_ranked<4>(l, at, n, s, w, o);
 }
 
 // ---------------------------------------------------------------------------
@@ -538,7 +547,13 @@ template <typename T, int MOST, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void k_sample_wave(az_sample_desc d, int32_t* action, float* log_prob,
                                                             double unit) {
   constexpr int V = 16 / sizeof(T), NB = 256;
-  __shared__ Shared<64, NB> shared[WAVES];
+  // (the histogram and the candidates' scratch are not used at the same time; 16 rows fit a compute unit's LDS)
+  union Scratch {
+    Shared<64, NB> s;
+    FewScratch few;
+    __device__ Scratch() {}
+  };
+  __shared__ Scratch scratch[WAVES];
   __shared__ float list[WAVES][MOST];
   __shared__ float few[WAVES][FEW];
   __shared__ int few_at[WAVES][FEW];
@@ -574,10 +589,10 @@ __global__ __launch_bounds__(64 * WAVES) void k_sample_wave(az_sample_desc d, in
   const float* l = list[wave];
   Result r;
   if (d.actions <= FEW) {
-    r = draw_few(l, nullptr, d.actions, shared[wave].bins, w, o);
+    r = draw_few(l, nullptr, d.actions, scratch[wave].few, w, o);
   } else {
     const ListRow row = {l, nullptr, d.actions, (d.actions + 63) / 64};
-    Shared<64, NB>& s = shared[wave];
+    Shared<64, NB>& s = scratch[wave].s;
     // the bin that holds the first cut, and the actions up to it (k_sample_group has the same, over more threads)
     const float scale = w.scale(NB);
     int bound = NB;
@@ -585,7 +600,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_sample_wave(az_sample_desc d, in
       clear(s);
       each(row, [&](float x, int) { count<false>(s, bin_of(top, x, scale, NB), w, x); });
       sync<64>();
-      find(s, 0, (u64)o.top_k, nullptr, 0);
+      find(s, 0, (u64)o.top_k);
       bound = s.found;
       if (bound >= NB - 1) bound = NB, o.top_k = 0;   // nothing that could be drawn is cut
     }
@@ -593,8 +608,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_sample_wave(az_sample_desc d, in
       clear(s);
       each(row, [&](float x, int) { count<true>(s, bin_of(top, x, scale, NB), w, x); });
       sync<64>();
-      const Share share(o.top_p);
-      o.goal = find(s, 0, 0, &share, 0);
+      o.goal = find(s, 0, 0, o.top_p);
       bound = s.found;
     }
     int n = FEW + 1;
@@ -611,7 +625,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_sample_wave(az_sample_desc d, in
       }
       sync<64>();
     }
-    r = n <= FEW ? draw_few(few[wave], few_at[wave], n, s.bins, w, o) : draw<NB>(row, s, w, o);
+    r = n <= FEW ? draw_few(few[wave], few_at[wave], n, scratch[wave].few, w, o) : draw<NB>(row, s, w, o);
   }
   if (lane == 0) write<T>(d, b, w, r, action, log_prob);
 }
@@ -656,6 +670,7 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
   __shared__ Shared<64, DIRECT ? 64 : 256> s1;
   __shared__ float list[DIRECT ? 1 : LIST];
   __shared__ int list_at[DIRECT ? 1 : LIST];
+  __shared__ FewScratch scratch;
   __shared__ float tops[NW];
   __shared__ int counts[NW];
   const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -674,6 +689,7 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
 #pragma unroll
     for (int v = 0; v < V; ++v) top = fmaxf(top, l[v]);
   });
+  float own = top;   // the thread's largest
   top = wave_max(top);
   if (lane == 0) tops[wave] = top;
   __syncthreads();
@@ -685,6 +701,7 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
   }
   if (top == INFINITY) {
     memory.infinite = true, top = 0.0f;
+    own = own == INFINITY ? 0.0f : -INFINITY;
     if constexpr (CHUNKS > 0) {
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c)
@@ -717,7 +734,17 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
     const float scale = w.scale(BINS);
     // the bin that holds the first cut
     int bound = BINS;
-    if (o.top_k > 0) {
+    if (o.top_k > 0 && o.top_k <= NT) {
+      // top_k threads whose largest logits are at or above some logit hold top_k actions there: the histogram of
+      // the threads' largest ones gives a bin that is low enough
+      clear(s);
+      if (own > -INFINITY) count<false>(s, bin_of(top, own, scale, BINS), w, own);
+      __syncthreads();
+      find(s, 0, (u64)o.top_k);
+      bound = s.found;
+      if (bound == BINS - 1) bound = BINS;
+    }
+    if (bound == BINS && o.top_k > 0) {
       clear(s);
       const float none = anew(-INFINITY), scale_ = anew(scale);
       front.chunks(memory, [&](int, const float* l) {
@@ -726,7 +753,7 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
           if (l[v] > none) count<false>(s, bin_of(top, l[v], scale_, BINS), w, l[v]);
       });
       __syncthreads();
-      find(s, 0, (u64)o.top_k, nullptr, 0);
+      find(s, 0, (u64)o.top_k);
       bound = s.found;
       if (bound >= BINS - 1) bound = BINS, o.top_k = 0;   // nothing that could be drawn is cut
     }
@@ -739,8 +766,7 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
           if (l[v] > none) count<true>(s, bin_of(top, l[v], scale_, BINS), w, l[v]);
       });
       __syncthreads();
-      const Share share(o.top_p);
-      o.goal = find(s, 0, 0, &share, 0);
+      o.goal = find(s, 0, 0, o.top_p);
       bound = s.found;
     }
     // the actions up to that bin, in index order, into the list
@@ -782,7 +808,7 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
     __syncthreads();
     if (wave > 0) return;
     const ListRow row = {list, list_at, n, (n + 63) / 64};
-    const Result r = n <= FEW ? draw_few(list, list_at, n, s1.bins, w, o) : draw<256>(row, s1, w, o);
+    const Result r = n <= FEW ? draw_few(list, list_at, n, scratch, w, o) : draw<256>(row, s1, w, o);
     if (lane == 0) write<T>(d, b, w, r, action, log_prob);
   }
 }
@@ -855,7 +881,11 @@ extern "C" int az_sample_actions(const az_sample_desc* d, int32_t* action, float
     constexpr int V = 16 / sizeof(T);
     const int n = d->actions;
     const dim3 rows(d->rows);
-    if (n <= 1024)
+    if (n <= 256)
+      k_sample_wave<T, 256, 1><<<rows, dim3(64), 0, stream>>>(*d, action, log_prob, unit);
+    else if (n <= 512)
+      k_sample_wave<T, 512, 1><<<rows, dim3(64), 0, stream>>>(*d, action, log_prob, unit);
+    else if (n <= 1024)
       k_sample_wave<T, 1024, 1><<<rows, dim3(64), 0, stream>>>(*d, action, log_prob, unit);
     else if (n <= 512 * 16)
       launch_group<T, 16 / V>(*d, action, log_prob, unit, stream);
