@@ -362,7 +362,9 @@ int64_t splits_for(int64_t tiles, int64_t want, int64_t K, int64_t least) {
 //     that have to be copied first: 1003 x 401 x 517 23 / 19
 //   float32: 4096 x 1024 x 1024 83 / 114, 1024 x 1024 x 1024 38 / 40, 256 x 2048 x 2048 43 / 38
 // 256 x 256 tiles pay from one for each compute unit on: 16384 x 512 x 2048 59 against 62 with 128 x 128 (512 tiles),
-// its dx 57 against 37 (128 tiles).
+// its dx 57 against 37 (128 tiles).  With fewer tiles they pay where the splits that fill the compute units stay long:
+// dkernel of 16384 x 2048 x 2048 in bfloat16 125 (4 splits of 4096) against 149, of 8192 x 2048 x 2048 83 (4 of 2048)
+// against 77; in float32, where every step is six, 389 against 436.
 // Few outputs, up to 1024 tiles of 16 x 16, as long as the reduction is not too long for the waves of one workgroup
 // (k_product_few / the best other form): 64 x 256 x 256 float32 3.4 / 7.3, bfloat16 3.2 / 7.0, 512 x 512 x 512 float32
 // 9.4 / 12.2, 1 x 4096 x 4096 float32 20.7 / 35, bfloat16 dx 8.4 / 10.2 but y (whose second operand it reads element by
@@ -383,8 +385,11 @@ Plan plan_of(int dtype, int64_t M, int64_t N, int64_t K, bool in_place, int cont
     s = splits_for(tiles, K >= 1024 ? 512 : 256, K, tiles <= 16 ? 32 : f32 ? 128 : 256);
   } else if (p.wide) {
     const int64_t large = az_ceil(M, 256) * az_ceil(N, 256), steps = f32 ? 6 * K : K;
-    p.big = large >= 256;
-    if (!p.big) {
+    const int64_t share = 256 / large;   // splits that give each compute unit a large tile
+    p.big = large >= 256 || (share >= 1 && large * share >= 192 && steps / share >= 4096);
+    if (p.big) {
+      s = large >= 256 ? 1 : share;
+    } else {
       const int64_t tiles = az_ceil(M, 128) * az_ceil(N, 128);
       const int64_t one = splits_for(tiles, 256, steps, 512), two = splits_for(tiles, 512, steps, 2048);
       s = one > two ? one : two;

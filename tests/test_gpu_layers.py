@@ -753,3 +753,18 @@ def test_graphed_learner_equals_the_eager_one():
     assert results[0][0] == pytest.approx(results[1][0], rel=1e-5)
     for a, b in zip(results[0][1], results[1][1]):
         assert torch.allclose(a, b, rtol=1e-5, atol=1e-6)
+
+
+def test_dense_split_large_tiles():
+    """A long reduction over few outputs in float32: 256 x 256 tiles, the reduction split (dkernel), and the forms
+    beside it; against 64-bit products on the GPU."""
+    M, K, N = 12288, 1000, 1024
+    x, w = rand((M, K), torch.float32, 1).requires_grad_(), rand((K, N), torch.float32, 2, K ** -0.5).requires_grad_()
+    dy = rand((M, N), torch.float32, 3)
+    y = mctx.dense(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    xd, wd, g = x.detach().double(), w.detach().double(), dy.double()
+    close(y.detach(), xd @ wd, (K + 4) * U * (xd.abs() @ wd.abs()), torch.float32, "y")
+    close(dx, g @ wd.t().contiguous(), (N + 4) * U * (g.abs() @ wd.abs().t().contiguous()), torch.float32, "dx")
+    xt = xd.t().contiguous()
+    close(dw, xt @ g, (M + 4) * U * (xt.abs() @ g.abs()), torch.float32, "dw")
