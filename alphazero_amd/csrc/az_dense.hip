@@ -138,12 +138,12 @@ __device__ __forceinline__ AzPack<C> piece(const S* p, int64_t ld, int rows, int
   return x;
 }
 
+// One workgroup's 16 x 16 outputs.
 template <typename C, typename SA, typename SB, typename TO, bool AKC, bool BKC, int EPI>
-__global__ __launch_bounds__(WAVES * 64) void k_product_few(Prod p) {
+__device__ __forceinline__ void few_outputs(const Prod& p, int block, az_f32x4 (*sums)[64]) {
   constexpr int E = AzPack<C>::N;
-  __shared__ az_f32x4 sums[WAVES][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int m0 = (blockIdx.x % p.tiles_m) * 16, n0 = (blockIdx.x / p.tiles_m) * 16;
+  const int m0 = (block % p.tiles_m) * 16, n0 = (block / p.tiles_m) * 16;
   az_f32x4 acc = {};
 #pragma unroll 2
   for (int k = wave * 4 * E; k < p.K; k += WAVES * 4 * E) {
@@ -158,6 +158,43 @@ __global__ __launch_bounds__(WAVES * 64) void k_product_few(Prod p) {
   for (int w = 1; w < WAVES; ++w) acc += sums[w][lane];
   const float v[4] = {acc[0], acc[1], acc[2], acc[3]};
   finish<TO, EPI>(p, m0 + (lane & 15), n0 + (lane >> 4) * 4, v);
+}
+
+template <typename C, typename SA, typename SB, typename TO, bool AKC, bool BKC, int EPI>
+__global__ __launch_bounds__(WAVES * 64) void k_product_few(Prod p) {
+  __shared__ az_f32x4 sums[WAVES][64];
+  few_outputs<C, SA, SB, TO, AKC, BKC, EPI>(p, blockIdx.x, sums);
+}
+
+// The bias' gradient from `chunks` rows of partial column sums, added in k_join's order: 64 columns a workgroup.
+template <typename T>
+__device__ __forceinline__ void join_columns(const float* part, int N, int chunks, T* out, int block, float (*sums)[64]) {
+  const int c = threadIdx.x & 63, w = threadIdx.x >> 6, n = block * 64 + c;
+  float s = 0.0f;
+  if (n < N) {
+#pragma unroll 4
+    for (int i = w; i < chunks; i += WAVES) s += part[(int64_t)i * N + n];
+  }
+  sums[w][c] = s;
+  __syncthreads();
+  if (w > 0 || n >= N) return;
+  for (int i = 1; i < WAVES; ++i) s += sums[i][c];
+  out[n] = (T)s;
+}
+
+// All of a small layer's backward pass behind dz in one launch (each launch costs the host three microseconds): dx,
+// then dkernel, then the bias' gradient.  S: the type of dz.
+template <typename C, typename S, typename T>
+__global__ __launch_bounds__(WAVES * 64) void k_gradients_few(Prod dx, Prod dw, int dx_blocks, int dw_blocks,
+                                                              const float* part, int chunks, T* dbias) {
+  __shared__ az_f32x4 sums[WAVES][64];
+  const int block = blockIdx.x;
+  if (block < dx_blocks)
+    few_outputs<C, S, T, T, true, true, EPI_STORE>(dx, block, sums);
+  else if (block < dx_blocks + dw_blocks)
+    few_outputs<C, T, S, T, false, false, EPI_STORE>(dw, block - dx_blocks, sums);
+  else
+    join_columns(part, dw.N, chunks, dbias, block - dx_blocks - dw_blocks, reinterpret_cast<float(*)[64]>(sums));
 }
 
 // ---------------------------------------------------------------------------
@@ -418,19 +455,24 @@ bool rows_aligned(const void* p, int64_t ld) {
   return ld % AzPack<S>::N == 0 && az_aligned16(p);
 }
 
+// Alignments and tiles of a product; the number of tiles.
+template <typename T, typename SA, typename SB>
+int64_t prepare(Prod& p, int tile) {
+  p.a_vec = rows_aligned<SA>(p.a, p.lda);
+  p.b_vec = rows_aligned<SB>(p.b, p.ldb);
+  auto four = [](const void* q) { return ((uintptr_t)q & (4 * sizeof(T) - 1)) == 0; };
+  p.out_vec = p.N % 4 == 0 && four(p.out) && four(p.bias) && four(p.residual) && az_aligned16(p.z);
+  p.tiles_m = (int)az_ceil(p.M, tile), p.tiles_n = (int)az_ceil(p.N, tile);
+  return (int64_t)p.tiles_m * p.tiles_n;
+}
+
 // One product (and, with `extra`, the join of the bias' gradient).  `partial` holds splits x M x N floats.  SA, SB: the
 // operands' types where they are not T's (few outputs in float32 arithmetic).
 template <typename T, bool AKC, bool BKC, int EPI, typename SA = T, typename SB = T>
 int product(Prod p, const Plan& plan, float* partial, const Join* extra, hipStream_t stream) {
   const int pass = EPI == EPI_FORWARD ? PASS_Y : AKC ? PASS_DX : PASS_DW;
   const int dtype = sizeof(T) == 4 ? AZ_TYPE_F32 : std::is_same_v<T, az_bf16> ? AZ_TYPE_BF16 : AZ_TYPE_F16;
-  p.a_vec = rows_aligned<SA>(p.a, p.lda);
-  p.b_vec = rows_aligned<SB>(p.b, p.ldb);
-  auto four = [](const void* q) { return ((uintptr_t)q & (4 * sizeof(T) - 1)) == 0; };
-  p.out_vec = p.N % 4 == 0 && four(p.out) && four(p.bias) && four(p.residual) && az_aligned16(p.z);
-  const int tile = plan.wide ? (plan.big ? 256 : 128) : plan.few ? 16 : TILE;
-  p.tiles_m = (int)az_ceil(p.M, tile), p.tiles_n = (int)az_ceil(p.N, tile);
-  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+  const int64_t tiles = prepare<T, SA, SB>(p, plan.wide ? (plan.big ? 256 : 128) : plan.few ? 16 : TILE);
   if (!az_grid_fits(tiles, plan.few ? WAVES * 64 : 512) || !az_grid_fits(az_ceil((int64_t)p.M * p.N, 256), 256))
     return az_fail(AZ_ERR_UNSUPPORTED, "dense: %d x %d outputs are too many for one launch", p.M, p.N);
   const int step = plan.wide ? 64 : Stage<T, true>::BK;
@@ -623,6 +665,25 @@ extern "C" int az_dense_backward(int32_t dtype, int32_t act, int32_t rows, int32
     const void* dz32 = copy ? ws + l.dz : dy;
     const int64_t ld32 = copy ? ld : fan_out;
     float* partial = (float*)(ws + l.partial);
+    if (dx && dkernel && l.dx.few && l.dw.few) {
+      Prod px = {}, pw = {};
+      operand_a(px, sdz, nullptr, 0);
+      operand_b(px, Source{kernel, fan_out, 0}, nullptr, 0);
+      px.M = rows, px.N = fan_in, px.K = fan_out, px.out = dx;
+      operand_a(pw, Source{x, fan_in, 0}, nullptr, 0);
+      operand_b(pw, sdz, nullptr, 0);
+      pw.M = fan_in, pw.N = fan_out, pw.K = rows, pw.out = dkernel;
+      auto run = [&]<typename C, typename S>() -> int {
+        const int64_t nx = prepare<T, S, T>(px, 16), nw = prepare<T, T, S>(pw, 16);
+        const int64_t nb = dbias ? az_ceil(fan_out, 64) : 0;
+        if (!az_grid_fits(nx + nw + nb, WAVES * 64)) return az_fail(AZ_ERR_UNSUPPORTED, "dense: too many outputs");
+        k_gradients_few<C, S, T><<<dim3((unsigned)(nx + nw + nb)), dim3(WAVES * 64), 0, stream>>>(
+            px, pw, (int)nx, (int)nw, (const float*)(ws + l.bias), l.chunks, (T*)dbias);
+        AZ_LAUNCH_CHECK();
+        return AZ_OK;
+      };
+      return whole ? run.template operator()<float, float>() : run.template operator()<T, T>();
+    }
     if (dx) {
       Prod p = {};
       Source sk = {kernel, fan_out, 0};

@@ -227,8 +227,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product_wide(Prod p) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
     const int n = n0 + wn + j0 * 16 + (lane & 15) * 4;
-    // the residual of the next four rows is loaded while these four are worked on
-    constexpr int AHEAD = 4;
+    // the residual of the next rows is loaded while these are worked on: 64 bytes a lane in flight
+    constexpr int AHEAD = 8;
     AzVec<TO, 4> next[AHEAD];
     const bool early = EPI == EPI_FORWARD && p.residual && p.out_vec;
     auto fetch = [&](int r0) {
