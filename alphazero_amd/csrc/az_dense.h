@@ -69,10 +69,9 @@ struct Prod {
   int64_t lda, ldb;
   int M, N, K;
   int k_chunk;          // reduction length of one split (blockIdx.z)
-  int a_vec, b_vec;     // 16-byte loads are aligned
   int tiles_m, tiles_n;
   // epilogue
-  int act, out_vec;     // out_vec: rows of the outputs can be read and written four elements at a time
+  int act;
   const void* bias;
   const void* residual;
   void* z;
@@ -85,27 +84,27 @@ struct Prod {
   int64_t lda32, ldb32;
 };
 
-// Four consecutive outputs of row m from column n.  `early`: the caller has loaded their residual.
+// Four consecutive outputs of row m from column n, at any address.  `early`: the caller has loaded their residual.
 template <typename T, int EPI>
 __device__ __forceinline__ void finish(const Prod& p, int m, int n, const float* v, bool early = false,
                                        AzVec<T, 4> loaded = {}) {
   if (m >= p.M || n >= p.N) return;
   const int64_t at = (int64_t)m * p.N + n;
-  const int have = p.N - n < 4 ? p.N - n : 4;
+  const int have = p.N - n;
   if constexpr (EPI == EPI_PARTIAL) {
     float* out = p.partial + (int64_t)blockIdx.z * p.M * p.N + at;
-    if (p.out_vec) {
-      *reinterpret_cast<float4*>(out) = float4{v[0], v[1], v[2], v[3]};
+    if (have >= 4) {
+      az_storeu<float, 4>(out, AzVec<float, 4>{v[0], v[1], v[2], v[3]});
     } else {
       for (int i = 0; i < have; ++i) out[i] = v[i];
     }
   } else {
     T* out = (T*)p.out + at;
     if constexpr (EPI == EPI_STORE) {
-      if (p.out_vec) {
+      if (have >= 4) {
         AzVec<T, 4> o;
         for (int i = 0; i < 4; ++i) o.v[i] = (T)v[i];
-        az_storev<T, 4>(out, o);
+        az_storeu<T, 4>(out, o);
       } else {
         for (int i = 0; i < have; ++i) out[i] = (T)v[i];
       }
@@ -114,19 +113,18 @@ __device__ __forceinline__ void finish(const Prod& p, int m, int n, const float*
       const T* bias = (const T*)p.bias;
       const T* res = p.residual ? (const T*)p.residual + at : nullptr;
       Z* z = p.z ? (Z*)p.z + at : nullptr;
-      if (p.out_vec) {
-        AzVec<T, 4> o, r, b;
+      if (have >= 4) {
+        AzVec<T, 4> o, r = loaded, b;
         AzVec<Z, 4> zz;
-        if (bias) b = az_loadv<T, 4>(bias + n);
-        r = loaded;
-        if (res && !early) r = az_loadv<T, 4>(res);
+        if (bias) b = az_loadu<T, 4>(bias + n);
+        if (res && !early) r = az_loadu<T, 4>(res);
         for (int i = 0; i < 4; ++i) {
           const float s = v[i] + (bias ? (float)b.v[i] : 0.0f);
           keep(&zz.v[i], s);
           o.v[i] = (T)(act_value(s, p.act) + (res ? (float)r.v[i] : 0.0f));
         }
-        if (z) az_storev<Z, 4>(z, zz);
-        az_storev<T, 4>(out, o);
+        if (z) az_storeu<Z, 4>(z, zz);
+        az_storeu<T, 4>(out, o);
       } else {
         for (int i = 0; i < have; ++i) {
           const float s = v[i] + (bias ? (float)bias[n + i] : 0.0f);

@@ -18,7 +18,7 @@ using namespace az_dense;
 namespace {
 
 // ---------------------------------------------------------------------------
-// Any sizes and alignments: 64 x 64 outputs a workgroup, four waves of 32 x 32, 256 bytes of reduction a step (64
+// Any sizes and alignments (gfx950 loads 16 bytes at any address): 64 x 64 outputs a workgroup, four waves of 32 x 32, 256 bytes of reduction a step (64
 // float32 elements, 128 of 16 bits).  Operands go through registers (one step ahead, every element guarded, zero outside)
 // into LDS, each row's reduction contiguous, rows 272 bytes apart so that the 16 rows of an operand read fall on
 // different banks.  A step this long keeps the loads of the next one in flight for two thousand cycles of matrix
@@ -36,15 +36,15 @@ struct Stage {
   __device__ static int red(int q) {
     return KC ? (threadIdx.x % (4 * PACKS)) * E : threadIdx.x / (TILE / E) + q * (BK / PACKS);
   }
-  __device__ void load(const T* p, int64_t ld, int rows, int r0, int k0, int k1, bool vec) {
+  __device__ void load(const T* p, int64_t ld, int rows, int r0, int k0, int k1) {
 #pragma unroll
     for (int q = 0; q < PACKS; ++q) {
       const int r_ = r0 + row(q), k_ = k0 + red(q);
       const int cont = KC ? k_ : r_, cont_end = KC ? k1 : rows;
       const bool line = KC ? r_ < rows : k_ < k1;
       const T* at = p + (KC ? (int64_t)r_ * ld + k_ : (int64_t)k_ * ld + r_);
-      if (line && vec && cont + E <= cont_end) {
-        r[q] = az_load16(at);
+      if (line && cont + E <= cont_end) {
+        __builtin_memcpy(&r[q], at, 16);   // (at any address)
       } else {
 #pragma unroll
         for (int e = 0; e < E; ++e) r[q].v[e] = line && cont + e < cont_end ? at[e] : (T)0.0f;
@@ -75,16 +75,16 @@ __global__ __launch_bounds__(256) void k_product_tile(Prod p) {
   Stage<T, AKC> sa;
   Stage<T, BKC> sb;
   az_f32x4 acc[2][2] = {};
-  sa.load((const T*)p.a, p.lda, p.M, m0, k_begin, k_end, p.a_vec);
-  sb.load((const T*)p.b, p.ldb, p.N, n0, k_begin, k_end, p.b_vec);
+  sa.load((const T*)p.a, p.lda, p.M, m0, k_begin, k_end);
+  sb.load((const T*)p.b, p.ldb, p.N, n0, k_begin, k_end);
   int buf = 0;
   for (int k = k_begin; k < k_end; k += BK, buf ^= 1) {
     sa.store(lds[buf][0]);
     sb.store(lds[buf][1]);
     __syncthreads();   // (the other buffer's readers passed the barrier of the step before)
     if (k + BK < k_end) {
-      sa.load((const T*)p.a, p.lda, p.M, m0, k + BK, k_end, p.a_vec);
-      sb.load((const T*)p.b, p.ldb, p.N, n0, k + BK, k_end, p.b_vec);
+      sa.load((const T*)p.a, p.lda, p.M, m0, k + BK, k_end);
+      sb.load((const T*)p.b, p.ldb, p.N, n0, k + BK, k_end);
     }
 #pragma unroll
     for (int q = 0; q < PACKS; ++q) {
@@ -118,13 +118,13 @@ constexpr int WAVES = 16;
 
 // C: the type that the matrix instructions take, S: the operand's in memory.
 template <typename C, typename S, bool KC>
-__device__ __forceinline__ AzPack<C> piece(const S* p, int64_t ld, int rows, int K, int r, int k, bool vec) {
+__device__ __forceinline__ AzPack<C> piece(const S* p, int64_t ld, int rows, int K, int r, int k) {
   constexpr int E = AzPack<C>::N;
   AzPack<C> x;
   if constexpr (KC) {
     const S* at = p + (int64_t)r * ld + k;
-    if (vec && r < rows && k + E <= K) {
-      const AzVec<S, E> v = az_loadv<S, E>(at);
+    if (r < rows && k + E <= K) {
+      const AzVec<S, E> v = az_loadu<S, E>(at);
 #pragma unroll
       for (int e = 0; e < E; ++e) x.v[e] = (C)v.v[e];
       return x;
@@ -148,8 +148,8 @@ __device__ __forceinline__ void few_outputs(const Prod& p, int block, az_f32x4 (
 #pragma unroll 2
   for (int k = wave * 4 * E; k < p.K; k += WAVES * 4 * E) {
     const int at = k + (lane >> 4) * E;
-    const AzPack<C> a = piece<C, SA, AKC>((const SA*)p.a, p.lda, p.M, p.K, m0 + (lane & 15), at, p.a_vec);
-    const AzPack<C> b = piece<C, SB, BKC>((const SB*)p.b, p.ldb, p.N, p.K, n0 + (lane & 15), at, p.b_vec);
+    const AzPack<C> a = piece<C, SA, AKC>((const SA*)p.a, p.lda, p.M, p.K, m0 + (lane & 15), at);
+    const AzPack<C> b = piece<C, SB, BKC>((const SB*)p.b, p.ldb, p.N, p.K, n0 + (lane & 15), at);
     acc = mma(b, a, acc);
   }
   sums[wave][lane] = acc;
@@ -239,7 +239,7 @@ __global__ __launch_bounds__(256) void k_join(Join q, Prod p) {
     for (int e = 0; e < 4; ++e) s[e] += sums[i * groups + g][e];
   if (seg) {
     for (int e = 0; e < have; ++e) ((T*)q.out1)[at + e] = (T)s[e];
-  } else if (p.out_vec) {   // N is a multiple of four: the group is in one row
+  } else if (p.N % 4 == 0) {   // the group is in one row
     finish<T, EPI>(p, (int)(at / p.N), (int)(at % p.N), s);
   } else {
     for (int e = 0; e < have; ++e) {
@@ -267,8 +267,9 @@ __device__ __forceinline__ void planes_of(float x, az_bf16* p) {
   p[2] = (az_bf16)x;
 }
 
-// dz = dy act'(z), rounded to T, and the partial column sums of dz before the rounding: a workgroup takes 64 V
-// columns (V a thread) of a chunk of rows, four rows at a time.
+// dz = dy act'(z), rounded to T, and the partial column sums of dz before the rounding: a workgroup takes 256
+// columns (four a thread) of a chunk of rows, four rows at a time.  Bound by memory: 16384 x 4096 bfloat16 75 us, 403 MB;
+// 8192 x 256 float32 10 us.
 struct Slope {
   const void* dy;
   const void* z;
@@ -281,36 +282,48 @@ struct Slope {
   int ld;              // of dz and the planes: columns N .. ld are set to zero
 };
 
-template <typename T, int V>
+// EXACT: N and ld are multiples of four.
+template <typename T, bool EXACT>
 __global__ __launch_bounds__(256) void k_slope(Slope p) {
   typedef typename Kept<T>::type Z;
+  constexpr int V = 4;
   __shared__ float sums[3][64][V];
   const int g = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int n = (blockIdx.x * 64 + g) * V;
   const int m_end = min(p.M, (int)(blockIdx.y + 1) * p.rows_per_chunk);
+  const int have = min(V, p.N - n), room = p.dz || p.dz32 || p.planes ? min(V, p.ld - n) : 0;   // columns to read, to write
   float s[V] = {};
-  if (n < p.N || ((p.dz || p.planes) && n < p.ld)) {   // (dz32: ld is N)
+  if (have > 0 || room > 0) {
 #pragma unroll 2
     for (int m = blockIdx.y * p.rows_per_chunk + w; m < m_end; m += 4) {
       const int64_t at = (int64_t)m * p.N + n, to = (int64_t)m * p.ld + n;
-      float d[V] = {};
-      if (n < p.N) {
-        const AzVec<T, V> dy = az_loadv<T, V>((const T*)p.dy + at);
-        AzVec<Z, V> z;
-        if (p.act != AZ_ACT_NONE) z = az_loadv<Z, V>((const Z*)p.z + at);
-        for (int i = 0; i < V; ++i) {
-          d[i] = p.act == AZ_ACT_NONE ? (float)dy.v[i] : (float)dy.v[i] * act_slope((float)z.v[i], p.act);
-          s[i] += d[i];
+      float d[V] = {}, z[V] = {};
+      if (EXACT ? have > 0 : have == V) {
+        const AzVec<T, V> dy = az_loadu<T, V>((const T*)p.dy + at);
+        for (int i = 0; i < V; ++i) d[i] = (float)dy.v[i];
+        if (p.act != AZ_ACT_NONE) {
+          const AzVec<Z, V> k = az_loadu<Z, V>((const Z*)p.z + at);
+          for (int i = 0; i < V; ++i) z[i] = (float)k.v[i];
         }
+      } else if (!EXACT) {
+        for (int i = 0; i < V; ++i)
+          if (i < have) {
+            d[i] = (float)((const T*)p.dy)[at + i];
+            if (p.act != AZ_ACT_NONE) z[i] = (float)((const Z*)p.z)[at + i];
+          }
       }
-      if (p.dz32) {
-        for (int i = 0; i < V; ++i) p.dz32[to + i] = d[i];
-      }
-      if (p.dz) {
-        AzVec<T, V> o;
-        for (int i = 0; i < V; ++i) o.v[i] = (T)d[i];
-        az_storev<T, V>((T*)p.dz + to, o);
-      }
+      if (p.act != AZ_ACT_NONE)
+        for (int i = 0; i < V; ++i) d[i] = EXACT || i < have ? d[i] * act_slope(z[i], p.act) : 0.0f;
+      for (int i = 0; i < V; ++i) s[i] += d[i];
+      auto put = [&](auto* out, const auto& vec) {
+        if (EXACT || room == V)
+          az_storeu(out, vec);
+        else
+          for (int i = 0; i < V; ++i)
+            if (i < room) out[i] = vec.v[i];
+      };
+      if (p.dz32) put(p.dz32 + to, AzVec<float, V>{d[0], d[1], d[2], d[3]});
+      if (p.dz) put((T*)p.dz + to, AzVec<T, V>{(T)d[0], (T)d[1], (T)d[2], (T)d[3]});
       if constexpr (sizeof(T) == 4) {
         if (p.planes) {
           AzVec<az_bf16, V> o[3];
@@ -319,7 +332,7 @@ __global__ __launch_bounds__(256) void k_slope(Slope p) {
             planes_of(d[i], q);
             for (int k = 0; k < 3; ++k) o[k].v[i] = q[k];
           }
-          for (int k = 0; k < 3; ++k) az_storev<az_bf16, V>(p.planes + k * p.plane + to, o[k]);
+          for (int k = 0; k < 3; ++k) put(p.planes + k * p.plane + to, o[k]);
         }
       }
     }
@@ -328,9 +341,10 @@ __global__ __launch_bounds__(256) void k_slope(Slope p) {
   if (w > 0)
     for (int i = 0; i < V; ++i) sums[w - 1][g][i] = s[i];
   __syncthreads();
-  if (w > 0 || n >= p.N) return;
+  if (w > 0) return;
   for (int i = 0; i < V; ++i)
-    p.partial[(int64_t)blockIdx.y * p.N + n + i] = ((s[i] + sums[0][g][i]) + sums[1][g][i]) + sums[2][g][i];
+    if (i < have)
+      p.partial[(int64_t)blockIdx.y * p.N + n + i] = ((s[i] + sums[0][g][i]) + sums[1][g][i]) + sums[2][g][i];
 }
 
 // Copies an operand for the wide kernel: rows of `ld` elements, the last ones zero; float32 as planes.
@@ -411,8 +425,9 @@ Plan plan_of(int dtype, int64_t M, int64_t N, int64_t K, bool in_place, int cont
   Plan p = {};
   const double work = (double)M * N * K;
   const bool f32 = dtype == AZ_TYPE_F32;
-  p.few = az_ceil(M, 16) * az_ceil(N, 16) <= 1024 &&
-          K <= (contiguous == 2 ? 4096 : contiguous == 1 ? (f32 ? 4096 : 2048) : 1024);
+  const int64_t pieces = az_ceil(M, 16) * az_ceil(N, 16);
+  p.few = pieces <= 1024 ? K <= (contiguous == 2 ? 4096 : contiguous == 1 ? (f32 ? 4096 : 2048) : 1024)
+                         : pieces <= 2560 && K <= 1024 && !f32 && !in_place;
   p.wide = !p.few && work >= (f32 ? 0x1p31 : in_place ? 0x1p25 : 0x1p29);
   int64_t s = 1;
   if (!p.few && !p.wide) {
@@ -449,19 +464,8 @@ int check(int dtype, int act, int64_t rows, int64_t fan_in, int64_t fan_out) {
   return AZ_OK;
 }
 
-// 16-byte aligned rows, of S elements
-template <typename S>
-bool rows_aligned(const void* p, int64_t ld) {
-  return ld % AzPack<S>::N == 0 && az_aligned16(p);
-}
-
-// Alignments and tiles of a product; the number of tiles.
-template <typename T, typename SA, typename SB>
+// The tiles of a product; their number.
 int64_t prepare(Prod& p, int tile) {
-  p.a_vec = rows_aligned<SA>(p.a, p.lda);
-  p.b_vec = rows_aligned<SB>(p.b, p.ldb);
-  auto four = [](const void* q) { return ((uintptr_t)q & (4 * sizeof(T) - 1)) == 0; };
-  p.out_vec = p.N % 4 == 0 && four(p.out) && four(p.bias) && four(p.residual) && az_aligned16(p.z);
   p.tiles_m = (int)az_ceil(p.M, tile), p.tiles_n = (int)az_ceil(p.N, tile);
   return (int64_t)p.tiles_m * p.tiles_n;
 }
@@ -472,14 +476,14 @@ template <typename T, bool AKC, bool BKC, int EPI, typename SA = T, typename SB 
 int product(Prod p, const Plan& plan, float* partial, const Join* extra, hipStream_t stream) {
   const int pass = EPI == EPI_FORWARD ? PASS_Y : AKC ? PASS_DX : PASS_DW;
   const int dtype = sizeof(T) == 4 ? AZ_TYPE_F32 : std::is_same_v<T, az_bf16> ? AZ_TYPE_BF16 : AZ_TYPE_F16;
-  const int64_t tiles = prepare<T, SA, SB>(p, plan.wide ? (plan.big ? 256 : 128) : plan.few ? 16 : TILE);
+  const int64_t tiles = prepare(p, plan.wide ? (plan.big ? 256 : 128) : plan.few ? 16 : TILE);
   if (!az_grid_fits(tiles, plan.few ? WAVES * 64 : 512) || !az_grid_fits(az_ceil((int64_t)p.M * p.N, 256), 256))
     return az_fail(AZ_ERR_UNSUPPORTED, "dense: %d x %d outputs are too many for one launch", p.M, p.N);
   const int step = plan.wide ? 64 : Stage<T, true>::BK;
   p.k_chunk = (int)(az_ceil(az_ceil(p.K, plan.splits), step) * step);
   const int splits = (int)az_ceil(p.K, p.k_chunk);
   Prod q = p;
-  if (splits > 1) q.partial = partial, q.out_vec = p.N % 4 == 0;
+  if (splits > 1) q.partial = partial;
   if constexpr (!std::is_same_v<SA, SB>) {
     k_product_few<float, SA, SB, T, AKC, BKC, EPI><<<dim3((unsigned)tiles), dim3(WAVES * 64), 0, stream>>>(q);
     AZ_LAUNCH_CHECK();
@@ -537,7 +541,7 @@ Layout layout_of(int dtype, int64_t M, int64_t K, int64_t N, int pass) {
     // float32 (and the products over them, which cost next to nothing, run in float32).
     l.whole = dtype != AZ_TYPE_F32 && (M * N <= 512 || (M * N <= 16384 && l.dx.few && l.dw.few));
     if (l.whole) l.dx = l.dw = Plan{false, false, true, 1};
-    l.chunks = slope_chunks(M, az_ceil(N, 64 * (N % 4 == 0 ? 4 : 1)));
+    l.chunks = slope_chunks(M, az_ceil(N, 256));
     l.dz = room(M * Np * (l.whole ? 4 : size_of(dtype)));
     if (dtype == AZ_TYPE_F32 && (l.dx.wide || l.dw.wide)) l.dz_planes = room(M * Np * 6);
     l.bias = room((int64_t)l.chunks * N * 4);
@@ -652,13 +656,11 @@ extern "C" int az_dense_backward(int32_t dtype, int32_t act, int32_t rows, int32
       if (F32 && wide) s.planes = (az_bf16*)(ws + l.dz_planes), s.plane = rows * ld;
       s.partial = dbias ? (float*)(ws + l.bias) : nullptr;
       s.M = rows, s.N = fan_out, s.act = act, s.rows_per_chunk = (int)az_ceil(rows, l.chunks), s.ld = (int)ld;
-      const bool vec = fan_out % 4 == 0 && ((uintptr_t)dy & (4 * sizeof(T) - 1)) == 0 && az_aligned16(z);
-      const int V = vec ? 4 : 1;
-      const dim3 grid((unsigned)az_ceil(ld, 64 * V), l.chunks), block(256);
-      if (vec)
-        k_slope<T, 4><<<grid, block, 0, stream>>>(s);
+      const dim3 grid((unsigned)az_ceil(ld, 256), l.chunks);
+      if (fan_out % 4 == 0)
+        k_slope<T, true><<<grid, dim3(256), 0, stream>>>(s);
       else
-        k_slope<T, 1><<<grid, block, 0, stream>>>(s);
+        k_slope<T, false><<<grid, dim3(256), 0, stream>>>(s);
       AZ_LAUNCH_CHECK();
     }
     // (the float32 operands of an output that the planes leave not finite)
@@ -674,7 +676,7 @@ extern "C" int az_dense_backward(int32_t dtype, int32_t act, int32_t rows, int32
       operand_b(pw, sdz, nullptr, 0);
       pw.M = fan_in, pw.N = fan_out, pw.K = rows, pw.out = dkernel;
       auto run = [&]<typename C, typename S>() -> int {
-        const int64_t nx = prepare<T, S, T>(px, 16), nw = prepare<T, T, S>(pw, 16);
+        const int64_t nx = prepare(px, 16), nw = prepare(pw, 16);
         const int64_t nb = dbias ? az_ceil(fan_out, 64) : 0;
         if (!az_grid_fits(nx + nw + nb, WAVES * 64)) return az_fail(AZ_ERR_UNSUPPORTED, "dense: too many outputs");
         k_gradients_few<C, S, T><<<dim3((unsigned)(nx + nw + nb)), dim3(WAVES * 64), 0, stream>>>(

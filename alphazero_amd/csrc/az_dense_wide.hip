@@ -230,13 +230,13 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product_wide(Prod p) {
     // the residual of the next rows is loaded while these are worked on: 64 bytes a lane in flight
     constexpr int AHEAD = 8;
     AzVec<TO, 4> next[AHEAD];
-    const bool early = EPI == EPI_FORWARD && p.residual && p.out_vec;
+    const bool early = EPI == EPI_FORWARD && p.residual && n + 4 <= p.N;
     auto fetch = [&](int r0) {
       if (!early) return;
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         const int m = m0 + wm + i0 * 16 + r0 + k * 4 + (lane >> 4);
-        if (m < p.M && n < p.N) next[k] = az_loadv<TO, 4>((const TO*)p.residual + (int64_t)m * p.N + n);
+        if (m < p.M) next[k] = az_loadu<TO, 4>((const TO*)p.residual + (int64_t)m * p.N + n);
       }
     };
     fetch(0);
