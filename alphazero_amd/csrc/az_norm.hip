@@ -4,7 +4,11 @@
 // Bound by memory: the forward pass reads x and writes y once, the backward pass reads x and dy and writes dx once.
 // A row stays in the registers of NT threads between its sums and its outputs, so the variance is taken from the
 // differences to the mean (no cancellation), and the backward pass adds its row's share of the scale's and bias'
-// gradients to registers that a thread keeps for its columns over all rows of its workgroup.
+// gradients to registers that a thread keeps for its columns over all rows of its workgroup.  Up to 1024 columns a wave
+// takes a row, up to 4096 four waves, up to 16384 sixteen: 16 elements a thread, what leaves room for the two gradients.
+// Odd widths are read 16 bytes at a time all the same (gfx950 loads at any address), the row's last piece by elements.
+// 16384 x 4096 bfloat16: forward 58-63 us (268 MB), backward 80 us (402 MB), a large copy 5.2 TB/s; 8191 x 1001
+// float32: 14 and 21 us (66 and 98 MB), with 4 us for the join.
 #include <hip/hip_runtime.h>
 
 #include "az_host.h"

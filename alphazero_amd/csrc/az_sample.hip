@@ -13,6 +13,10 @@
 // up to the cut's, in index order, into a list in LDS; one wave ends the draw on the list while the
 // others make room for the next row.  A row whose list would not fit (ties, a flat distribution) is left to a second
 // kernel that works over the row in memory.
+//
+// 4096 x 32768 float32, top_k 100 and top_p 0.9: 166 us, of which reading the 537 MB takes 126-139 in this form (104 at a
+// large copy's rate: two rows a compute unit are in flight, as many as the registers hold); 4096 x 362 with a mask and
+// top_p: 15 us, the latency of a wave's steps; 64 x 18: 5 us.
 #include <hip/hip_runtime.h>
 
 #include <cfloat>
