@@ -18,20 +18,25 @@ using namespace az_dense;
 namespace {
 
 // ---------------------------------------------------------------------------
-// Any sizes and alignments (gfx950 loads 16 bytes at any address): 64 x 64 outputs a workgroup, four waves of 32 x 32, 256 bytes of reduction a step (64
-// float32 elements, 128 of 16 bits).  Operands go through registers (one step ahead, every element guarded, zero outside)
-// into LDS, each row's reduction contiguous, rows 272 bytes apart so that the 16 rows of an operand read fall on
-// different banks.  A step this long keeps the loads of the next one in flight for two thousand cycles of matrix
-// instructions; with 64 bytes a step the loop waited for memory.  8192 x 256 x 256 float32: 22 us with swish, 17-18 us
-// for the gradients' products (at the rate of a large library product in float32, 150 TFLOP/s, they would take 7 us:
-// at two workgroups a compute unit the four steps' first loads and last stores are not hidden).
-constexpr int TILE = 64, ROW_BYTES = 272, PACKS = 4;
+// Any sizes and alignments (gfx950 loads 16 bytes at any address): 64 x 64 outputs a workgroup, four waves of 32 x 32,
+// 256 bytes of reduction a step (64 float32 elements, 128 of 16 bits).  Operands go through registers (one step ahead,
+// every element guarded, zero outside) into LDS as they lie in memory.  One whose reduction is contiguous: 64 rows, 272
+// bytes apart so that the 16 rows of a read fall on different banks, read 16 bytes a lane.  The other: a row of 64
+// elements for each reduction index, read element by element (float32; rows 320 bytes apart, the four of a read on
+// different banks) or by the transposing read (16 bits; rows 160 bytes apart).  Writing it transposed instead cost as many
+// LDS cycles as the matrix instructions take.  A step this long keeps the loads of the next one in flight for two
+// thousand cycles of matrix instructions; with 64 bytes a step the loop waited for memory.
+constexpr int TILE = 64, PACKS = 4;
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 template <typename T, bool KC>
 struct Stage {
   static constexpr int E = AzPack<T>::N, BK = 4 * PACKS * E;
+  static constexpr int PITCH = KC ? 272 : sizeof(T) == 4 ? 320 : 160, BYTES = PITCH * (KC ? TILE : BK);
   AzPack<T> r[PACKS];
-  // row / first reduction index (KC) or first row / reduction index (not KC) of this thread's pack q
+  // output row / first reduction index (KC) or first output row / reduction index (not KC) of this thread's pack q
   __device__ static int row(int q) {
     return KC ? threadIdx.x / (4 * PACKS) + q * (TILE / PACKS) : (threadIdx.x % (TILE / E)) * E;
   }
@@ -39,6 +44,14 @@ struct Stage {
     return KC ? (threadIdx.x % (4 * PACKS)) * E : threadIdx.x / (TILE / E) + q * (BK / PACKS);
   }
   __device__ void load(const T* p, int64_t ld, int rows, int r0, int k0, int k1) {
+    if (r0 + TILE <= rows && k0 + BK <= k1) {   // the whole step: loads without a branch between them, in flight together
+#pragma unroll
+      for (int q = 0; q < PACKS; ++q) {
+        const int r_ = r0 + row(q), k_ = k0 + red(q);
+        __builtin_memcpy(&r[q], p + (KC ? (int64_t)r_ * ld + k_ : (int64_t)k_ * ld + r_), 16);
+      }
+      return;
+    }
 #pragma unroll
     for (int q = 0; q < PACKS; ++q) {
       const int r_ = r0 + row(q), k_ = k0 + red(q);
@@ -55,34 +68,53 @@ struct Stage {
   }
   __device__ void store(char* lds) const {
 #pragma unroll
-    for (int q = 0; q < PACKS; ++q) {
-      if constexpr (KC) {
-        az_store16((T*)(lds + row(q) * ROW_BYTES) + red(q), r[q]);
-      } else {
+    for (int q = 0; q < PACKS; ++q)
+      az_store16((T*)(lds + (KC ? row(q) : red(q)) * PITCH) + (KC ? red(q) : row(q)), r[q]);
+  }
+  // the 16 rows from r0, 64 bytes of reduction from the q-th on: lane l has row l % 16, those at (l / 16) * 16 bytes
+  __device__ static AzPack<T> fragment(const char* lds, int r0, int q, int lane) {
+    if constexpr (KC) {
+      return az_load16((const T*)(lds + (r0 + (lane & 15)) * PITCH + q * 64 + (lane >> 4) * 16));
+    } else if constexpr (sizeof(T) == 4) {
+      AzPack<T> x;
+      const char* p = lds + (q * 16 + (lane >> 4) * 4) * PITCH + (r0 + (lane & 15)) * 4;
 #pragma unroll
-        for (int e = 0; e < E; ++e) ((T*)(lds + (row(q) + e) * ROW_BYTES))[red(q)] = r[q].v[e];
-      }
+      for (int e = 0; e < 4; ++e) x.v[e] = *reinterpret_cast<const T*>(p + e * PITCH);
+      return x;
+    } else {
+      // the transposing read hands lane i of 16 the i-th column of the four rows of 16 that the lanes point into
+      const char* p = lds + (q * 32 + (lane >> 4) * 8 + ((lane >> 2) & 3)) * PITCH + (r0 + (lane & 3) * 4) * 2;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 4 * PITCH));
+      AzPack<T> x;
+      __builtin_memcpy(&x, &lo, 8);
+      __builtin_memcpy((char*)&x + 8, &hi, 8);
+      return x;
     }
   }
 };
 
 template <typename T, bool AKC, bool BKC, int EPI>
 __global__ __launch_bounds__(256) void k_product_tile(Prod p) {
-  constexpr int BK = Stage<T, true>::BK;
-  __shared__ alignas(16) char lds[2][2][TILE * ROW_BYTES];
+  typedef Stage<T, AKC> StageA;
+  typedef Stage<T, BKC> StageB;
+  constexpr int BK = StageA::BK;
+  __shared__ alignas(16) char lds[2][StageA::BYTES + StageB::BYTES];
   const int m0 = (blockIdx.x % p.tiles_m) * TILE, n0 = (blockIdx.x / p.tiles_m) * TILE;
   const int k_begin = blockIdx.z * p.k_chunk, k_end = min(p.K, k_begin + p.k_chunk);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
-  Stage<T, AKC> sa;
-  Stage<T, BKC> sb;
+  StageA sa;
+  StageB sb;
   az_f32x4 acc[2][2] = {};
   sa.load((const T*)p.a, p.lda, p.M, m0, k_begin, k_end);
   sb.load((const T*)p.b, p.ldb, p.N, n0, k_begin, k_end);
   int buf = 0;
   for (int k = k_begin; k < k_end; k += BK, buf ^= 1) {
-    sa.store(lds[buf][0]);
-    sb.store(lds[buf][1]);
+    char* la = lds[buf];
+    char* lb = la + StageA::BYTES;
+    sa.store(la);
+    sb.store(lb);
     __syncthreads();   // (the other buffer's readers passed the barrier of the step before)
     if (k + BK < k_end) {
       sa.load((const T*)p.a, p.lda, p.M, m0, k + BK, k_end);
@@ -92,11 +124,10 @@ __global__ __launch_bounds__(256) void k_product_tile(Prod p) {
     for (int q = 0; q < PACKS; ++q) {
       if (k + q * (BK / PACKS) >= k_end) break;   // zeros from here on
       AzPack<T> fa[2], fb[2];
-      const int off = (lane & 15) * ROW_BYTES + q * 64 + (lane >> 4) * 16;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        fa[i] = az_load16((const T*)(lds[buf][0] + (wm + i * 16) * ROW_BYTES + off));
-        fb[i] = az_load16((const T*)(lds[buf][1] + (wn + i * 16) * ROW_BYTES + off));
+        fa[i] = StageA::fragment(la, wm + i * 16, q, lane);
+        fb[i] = StageB::fragment(lb, wn + i * 16, q, lane);
       }
       // operands exchanged: a lane then holds four consecutive columns of one output row
 #pragma unroll
@@ -118,40 +149,44 @@ __global__ __launch_bounds__(256) void k_product_tile(Prod p) {
 // into registers, element by element where the reduction is not contiguous.
 constexpr int WAVES = 16;
 
-// C: the type that the matrix instructions take, S: the operand's in memory.
-template <typename C, typename S, bool KC>
-__device__ __forceinline__ AzPack<C> piece(const S* p, int64_t ld, int rows, int K, int r, int k) {
+// C: the type that the matrix instructions take, S: the operand's in memory.  Row r's elements k .. (WHOLE: all of them
+// below K).
+template <typename C, typename S, bool KC, bool WHOLE>
+__device__ __forceinline__ AzPack<C> piece(const S* p, int64_t ld, int K, int r, int k) {
   constexpr int E = AzPack<C>::N;
   AzPack<C> x;
-  if constexpr (KC) {
-    const S* at = p + (int64_t)r * ld + k;
-    if (r < rows && k + E <= K) {
-      const AzVec<S, E> v = az_loadu<S, E>(at);
+  if constexpr (KC && WHOLE) {
+    const AzVec<S, E> v = az_loadu<S, E>(p + (int64_t)r * ld + k);
 #pragma unroll
-      for (int e = 0; e < E; ++e) x.v[e] = (C)v.v[e];
-      return x;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) x.v[e] = r < rows && k + e < K ? (C)at[e] : (C)0.0f;
+    for (int e = 0; e < E; ++e) x.v[e] = (C)v.v[e];
   } else {
+    const S* at = p + (KC ? (int64_t)r * ld + k : (int64_t)k * ld + r);
 #pragma unroll
-    for (int e = 0; e < E; ++e) x.v[e] = r < rows && k + e < K ? (C)p[(int64_t)(k + e) * ld + r] : (C)0.0f;
+    for (int e = 0; e < E; ++e) x.v[e] = WHOLE || k + e < K ? (C)at[KC ? e : e * ld] : (C)0.0f;
   }
   return x;
 }
 
-// One workgroup's 16 x 16 outputs.
+// One workgroup's 16 x 16 outputs.  Rows and columns beyond the edge read the last one's operands and are not stored.
 template <typename C, typename SA, typename SB, typename TO, bool AKC, bool BKC, int EPI>
 __device__ __forceinline__ void few_outputs(const Prod& p, int block, az_f32x4 (*sums)[64]) {
   constexpr int E = AzPack<C>::N;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m0 = (block % p.tiles_m) * 16, n0 = (block / p.tiles_m) * 16;
+  const int m = min(m0 + (lane & 15), p.M - 1), n = min(n0 + (lane & 15), p.N - 1);
   az_f32x4 acc = {};
-#pragma unroll 2
-  for (int k = wave * 4 * E; k < p.K; k += WAVES * 4 * E) {
+  int k = wave * 4 * E;
+#pragma unroll 4
+  for (; k + 4 * E <= p.K; k += WAVES * 4 * E) {
     const int at = k + (lane >> 4) * E;
-    const AzPack<C> a = piece<C, SA, AKC>((const SA*)p.a, p.lda, p.M, p.K, m0 + (lane & 15), at);
-    const AzPack<C> b = piece<C, SB, BKC>((const SB*)p.b, p.ldb, p.N, p.K, n0 + (lane & 15), at);
+    const AzPack<C> a = piece<C, SA, AKC, true>((const SA*)p.a, p.lda, p.K, m, at);
+    const AzPack<C> b = piece<C, SB, BKC, true>((const SB*)p.b, p.ldb, p.K, n, at);
+    acc = mma(b, a, acc);
+  }
+  if (k < p.K) {
+    const int at = k + (lane >> 4) * E;
+    const AzPack<C> a = piece<C, SA, AKC, false>((const SA*)p.a, p.lda, p.K, m, at);
+    const AzPack<C> b = piece<C, SB, BKC, false>((const SB*)p.b, p.ldb, p.K, n, at);
     acc = mma(b, a, acc);
   }
   sums[wave][lane] = acc;
@@ -420,9 +455,10 @@ int64_t splits_for(int64_t tiles, int64_t want, int64_t K, int64_t least) {
 // dkernel of 16384 x 2048 x 2048 in bfloat16 125 (4 splits of 4096) against 149, of 8192 x 2048 x 2048 83 (4 of 2048)
 // against 77; in float32, where every step is six, 389 against 436.
 // Few outputs, up to 1024 tiles of 16 x 16, as long as the reduction is not too long for the waves of one workgroup
-// (k_product_few / the best other form): 64 x 256 x 256 float32 3.4 / 7.3, bfloat16 3.2 / 7.0, 512 x 512 x 512 float32
-// 9.4 / 12.2, 1 x 4096 x 4096 float32 20.7 / 35, bfloat16 dx 8.4 / 10.2 but y (whose second operand it reads element by
-// element) 23 / 11.
+// (k_product_few / the best other form): 64 x 256 x 256 float32 3.2 / 7.1, bfloat16 3.0 / 7.0, 512 x 512 x 512 float32
+// 8.5 / 11.6, 8 x 2048 x 2048 float32 8.2 / 14.3, 8 x 4096 x 4096 bfloat16 dx 8.6 / 12.0 but y (whose second operand it
+// reads element by element) 22.5 / 12.1; up to 2560 tiles of 16-bit operands that the wide kernel would have to copy:
+// 1003 x 401 x 517 15 / 13-15, in fewer launches.
 // in_place: a 16-bit operand need not be copied for the wide kernel.  contiguous: operands with a contiguous reduction.
 Plan plan_of(int dtype, int64_t M, int64_t N, int64_t K, bool in_place, int contiguous) {
   Plan p = {};
