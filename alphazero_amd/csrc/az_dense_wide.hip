@@ -215,9 +215,9 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product_wide(Prod p) {
     interleave();
     __builtin_amdgcn_sched_barrier(0);
   }
-  // The outputs leave through LDS, 64 rows of a wave at a time, so that a row's columns are written together; the
+  // The outputs leave through LDS, up to 64 rows of a wave at a time, so that a row's columns are written together; the
   // sixteen groups of four columns are exchanged by the row, which spreads the rows over the banks.
-  constexpr int ROUND = 4;
+  constexpr int ROUND = FM < 4 ? FM : 4;
   static_assert(FN % 4 == 0 && FM % ROUND == 0 && NW * ROUND * 16 * 64 * 4 <= 2 * STAGE);
   float* out = reinterpret_cast<float*>(lds) + wave * (ROUND * 16 * 64);
   __syncthreads();
@@ -283,6 +283,12 @@ int launch(const Prod& p, bool big, int splits, hipStream_t stream) {
   const dim3 grid(p.tiles_m * p.tiles_n, 1, splits);
   if (big)
     k_product_wide<T, TO, 256, 256, 2, 4, AKC, BKC, EPI, SPLIT><<<grid, dim3(512), 0, stream>>>(p);
+  else if constexpr (AKC && !SPLIT)
+    // Eight waves of 32 x 64: a compute unit with one tile hides more of its latencies than with four of 64 x 64, whose
+    // fewer LDS reads win where both operands take transposing reads (dkernel) and over float32's long reductions:
+    // 2048 x 512 x 512 bfloat16 y 10.6 / 13.3 us, dx 7.5 / 8.5, but dkernel of 4096 x 2048 x 2048 55.5 / 50.8 and float32
+    // y of 4096 x 1024 x 1024 91 / 79
+    k_product_wide<T, TO, 128, 128, 4, 2, AKC, BKC, EPI, SPLIT><<<grid, dim3(512), 0, stream>>>(p);
   else
     k_product_wide<T, TO, 128, 128, 2, 2, AKC, BKC, EPI, SPLIT><<<grid, dim3(256), 0, stream>>>(p);
   AZ_LAUNCH_CHECK();
