@@ -26,6 +26,9 @@ namespace {
 // different banks) or by the transposing read (16 bits; rows 160 bytes apart).  Writing it transposed instead cost as many
 // LDS cycles as the matrix instructions take.  A step this long keeps the loads of the next one in flight for two
 // thousand cycles of matrix instructions; with 64 bytes a step the loop waited for memory.
+// 8192 x 256 x 256 float32: 20.5 us with swish, 16.5 us for dx and, in splits, dkernel (at the rate of a large library
+// product in float32, 150 TFLOP/s, 7 us: with two workgroups a compute unit the first loads and last stores of four steps
+// are not hidden).
 constexpr int TILE = 64, PACKS = 4;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
