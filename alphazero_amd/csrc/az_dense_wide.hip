@@ -14,9 +14,9 @@
 // Bound: 16384 x 4096 x 4096 bfloat16 takes 391-416 us for a plain product (1.3-1.4 PFLOP/s; a library product of that
 // size reaches 1.2), at which the matrix pipes are busy 0.69 of the cycles of a clock that the power limit holds near 2 GHz;
 // the forward pass takes 527 us, its epilogue moving another 400 MB that nothing overlaps (one workgroup a compute unit:
-// two stages are 128 KB).  LDS is busy a quarter of the cycles, without bank conflicts.  Measured and not kept: four waves of 128 x 128 (fewer LDS reads, but
-// one wave a SIMD: 1.83 ms a step instead of 1.52), three to five stages for the 128 x 128 tiles (8192 x 1024 x 1024:
-// 44 us instead of 28: their loads already fill the way from L2, 64 bytes a cycle).
+// two stages are 128 KB).  LDS is busy a quarter of the cycles, without bank conflicts.  Measured and not kept: four
+// waves of 128 x 128 (fewer LDS reads, but one wave a SIMD: 1.83 ms a step instead of 1.52), three to five stages for the
+// 128 x 128 tiles (8192 x 1024 x 1024: 44 us instead of 28: their loads already fill the way from L2, 64 bytes a cycle).
 //
 // float32 products run on the same instructions: an operand is split into three bfloat16 planes x = x0 + x1 + x2
 // (each the rounding of what the planes before it left, so the three hold all 24 bits), and of the nine products the

@@ -7,12 +7,12 @@
 // evenly, then over the order-preserving integer of the logit within the bin that holds the cut, until that bin is a
 // single logit.  Weights are summed as 64-bit integers: the order of the LDS atomics does not matter.
 //
-// Up to 1024 actions a wave takes a row, which it holds in LDS.  Of up to 256 candidates every one is compared with
-// every other: that gives each its place in the descending order and the weight ahead of it at once.  Beyond, a workgroup holds the row in registers (up to
-// 32768 actions; wider rows are read from L2 again), takes the first histogram over it, and moves the actions of the bins
-// up to the cut's, in index order, into a list in LDS; one wave ends the draw on the list while the
-// others make room for the next row.  A row whose list would not fit (ties, a flat distribution) is left to a second
-// kernel that works over the row in memory.
+// Up to 1024 actions a wave takes a row, which it holds in LDS.  Beyond, a workgroup holds the row in registers (up to
+// 32768 actions; wider rows are read from L2 again), takes the first histogram over it -- for top_k over the threads'
+// largest logits alone -- and moves the actions of the bins up to the cut's, in index order, into a list in LDS; one wave
+// ends the draw on the list while the others make room for the next row.  Of up to 256 candidates every one is compared
+// with every other: that gives each its place in the descending order and the weight ahead of it at once.  A row whose
+// list would not fit (ties, a flat distribution) is left to a second kernel that works over the row in memory.
 //
 // 4096 x 32768 float32, top_k 100 and top_p 0.9: 166 us, of which reading the 537 MB takes 126-139 in this form (104 at a
 // large copy's rate: two rows a compute unit are in flight, as many as the registers hold); 4096 x 362 with a mask and

@@ -47,11 +47,6 @@ struct alignas(sizeof(T) * V) AzVec {
 };
 
 template <typename T, int V>
-static __device__ __forceinline__ AzVec<T, V> az_loadv(const T* p) {
-  return *reinterpret_cast<const AzVec<T, V>*>(p);
-}
-
-template <typename T, int V>
 static __device__ __forceinline__ void az_storev(T* p, const AzVec<T, V>& r) {
   *reinterpret_cast<AzVec<T, V>*>(p) = r;
 }

@@ -453,7 +453,7 @@ def check_sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, inva
         assert int(action[b]) == want[0], what
         if want[1] == -math.inf:
             assert float(lp[b]) == -math.inf, what
-        else:   # a float32 of a 64-bit log; the total is a sum of integers at least 2^-42 fine
+        else:   # a float32 of a 64-bit log; the total is a sum of integers at least 2^-41 fine
             assert abs(float(lp[b]) - want[1]) <= U * abs(want[1]) + 1e-9, what
 
 
