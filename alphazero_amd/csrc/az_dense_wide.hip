@@ -23,7 +23,7 @@
 // six that matter, x0 y0, x0 y1, x1 y0, x1 y1, x0 y2, x2 y0, are added in one float32 accumulator, the small ones
 // first.  What is left out is below 2^-26 of the terms' magnitudes.  Six bfloat16 products cost 6 / 16 of
 // the float32 instruction's time.  An infinity or an overflow turns into NaN on the way (inf - inf, inf * 0): an output
-// that is not finite is worked out again from the float32 operands, term by term.
+// that is not finite is worked out again from the float32 operands by the float32 instruction, 16 rows of a wave at a time.
 #include <hip/hip_runtime.h>
 
 #include "az_dense.h"
@@ -231,6 +231,43 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product_wide(Prod p) {
         const int row = i * 16 + (lane & 15), quad = j * 4 + (lane >> 4);
         *reinterpret_cast<az_f32x4*>(out + row * 64 + ((quad ^ (row & 15)) * 4)) = acc[i0 + i][j0 + j];
       }
+    if constexpr (SPLIT) {
+      // outputs that are not finite, 16 rows at a time, from the float32 operands (a row and column beyond the edge
+      // stand for the last one)
+#pragma unroll 1
+      for (int i = 0; i < ROUND; ++i) {
+        const int row = i * 16 + (lane & 15);
+        auto at = [&](int j) {
+          return reinterpret_cast<az_f32x4*>(out + row * 64 + (((j * 4 + (lane >> 4)) ^ (row & 15)) * 4));
+        };
+        bool bad = false;
+        for (int j = 0; j < 4; ++j)
+          for (int e = 0; e < 4; ++e) bad |= !(fabsf((*at(j))[e]) < INFINITY);
+        if (__ballot(bad) == 0) continue;
+        const int64_t m = min(m0 + wm + i0 * 16 + row, p.M - 1);
+        const int k1 = min(p.K, t1 * STEP);
+        az_f32x4 sum[4] = {};
+        for (int k = t0 * STEP; k < k1; k += 16) {
+          const int kk = k + (lane >> 4) * 4;
+          AzPack<float> x;
+          for (int e = 0; e < 4; ++e)
+            x.v[e] = kk + e < k1 ? p.a32[AKC ? m * p.lda32 + kk + e : (kk + e) * p.lda32 + m] : 0.0f;
+          for (int j = 0; j < 4; ++j) {
+            const int64_t n = min(n0 + wn + (j0 + j) * 16 + (lane & 15), p.N - 1);
+            AzPack<float> y;
+            for (int e = 0; e < 4; ++e)
+              y.v[e] = kk + e < k1 ? p.b32[BKC ? n * p.ldb32 + kk + e : (kk + e) * p.ldb32 + n] : 0.0f;
+            sum[j] = mma(y, x, sum[j]);
+          }
+        }
+        for (int j = 0; j < 4; ++j) {
+          az_f32x4 v = *at(j);
+          for (int e = 0; e < 4; ++e)
+            if (!(fabsf(v[e]) < INFINITY)) v[e] = sum[j][e];
+          *at(j) = v;
+        }
+      }
+    }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     __builtin_amdgcn_wave_barrier();
     const int n = n0 + wn + j0 * 16 + (lane & 15) * 4;
@@ -258,18 +295,6 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product_wide(Prod p) {
         const int row = r0 + 4 * k + (lane >> 4), m = m0 + wm + i0 * 16 + row;
         const az_f32x4 x = *reinterpret_cast<const az_f32x4*>(out + row * 64 + (((lane & 15) ^ (row & 15)) * 4));
         float v[4] = {x[0], x[1], x[2], x[3]};
-        if constexpr (SPLIT) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (!(fabsf(v[e]) < INFINITY) && m < p.M && n + e < p.N) {
-              float sum = 0.0f;
-              const int k1 = min(p.K, t1 * STEP);
-              for (int j = t0 * STEP; j < k1; ++j)
-                sum = fmaf(p.a32[AKC ? m * p.lda32 + j : j * p.lda32 + m],
-                           p.b32[BKC ? (n + e) * p.ldb32 + j : j * p.ldb32 + n + e], sum);
-              v[e] = sum;
-            }
-        }
         finish<TO, EPI>(p, m, n, v, early, res[k]);
       }
     }

@@ -198,7 +198,7 @@ def test_dense_shapes_strides_and_streams(T):
 
 
 @pytest.mark.parametrize("T", TYPES, ids=str)
-@pytest.mark.parametrize("M,K,N", [(70, 96, 80), (600, 512, 576)])
+@pytest.mark.parametrize("M,K,N", [(70, 96, 80), (600, 512, 576), (1300, 1304, 1300)])
 def test_dense_non_finite_values_stay_in_their_rows(T, M, K, N):
     """An infinity or NaN of x reaches its own row of y and nothing else, one of the kernel its column."""
     x, w = rand((M, K), T, 1), rand((K, N), T, 2, 0.1)
@@ -229,7 +229,7 @@ def test_dense_non_finite_values_stay_in_their_rows(T, M, K, N):
     assert torch.equal(dw[:, 7].float(), torch.where(x[3].float() > 0, math.inf, -math.inf))
 
 
-@pytest.mark.parametrize("M,K,N", [(70, 96, 80), (600, 512, 576)])
+@pytest.mark.parametrize("M,K,N", [(70, 96, 80), (600, 512, 576), (1300, 1304, 1300)])
 def test_dense_float32_extremes(M, K, N):
     """float32 keeps its range and its precision on values far apart: exact where the sum has one term."""
     x = torch.zeros((M, K), device="cuda")
@@ -768,3 +768,19 @@ def test_dense_split_large_tiles():
     close(dx, g @ wd.t().contiguous(), (N + 4) * U * (g.abs() @ wd.abs().t().contiguous()), torch.float32, "dx")
     xt = xd.t().contiguous()
     close(dw, xt @ g, (M + 4) * U * (xt.abs() @ g.abs()), torch.float32, "dw")
+
+
+def test_dense_of_nothing_but_nan():
+    """A diverged float32 layer: every output of the large products is worked out again, in the time of some steps."""
+    M, K, N = 4096, 1024, 1024
+    x, w = torch.full((M, K), math.nan, device="cuda").requires_grad_(), rand((K, N), torch.float32, 1).requires_grad_()
+    dy = rand((M, N), torch.float32, 2)
+    start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    start.record()
+    y = mctx.dense(x, w, None, "swish")
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    end.record()
+    torch.cuda.synchronize()
+    assert bool(torch.isnan(y).all()) and bool(torch.isnan(dx).all()) and bool(torch.isnan(dw).all())
+    # three products of 4.3e9 multiply-adds: milliseconds; a term-by-term fallback would take tens of seconds
+    assert start.elapsed_time(end) < 1000
