@@ -10,7 +10,7 @@
 // Up to 1024 actions a wave takes a row, which it holds in LDS.  Beyond, a workgroup holds the row in registers (up to
 // 32768 actions; wider rows are read from L2 again), takes the first histogram over it -- for top_k over the threads'
 // largest logits alone -- and moves the actions of the bins up to the cut's, in index order, into a list in LDS; one wave
-// ends the draw on the list while the others make room for the next row.  Of up to 256 candidates every one is compared
+// ends the draw on a short list while the others make room for the next row, all of them on a long one.  Of up to 256 candidates every one is compared
 // with every other: that gives each its place in the descending order and the weight ahead of it at once.  A row whose
 // list would not fit (ties, a flat distribution) is left to a second kernel that works over the row in memory.
 //
@@ -120,18 +120,22 @@ struct MemoryRow {
   }
 };
 
-// in LDS, for one wave
+// in LDS, spread over NT threads
+template <int NT>
 struct ListRow {
-  static constexpr int V = 1, THREADS = 64;
+  static constexpr int V = 1, THREADS = NT;
   const float* l;
   const int* at;    // null: the place itself
   int n, chunks;
+  __device__ __forceinline__ int place(int c) const {
+    return ((NT > 64 ? (threadIdx.x >> 6) * chunks : 0) + c) * 64 + (threadIdx.x & 63);
+  }
   __device__ __forceinline__ int index(int c, int) const {
-    const int j = c * 64 + (threadIdx.x & 63);
+    const int j = place(c);
     return at ? (j < n ? at[j] : 0) : j;
   }
   __device__ __forceinline__ void fetch(int c, float* x) const {
-    const int j = c * 64 + (threadIdx.x & 63);
+    const int j = place(c);
     *x = j < n ? l[j] : -INFINITY;
   }
 };
@@ -595,7 +599,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_sample_wave(az_sample_desc d, in
   if (d.actions <= FEW) {
     r = draw_few(l, nullptr, d.actions, scratch[wave].few, w, o);
   } else {
-    const ListRow row = {l, nullptr, d.actions, (d.actions + 63) / 64};
+    const ListRow<64> row = {l, nullptr, d.actions, (d.actions + 63) / 64};
     Shared<64, NB>& s = scratch[wave].s;
     // the bin that holds the first cut, and the actions up to it (k_sample_group has the same, over more threads)
     const float scale = w.scale(NB);
@@ -671,7 +675,7 @@ template <typename T, int NT, int CHUNKS, bool DIRECT>
 __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_t* action, float* log_prob, double unit) {
   constexpr int V = 16 / sizeof(T), NW = NT / 64;
   __shared__ Shared<NT, DIRECT ? NT : BINS> s;
-  __shared__ Shared<64, DIRECT ? 64 : 256> s1;
+  __shared__ Shared<64, 64> s1;   // (DIRECT)
   __shared__ float list[DIRECT ? 1 : LIST];
   __shared__ int list_at[DIRECT ? 1 : LIST];
   __shared__ FewScratch scratch;
@@ -810,9 +814,14 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
         }
     });
     __syncthreads();
+    if (n > FEW) {
+      const ListRow<NT> row = {list, list_at, n, (n + NT - 1) / NT};
+      const Result r = draw<BINS>(row, s, w, o);
+      if (threadIdx.x == 0) write<T>(d, b, w, r, action, log_prob);
+      return;
+    }
     if (wave > 0) return;
-    const ListRow row = {list, list_at, n, (n + 63) / 64};
-    const Result r = n <= FEW ? draw_few(list, list_at, n, scratch, w, o) : draw<256>(row, s1, w, o);
+    const Result r = draw_few(list, list_at, n, scratch, w, o);
     if (lane == 0) write<T>(d, b, w, r, action, log_prob);
   }
 }
