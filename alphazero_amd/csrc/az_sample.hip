@@ -10,13 +10,14 @@
 // Up to 1024 actions a wave takes a row, which it holds in LDS.  Beyond, a workgroup holds the row in registers (up to
 // 32768 actions; wider rows are read from L2 again), takes the first histogram over it -- for top_k over the threads'
 // largest logits alone -- and moves the actions of the bins up to the cut's, in index order, into a list in LDS; one wave
-// ends the draw on a short list while the others make room for the next row, all of them on a long one.  Of up to 256 candidates every one is compared
-// with every other: that gives each its place in the descending order and the weight ahead of it at once.  A row whose
-// list would not fit (ties, a flat distribution) is left to a second kernel that works over the row in memory.
+// ends the draw on a short list, all of them on a long one.  Of up to 256 candidates every one is compared with every
+// other: that gives each its place in the descending order and the weight ahead of it at once.  A row whose list would
+// not fit (ties, a flat distribution) is left to a second kernel that works over the row in memory.
 //
 // 4096 x 32768 float32, top_k 100 and top_p 0.9: 166 us, of which reading the 537 MB takes 126-139 in this form (104 at a
 // large copy's rate: two rows a compute unit are in flight, as many as the registers hold); 4096 x 362 with a mask and
-// top_p: 15 us, the latency of a wave's steps; 64 x 18: 5 us.
+// top_p: 15 us, the latency of a wave's steps; 64 x 18: 5 us.  Bound by the weights' exponentials in 64 bits instead:
+// top_p alone over 4096 x 32768, 840 us for normal logits of deviation 2.5, 1.9 ms for flat ones.
 #include <hip/hip_runtime.h>
 
 #include <cfloat>
@@ -826,17 +827,17 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
   }
 }
 
-// The rows that k_sample_group left, over the row in memory: a workgroup looks through PER rows.
-template <typename T, int NT, int PER>
-__global__ __launch_bounds__(NT) void k_sample_rest(az_sample_desc d, int32_t* action, float* log_prob, double unit) {
+// The rows that k_sample_group left, over the row in memory: a workgroup looks through `per` rows, up to 64.
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void k_sample_rest(az_sample_desc d, int32_t* action, float* log_prob, double unit,
+                                                    int per) {
   constexpr int V = 16 / sizeof(T), NW = NT / 64;
-  static_assert(PER <= 64);
   __shared__ Shared<NT, BINS> s;
   __shared__ float tops[NW];
-  const int64_t first = (int64_t)blockIdx.x * PER;
+  const int64_t first = (int64_t)blockIdx.x * per;
   // (every wave reads the flags of its own accord; a row's is overwritten behind a barrier that all of them passed)
   const int64_t mine = first + (threadIdx.x & 63);
-  u64 left = __ballot((threadIdx.x & 63) < PER && mine < d.rows && action[mine] == -1);
+  u64 left = __ballot((int)(threadIdx.x & 63) < per && mine < d.rows && action[mine] == -1);
   __syncthreads();
   for (; left; left &= left - 1) {
     const int b = (int)first + __ffsll(left) - 1;
@@ -867,9 +868,11 @@ void launch_group(const az_sample_desc& d, int32_t* action, float* log_prob, dou
   if (direct) {
     k_sample_group<T, 512, CHUNKS, true><<<dim3(d.rows), dim3(512), 0, stream>>>(d, action, log_prob, unit);
   } else {
-    constexpr int PER = 8;
+    // (the rows left are often all or none: a workgroup a row up to 1024, so that all of them share the work; 4096 x
+    // 32768 with top_p alone 842 us against 988 with eight rows a workgroup at every size)
+    const int per = d.rows >= 8192 ? 8 : d.rows >= 1024 ? d.rows / 1024 : 1;
     k_sample_group<T, 512, CHUNKS, false><<<dim3(d.rows), dim3(512), 0, stream>>>(d, action, log_prob, unit);
-    k_sample_rest<T, 512, PER><<<dim3((unsigned)az_ceil(d.rows, PER)), dim3(512), 0, stream>>>(d, action, log_prob, unit);
+    k_sample_rest<T, 512><<<dim3((unsigned)az_ceil(d.rows, per)), dim3(512), 0, stream>>>(d, action, log_prob, unit, per);
   }
 }
 
