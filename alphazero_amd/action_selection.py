@@ -153,6 +153,11 @@ def sample_actions(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0
                 raise ValueError(f"sample_actions: {name} {tuple(value.shape)} must be a number or [{B}]")
             if value.device != logits.device:
                 raise ValueError(f"sample_actions: {name} is on {value.device}, logits on {logits.device}")
+            if name == "top_k":
+                if value.is_floating_point() or value.is_complex():
+                    raise TypeError(f"sample_actions: top_k must hold integers, got {value.dtype}")
+                if value.dtype != dtype:   # (counts beyond 32 bits do not wrap)
+                    value = value.long().clamp(0, A)
             keep.append(value.to(dtype).contiguous())
             setattr(d, name + "_rows", keep[-1].data_ptr())
             values[i] = 0

@@ -550,6 +550,18 @@ def test_sample_actions_parameters_by_row_and_extremes():
     assert a.shape == (0,) and lp.shape == (0,)
 
 
+@pytest.mark.parametrize("A", [18, 400, 1500, 9000, 40000])
+def test_sample_actions_wide_counts_and_endless_temperatures(A):
+    """64-bit counts beyond 32 bits mean all actions; an infinite temperature makes the legal actions equal."""
+    logits = rand((4, A), torch.float32, 2, 2.5)
+    counts = torch.tensor([2 ** 32 + 1, 2 ** 63 - 1, 1, -2 ** 40], device="cuda")
+    check_sample(logits, uniforms(4, 3), top_k=counts)
+    check_sample(logits, uniforms(4, 4), top_k=torch.tensor([0, 1, 2, 255], dtype=torch.uint8, device="cuda"))
+    endless = torch.tensor([math.inf, 1.0, math.inf, 3e38], device="cuda")
+    for kw in (dict(), dict(top_k=3), dict(top_p=0.5), dict(min_p=0.5)):
+        check_sample(logits, uniforms(4, 5), temperature=endless, **kw)
+
+
 def test_sample_actions_follow_the_distribution():
     """2^16 evenly spread uniforms: counts of each action off by at most one from its probability's share."""
     n = 1 << 16

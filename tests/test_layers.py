@@ -133,6 +133,11 @@ def test_native_refusals():
     assert lib.az_sample_actions(C.byref(d), None, None, None) == 0
 
 
+def test_sample_actions_refuses_fractional_counts():
+    with pytest.raises(TypeError, match="top_k"):
+        mctx.sample_actions(t(4, 3), t(4), top_k=torch.full((4,), 1.5))
+
+
 def test_prior_policy_and_networks_refusals():
     from alphazero_amd import networks, trainer
     root = mctx.RootFnOutput(prior_logits=t(4, 3), value=t(4), embedding=None)
