@@ -305,7 +305,10 @@ def prior_policy(params, rng_key, root, invalid_actions=None, *, temperature=1.0
     weights = logits.float()
     if invalid_actions is not None:
         weights = weights.masked_fill(invalid_actions != 0, -torch.inf)
-    weights = torch.nan_to_num(torch.softmax(weights, -1))   # (a row without a legal action: zeros)
+    # as the draw sees them: NaN is illegal, +inf logits share a row, one without a legal action has zeros
+    weights = weights.masked_fill(weights.isnan(), -torch.inf)
+    top = weights.amax(-1, keepdim=True)
+    weights = torch.softmax(torch.where(weights == top, 0.0, weights - top), -1) * (top > -torch.inf)
     return base.PolicyOutput(action=action, action_weights=weights, search_tree=None)
 
 

@@ -719,6 +719,21 @@ def test_prior_policy():
     assert torch.equal(a.action, mctx.sample_actions(logits, u, top_p=0.9)[0])
 
 
+def test_prior_policy_of_special_logits():
+    """The weights follow the draw: NaN and -inf are illegal, +inf logits share the row."""
+    nan, inf = math.nan, math.inf
+    logits = torch.tensor([[0.0, nan, 0.0, -inf], [inf, 1.0, nan, inf], [nan] * 4, [-inf] * 4, [3.0, 3.0, 3.0, 3.0],
+                           [0.0, nan, 0.0, 5.0]], device="cuda")
+    inv = torch.zeros_like(logits)
+    inv[5, 3] = 1
+    root = mctx.RootFnOutput(prior_logits=logits, value=torch.zeros(6, device="cuda"), embedding=None)
+    out = mctx.prior_policy((), 3, root, invalid_actions=inv)
+    want = torch.tensor([[0.5, 0, 0.5, 0], [0.5, 0, 0, 0.5], [0] * 4, [0] * 4, [0.25] * 4, [0.5, 0, 0.5, 0]], device="cuda")
+    assert torch.equal(out.action_weights, want)      # (powers of two: exact)
+    drawn = out.action_weights.gather(1, out.action.long()[:, None])[:, 0]
+    assert bool(((drawn > 0) == (want.sum(1) > 0)).all())
+
+
 @pytest.mark.parametrize("kw", [dict(env_id="CartPole-v1", native_dense=True),
                                 dict(env_id="Breakout-MinAtar", torso="residual", residual_width=64)],
                          ids=["native_dense", "residual_torso"])
