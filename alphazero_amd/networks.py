@@ -153,8 +153,9 @@ class ResidualNetworks:
 
     Takes the networks' place in the learner's functions, as minatar.AtariNetworks does (forward(obs, mean,
     std) and leaves()); observations [..., *obs_shape] or flattened.  Kernels are lecun_uniform (the second one of
-    a block scaled by 1 / sqrt(2 blocks)), biases zero, scales one.  hidden: a block's inner width (default: width).  dtype: of the parameters and the products
-    (float32, bfloat16 or float16); logits and value come back as float32."""
+    a block scaled by 1 / sqrt(2 blocks)), biases zero, scales one.  hidden: a block's inner width (default:
+    width).  dtype: of the parameters and the products (float32, bfloat16 or float16); logits and value come
+    back as float32."""
 
     def __init__(self, obs_size, num_actions, num_atoms=1, width=256, blocks=2, hidden=None, generator=None,
                  device="cuda", dtype=torch.float32):
