@@ -110,34 +110,41 @@ __global__ __launch_bounds__(256) void k_product_tile(Prod p) {
   StageA sa;
   StageB sb;
   az_f32x4 acc[2][2] = {};
-  sa.load((const T*)p.a, p.lda, p.M, m0, k_begin, k_end);
-  sb.load((const T*)p.b, p.ldb, p.N, n0, k_begin, k_end);
   int buf = 0;
-  for (int k = k_begin; k < k_end; k += BK, buf ^= 1) {
-    char* la = lds[buf];
-    char* lb = la + StageA::BYTES;
-    sa.store(la);
-    sb.store(lb);
-    __syncthreads();   // (the other buffer's readers passed the barrier of the step before)
-    if (k + BK < k_end) {
-      sa.load((const T*)p.a, p.lda, p.M, m0, k + BK, k_end);
-      sb.load((const T*)p.b, p.ldb, p.N, n0, k + BK, k_end);
-    }
-#pragma unroll
-    for (int q = 0; q < PACKS; ++q) {
-      if (k + q * (BK / PACKS) >= k_end) break;   // zeros from here on
-      AzPack<T> fa[2], fb[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        fa[i] = StageA::fragment(la, wm + i * 16, q, lane);
-        fb[i] = StageB::fragment(lb, wn + i * 16, q, lane);
+  for (int plane = p.planes - 1; plane >= 0; --plane) {
+    const T* a = (const T*)p.a + plane * p.a_plane;
+    const T* b = (const T*)p.b + plane * p.b_plane;
+    sa.load(a, p.lda, p.M, m0, k_begin, k_end);
+    sb.load(b, p.ldb, p.N, n0, k_begin, k_end);
+    for (int k = k_begin; k < k_end; k += BK, buf ^= 1) {
+      char* la = lds[buf];
+      char* lb = la + StageA::BYTES;
+      sa.store(la);
+      sb.store(lb);
+      __syncthreads();   // (the other buffer's readers passed the barrier of the step before)
+      if (k + BK < k_end) {
+        sa.load(a, p.lda, p.M, m0, k + BK, k_end);
+        sb.load(b, p.ldb, p.N, n0, k + BK, k_end);
       }
-      // operands exchanged: a lane then holds four consecutive columns of one output row
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int q = 0; q < PACKS; ++q) {
+        if (k + q * (BK / PACKS) >= k_end) break;   // zeros from here on
+        AzPack<T> fa[2], fb[2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
+        for (int i = 0; i < 2; ++i) {
+          fa[i] = StageA::fragment(la, wm + i * 16, q, lane);
+          fb[i] = StageB::fragment(lb, wn + i * 16, q, lane);
+        }
+        // operands exchanged: a lane then holds four consecutive columns of one output row
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
+      }
     }
+    if (plane > 0)
+      for (int i = 0; i < 2; ++i)
+        for (int j = 0; j < 2; ++j) scale_low<T>(acc[i][j]);
   }
   for (int i = 0; i < 2; ++i)
     for (int j = 0; j < 2; ++j) {
@@ -152,58 +159,60 @@ __global__ __launch_bounds__(256) void k_product_tile(Prod p) {
 // into registers, element by element where the reduction is not contiguous.
 constexpr int WAVES = 16;
 
-// C: the type that the matrix instructions take, S: the operand's in memory.  Row r's elements k .. (WHOLE: all of them
-// below K).
-template <typename C, typename S, bool KC, bool WHOLE>
-__device__ __forceinline__ AzPack<C> piece(const S* p, int64_t ld, int K, int r, int k) {
-  constexpr int E = AzPack<C>::N;
-  AzPack<C> x;
+// Row r's elements k .. (WHOLE: all of them below K).
+template <typename T, bool KC, bool WHOLE>
+__device__ __forceinline__ AzPack<T> piece(const T* p, int64_t ld, int K, int r, int k) {
+  constexpr int E = AzPack<T>::N;
+  AzPack<T> x;
   if constexpr (KC && WHOLE) {
-    const AzVec<S, E> v = az_loadu<S, E>(p + (int64_t)r * ld + k);
-#pragma unroll
-    for (int e = 0; e < E; ++e) x.v[e] = (C)v.v[e];
+    __builtin_memcpy(&x, p + (int64_t)r * ld + k, 16);   // (at any address)
   } else {
-    const S* at = p + (KC ? (int64_t)r * ld + k : (int64_t)k * ld + r);
+    const T* at = p + (KC ? (int64_t)r * ld + k : (int64_t)k * ld + r);
 #pragma unroll
-    for (int e = 0; e < E; ++e) x.v[e] = WHOLE || k + e < K ? (C)at[KC ? e : e * ld] : (C)0.0f;
+    for (int e = 0; e < E; ++e) x.v[e] = WHOLE || k + e < K ? at[KC ? e : e * ld] : (T)0.0f;
   }
   return x;
 }
 
 // One workgroup's 16 x 16 outputs.  Rows and columns beyond the edge read the last one's operands and are not stored.
-template <typename C, typename SA, typename SB, typename TO, bool AKC, bool BKC, int EPI>
+template <typename T, bool AKC, bool BKC, int EPI>
 __device__ __forceinline__ void few_outputs(const Prod& p, int block, az_f32x4 (*sums)[64]) {
-  constexpr int E = AzPack<C>::N;
+  constexpr int E = AzPack<T>::N;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m0 = (block % p.tiles_m) * 16, n0 = (block / p.tiles_m) * 16;
   const int m = min(m0 + (lane & 15), p.M - 1), n = min(n0 + (lane & 15), p.N - 1);
   az_f32x4 acc = {};
-  int k = wave * 4 * E;
+  for (int plane = p.planes - 1; plane >= 0; --plane) {
+    const T* pa = (const T*)p.a + plane * p.a_plane;
+    const T* pb = (const T*)p.b + plane * p.b_plane;
+    int k = wave * 4 * E;
 #pragma unroll 4
-  for (; k + 4 * E <= p.K; k += WAVES * 4 * E) {
-    const int at = k + (lane >> 4) * E;
-    const AzPack<C> a = piece<C, SA, AKC, true>((const SA*)p.a, p.lda, p.K, m, at);
-    const AzPack<C> b = piece<C, SB, BKC, true>((const SB*)p.b, p.ldb, p.K, n, at);
-    acc = mma(b, a, acc);
-  }
-  if (k < p.K) {
-    const int at = k + (lane >> 4) * E;
-    const AzPack<C> a = piece<C, SA, AKC, false>((const SA*)p.a, p.lda, p.K, m, at);
-    const AzPack<C> b = piece<C, SB, BKC, false>((const SB*)p.b, p.ldb, p.K, n, at);
-    acc = mma(b, a, acc);
+    for (; k + 4 * E <= p.K; k += WAVES * 4 * E) {
+      const int at = k + (lane >> 4) * E;
+      const AzPack<T> a = piece<T, AKC, true>(pa, p.lda, p.K, m, at);
+      const AzPack<T> b = piece<T, BKC, true>(pb, p.ldb, p.K, n, at);
+      acc = mma(b, a, acc);
+    }
+    if (k < p.K) {
+      const int at = k + (lane >> 4) * E;
+      const AzPack<T> a = piece<T, AKC, false>(pa, p.lda, p.K, m, at);
+      const AzPack<T> b = piece<T, BKC, false>(pb, p.ldb, p.K, n, at);
+      acc = mma(b, a, acc);
+    }
+    if (plane > 0) scale_low<T>(acc);
   }
   sums[wave][lane] = acc;
   __syncthreads();
   if (wave > 0) return;
   for (int w = 1; w < WAVES; ++w) acc += sums[w][lane];
   const float v[4] = {acc[0], acc[1], acc[2], acc[3]};
-  finish<TO, EPI>(p, m0 + (lane & 15), n0 + (lane >> 4) * 4, v);
+  finish<T, EPI>(p, m0 + (lane & 15), n0 + (lane >> 4) * 4, v);
 }
 
-template <typename C, typename SA, typename SB, typename TO, bool AKC, bool BKC, int EPI>
+template <typename T, bool AKC, bool BKC, int EPI>
 __global__ __launch_bounds__(WAVES * 64) void k_product_few(Prod p) {
   __shared__ az_f32x4 sums[WAVES][64];
-  few_outputs<C, SA, SB, TO, AKC, BKC, EPI>(p, blockIdx.x, sums);
+  few_outputs<T, AKC, BKC, EPI>(p, blockIdx.x, sums);
 }
 
 // The bias' gradient from `chunks` rows of partial column sums, added in k_join's order: 64 columns a workgroup.
@@ -223,16 +232,16 @@ __device__ __forceinline__ void join_columns(const float* part, int N, int chunk
 }
 
 // All of a small layer's backward pass behind dz in one launch (each launch costs the host three microseconds): dx,
-// then dkernel, then the bias' gradient.  S: the type of dz.
-template <typename C, typename S, typename T>
+// then dkernel, then the bias' gradient.
+template <typename T>
 __global__ __launch_bounds__(WAVES * 64) void k_gradients_few(Prod dx, Prod dw, int dx_blocks, int dw_blocks,
                                                               const float* part, int chunks, T* dbias) {
   __shared__ az_f32x4 sums[WAVES][64];
   const int block = blockIdx.x;
   if (block < dx_blocks)
-    few_outputs<C, S, T, T, true, true, EPI_STORE>(dx, block, sums);
+    few_outputs<T, true, true, EPI_STORE>(dx, block, sums);
   else if (block < dx_blocks + dw_blocks)
-    few_outputs<C, T, S, T, false, false, EPI_STORE>(dw, block - dx_blocks, sums);
+    few_outputs<T, false, false, EPI_STORE>(dw, block - dx_blocks, sums);
   else
     join_columns(part, dw.N, chunks, dbias, block - dx_blocks - dw_blocks, reinterpret_cast<float(*)[64]>(sums));
 }
@@ -296,7 +305,6 @@ __global__ __launch_bounds__(256) void k_join(Join q, Prod p) {
 }
 
 // ---------------------------------------------------------------------------
-// ---------------------------------------------------------------------------
 // The three bfloat16 planes of a float32 value: each the rounding of what is left.  (A value that is not finite has
 // no such planes; the wide kernel works its outputs out again.)
 __device__ __forceinline__ void planes_of(float x, az_bf16* p) {
@@ -307,16 +315,16 @@ __device__ __forceinline__ void planes_of(float x, az_bf16* p) {
   p[2] = (az_bf16)x;
 }
 
-// dz = dy act'(z), rounded to T, and the partial column sums of dz before the rounding: a workgroup takes 256
-// columns (four a thread) of a chunk of rows, four rows at a time.  Bound by memory: 16384 x 4096 bfloat16 75 us, 403 MB;
-// 8192 x 256 float32 10 us.
+// dz = dy act'(z), rounded to T (and, for 16 bits, what that rounding leaves as a second plane), and the partial column sums of
+// dz before the rounding: a workgroup takes 256 columns (four a thread) of a chunk of rows, four rows at a time.  Bound by
+// memory: 16384 x 4096 bfloat16 97 us with both planes, 537 MB; 8192 x 256 float32 10 us.
 struct Slope {
   const void* dy;
   const void* z;
   void* dz;            // may be null (no activation: dy itself is dz)
-  float* dz32;         // dz before the rounding, may be null
   az_bf16* planes;     // float32 only: dz as planes, may be null
-  int64_t plane;
+  int64_t plane;       // elements from one plane to the next
+  bool low;            // 16 bits only: the lo plane too, behind dz
   float* partial;      // [chunks][N], may be null
   int M, N, act, rows_per_chunk;
   int ld;              // of dz and the planes: columns N .. ld are set to zero
@@ -331,7 +339,7 @@ __global__ __launch_bounds__(256) void k_slope(Slope p) {
   const int g = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int n = (blockIdx.x * 64 + g) * V;
   const int m_end = min(p.M, (int)(blockIdx.y + 1) * p.rows_per_chunk);
-  const int have = min(V, p.N - n), room = p.dz || p.dz32 || p.planes ? min(V, p.ld - n) : 0;   // columns to read, to write
+  const int have = min(V, p.N - n), room = p.dz || p.planes ? min(V, p.ld - n) : 0;   // columns to read, to write
   float s[V] = {};
   if (have > 0 || room > 0) {
 #pragma unroll 2
@@ -362,9 +370,18 @@ __global__ __launch_bounds__(256) void k_slope(Slope p) {
           for (int i = 0; i < V; ++i)
             if (i < room) out[i] = vec.v[i];
       };
-      if (p.dz32) put(p.dz32 + to, AzVec<float, V>{d[0], d[1], d[2], d[3]});
-      if (p.dz) put((T*)p.dz + to, AzVec<T, V>{(T)d[0], (T)d[1], (T)d[2], (T)d[3]});
-      if constexpr (sizeof(T) == 4) {
+      const AzVec<T, V> hi = {(T)d[0], (T)d[1], (T)d[2], (T)d[3]};
+      if (p.dz) put((T*)p.dz + to, hi);
+      if constexpr (sizeof(T) == 2) {
+        if (p.low) {
+          AzVec<T, V> lo;   // (exact but for its own rounding; 0 where dz or its rounding is not finite)
+          for (int i = 0; i < V; ++i) {
+            const float h = (float)hi.v[i];
+            lo.v[i] = (T)(fabsf(h) < INFINITY ? (d[i] - h) * Low<T>::UP : 0.0f);
+          }
+          put((T*)p.dz + p.plane + to, lo);
+        }
+      } else {
         if (p.planes) {
           AzVec<az_bf16, V> o[3];
           for (int i = 0; i < V; ++i) {
@@ -512,9 +529,8 @@ int64_t prepare(Prod& p, int tile) {
   return (int64_t)p.tiles_m * p.tiles_n;
 }
 
-// One product (and, with `extra`, the join of the bias' gradient).  `partial` holds splits x M x N floats.  SA, SB: the
-// operands' types where they are not T's (few outputs in float32 arithmetic).
-template <typename T, bool AKC, bool BKC, int EPI, typename SA = T, typename SB = T>
+// One product (and, with `extra`, the join of the bias' gradient).  `partial` holds splits x M x N floats.
+template <typename T, bool AKC, bool BKC, int EPI>
 int product(Prod p, const Plan& plan, float* partial, const Join* extra, hipStream_t stream) {
   const int pass = EPI == EPI_FORWARD ? PASS_Y : AKC ? PASS_DX : PASS_DW;
   const int dtype = sizeof(T) == 4 ? AZ_TYPE_F32 : std::is_same_v<T, az_bf16> ? AZ_TYPE_BF16 : AZ_TYPE_F16;
@@ -526,13 +542,10 @@ int product(Prod p, const Plan& plan, float* partial, const Join* extra, hipStre
   const int splits = (int)az_ceil(p.K, p.k_chunk);
   Prod q = p;
   if (splits > 1) q.partial = partial;
-  if constexpr (!std::is_same_v<SA, SB>) {
-    k_product_few<float, SA, SB, T, AKC, BKC, EPI><<<dim3((unsigned)tiles), dim3(WAVES * 64), 0, stream>>>(q);
-    AZ_LAUNCH_CHECK();
-  } else if (plan.wide) {
+  if (plan.wide) {
     if (int rc = az_product_wide(dtype, pass, splits > 1, plan.big, &q, splits, stream)) return rc;
   } else if (plan.few) {
-    k_product_few<T, T, T, T, AKC, BKC, EPI><<<dim3((unsigned)tiles), dim3(WAVES * 64), 0, stream>>>(q);
+    k_product_few<T, AKC, BKC, EPI><<<dim3((unsigned)tiles), dim3(WAVES * 64), 0, stream>>>(q);
     AZ_LAUNCH_CHECK();
   } else {
     const dim3 grid((unsigned)tiles, 1, splits), block(256);
@@ -559,7 +572,6 @@ int product(Prod p, const Plan& plan, float* partial, const Join* extra, hipStre
 // (always room for them), dz, the partial sums of the bias' gradient, the partial sums of a split product.
 struct Layout {
   Plan y, dx, dw;
-  bool whole;       // dz is not rounded to 16 bits
   int chunks;
   int64_t x, kernel, dz, dz_planes, bias, partial, total;
 };
@@ -579,12 +591,8 @@ Layout layout_of(int dtype, int64_t M, int64_t K, int64_t N, int pass) {
     if (l.y.splits > 1) l.partial = room(l.y.splits * M * N * 4);
   } else {
     l.dx = plan_of(dtype, M, K, N, N % 64 == 0, 2), l.dw = plan_of(dtype, K, N, M, K % 8 == 0 && N % 8 == 0, 0);
-    // Few values of dz would not average out what rounding them to 16 bits takes from the gradients' sums: they stay
-    // float32 (and the products over them, which cost next to nothing, run in float32).
-    l.whole = dtype != AZ_TYPE_F32 && (M * N <= 512 || (M * N <= 16384 && l.dx.few && l.dw.few));
-    if (l.whole) l.dx = l.dw = Plan{false, false, true, 1};
     l.chunks = slope_chunks(M, az_ceil(N, 256));
-    l.dz = room(M * Np * (l.whole ? 4 : size_of(dtype)));
+    l.dz = room(M * Np * 4);   // float32, or two planes of 16 bits
     if (dtype == AZ_TYPE_F32 && (l.dx.wide || l.dw.wide)) l.dz_planes = room(M * Np * 6);
     l.bias = room((int64_t)l.chunks * N * 4);
     if (l.dw.wide) l.x = room(M * Kp * each);
@@ -597,7 +605,7 @@ Layout layout_of(int dtype, int64_t M, int64_t K, int64_t N, int pass) {
 }
 
 // An operand [rows, cols] as the wide kernel reads it: in place, or copied to `to` (float32 always: planes).
-// along: its rows are the reduction's axis and have to be whole steps long.
+// along: its rows are the reduction's axis and have to be whole steps long.  plane: elements between its planes, 0 for one.
 struct Source {
   const void* p;
   int64_t ld, plane;
@@ -611,7 +619,7 @@ int source(const void* src, int64_t rows, int64_t cols, bool along, void* to, hi
   }
   const int64_t ld = round64(cols), threads = rows * (ld / 8);
   if (!az_grid_fits(az_ceil(threads, 256), 256)) return az_fail(AZ_ERR_UNSUPPORTED, "dense: operand too large");
-  *out = {to, ld, rows * ld};
+  *out = {to, ld, sizeof(T) == 4 ? rows * ld : 0};
   k_pack<T><<<dim3((unsigned)az_ceil(threads, 256)), dim3(256), 0, stream>>>((const T*)src, (int)rows, (int)cols,
                                                                              (int)ld, to, rows * ld);
   AZ_LAUNCH_CHECK();
@@ -653,7 +661,7 @@ extern "C" int az_dense_forward(int32_t dtype, int32_t act, int32_t rows, int32_
     }
     operand_a(p, sx, x, fan_in);
     operand_b(p, sk, kernel, fan_out);
-    p.M = rows, p.N = fan_out, p.K = fan_in;
+    p.M = rows, p.N = fan_out, p.K = fan_in, p.planes = 1;
     p.act = act, p.bias = bias, p.residual = residual, p.z = act == AZ_ACT_NONE ? nullptr : z, p.out = y;
     return product<T, true, false, EPI_FORWARD>(p, l.y, (float*)(ws + l.partial), nullptr, stream);
   });
@@ -688,14 +696,15 @@ extern "C" int az_dense_backward(int32_t dtype, int32_t act, int32_t rows, int32
     constexpr bool F32 = sizeof(T) == 4;
     const bool copy = act != AZ_ACT_NONE ||
                       (wide && !F32 && (!az_aligned16(dy) || fan_out % 8 || (wide_dx && fan_out % 64)));
+    // (without an activation or with relu, whose slope is 0 or 1, dz has the 16 bits of dy)
+    const bool low = !F32 && act != AZ_ACT_NONE && act != AZ_ACT_RELU;
     Source sdz = {dy, fan_out, 0}, sdzw = sdz;
-    if (copy) sdz = sdzw = {ws + l.dz, ld, 0};
+    if (copy) sdz = sdzw = {ws + l.dz, ld, low ? rows * ld : 0};
     if (F32 && wide) sdzw = {ws + l.dz_planes, ld, rows * ld};
-    const bool whole = l.whole && copy;   // (without an activation dz is dy, which has 16 bits)
     if (copy || dbias || (F32 && wide)) {
       Slope s = {};
-      s.dy = dy, s.z = z, s.dz = copy && !whole ? ws + l.dz : nullptr, s.dz32 = whole ? (float*)(ws + l.dz) : nullptr;
-      if (F32 && wide) s.planes = (az_bf16*)(ws + l.dz_planes), s.plane = rows * ld;
+      s.dy = dy, s.z = z, s.dz = copy ? ws + l.dz : nullptr, s.plane = rows * ld, s.low = low;
+      if (F32 && wide) s.planes = (az_bf16*)(ws + l.dz_planes);
       s.partial = dbias ? (float*)(ws + l.bias) : nullptr;
       s.M = rows, s.N = fan_out, s.act = act, s.rows_per_chunk = (int)az_ceil(rows, l.chunks), s.ld = (int)ld;
       const dim3 grid((unsigned)az_ceil(ld, 256), l.chunks);
@@ -713,20 +722,17 @@ extern "C" int az_dense_backward(int32_t dtype, int32_t act, int32_t rows, int32
       Prod px = {}, pw = {};
       operand_a(px, sdz, nullptr, 0);
       operand_b(px, Source{kernel, fan_out, 0}, nullptr, 0);
-      px.M = rows, px.N = fan_in, px.K = fan_out, px.out = dx;
+      px.M = rows, px.N = fan_in, px.K = fan_out, px.out = dx, px.planes = 1 + low;
       operand_a(pw, Source{x, fan_in, 0}, nullptr, 0);
       operand_b(pw, sdz, nullptr, 0);
-      pw.M = fan_in, pw.N = fan_out, pw.K = rows, pw.out = dkernel;
-      auto run = [&]<typename C, typename S>() -> int {
-        const int64_t nx = prepare(px, 16), nw = prepare(pw, 16);
-        const int64_t nb = dbias ? az_ceil(fan_out, 64) : 0;
-        if (!az_grid_fits(nx + nw + nb, WAVES * 64)) return az_fail(AZ_ERR_UNSUPPORTED, "dense: too many outputs");
-        k_gradients_few<C, S, T><<<dim3((unsigned)(nx + nw + nb)), dim3(WAVES * 64), 0, stream>>>(
-            px, pw, (int)nx, (int)nw, (const float*)(ws + l.bias), l.chunks, (T*)dbias);
-        AZ_LAUNCH_CHECK();
-        return AZ_OK;
-      };
-      return whole ? run.template operator()<float, float>() : run.template operator()<T, T>();
+      pw.M = fan_in, pw.N = fan_out, pw.K = rows, pw.out = dkernel, pw.planes = 1 + low;
+      const int64_t nx = prepare(px, 16), nw = prepare(pw, 16);
+      const int64_t nb = dbias ? az_ceil(fan_out, 64) : 0;
+      if (!az_grid_fits(nx + nw + nb, WAVES * 64)) return az_fail(AZ_ERR_UNSUPPORTED, "dense: too many outputs");
+      k_gradients_few<T><<<dim3((unsigned)(nx + nw + nb)), dim3(WAVES * 64), 0, stream>>>(
+          px, pw, (int)nx, (int)nw, (const float*)(ws + l.bias), l.chunks, (T*)dbias);
+      AZ_LAUNCH_CHECK();
+      return AZ_OK;
     }
     if (dx) {
       Prod p = {};
@@ -735,10 +741,8 @@ extern "C" int az_dense_backward(int32_t dtype, int32_t act, int32_t rows, int32
         if (int rc = source<T>(kernel, fan_in, fan_out, true, ws + l.kernel, stream, &sk)) return rc;
       operand_a(p, wide_dx ? sdzw : sdz, dz32, ld32);
       operand_b(p, sk, kernel, fan_out);
-      p.M = rows, p.N = fan_in, p.K = fan_out, p.out = dx;
-      if (int rc = whole ? product<T, true, true, EPI_STORE, float, T>(p, l.dx, partial, nullptr, stream)
-                         : product<T, true, true, EPI_STORE>(p, l.dx, partial, nullptr, stream))
-        return rc;
+      p.M = rows, p.N = fan_in, p.K = fan_out, p.out = dx, p.planes = 1 + low;
+      if (int rc = product<T, true, true, EPI_STORE>(p, l.dx, partial, nullptr, stream)) return rc;
     }
     Join j = {};
     j.part[1] = (const float*)(ws + l.bias), j.length[1] = fan_out, j.splits[1] = l.chunks, j.out1 = dbias;
@@ -749,9 +753,8 @@ extern "C" int az_dense_backward(int32_t dtype, int32_t act, int32_t rows, int32
         if (int rc = source<T>(x, rows, fan_in, false, ws + l.x, stream, &sx)) return rc;
       operand_a(p, sx, x, fan_in);
       operand_b(p, wide_dw ? sdzw : sdz, dz32, ld32);
-      p.M = fan_in, p.N = fan_out, p.K = rows, p.out = dkernel;
-      return whole ? product<T, false, false, EPI_STORE, T, float>(p, l.dw, partial, dbias ? &j : nullptr, stream)
-                   : product<T, false, false, EPI_STORE>(p, l.dw, partial, dbias ? &j : nullptr, stream);
+      p.M = fan_in, p.N = fan_out, p.K = rows, p.out = dkernel, p.planes = 1 + low;
+      return product<T, false, false, EPI_STORE>(p, l.dw, partial, dbias ? &j : nullptr, stream);
     }
     if (dbias) {
       k_join<T, EPI_STORE><<<dim3((unsigned)az_ceil(fan_out, 64)), dim3(256), 0, stream>>>(j, Prod{});

@@ -136,8 +136,9 @@ __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int* t
   *tn = in / height;
 }
 
-// T: type of the operands in memory and LDS; TO: of the outputs; SPLIT: T is bfloat16 planes of float32 operands.
-template <typename T, typename TO, int BM, int BN, int WM, int WN, bool AKC, bool BKC, int EPI, bool SPLIT>
+// T: type of the operands in memory and LDS; TO: of the outputs; SPLIT: T is bfloat16 planes of float32 operands; LOW: one
+// operand is dz as a hi and a lo plane.
+template <typename T, typename TO, int BM, int BN, int WM, int WN, bool AKC, bool BKC, int EPI, bool SPLIT, bool LOW>
 __global__ __launch_bounds__(WM* WN * 64, 2) void k_product_wide(Prod p) {
   constexpr int NW = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
   typedef Operand<AKC, BM, NW> OpA;
@@ -154,9 +155,9 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product_wide(Prod p) {
   OpB b;
   a.init(p.a, p.lda, p.M, p.K, m0, wave, lane);
   b.init(p.b, p.ldb, p.N, p.K, n0, wave, lane);
-  // stages of this split; float32 operands go through them once for each pair of planes
+  // stages of this split; float32 operands go through them once for each pair of planes, dz for each of its two
   const int t0 = blockIdx.z * (p.k_chunk / STEP), t1 = min((p.K + STEP - 1) / STEP, t0 + p.k_chunk / STEP);
-  const int stages = (t1 - t0) * (SPLIT ? 6 : 1);
+  const int stages = (t1 - t0) * (SPLIT ? 6 : LOW ? 2 : 1);
   auto load = [&](int s, int buf) {
     int t = t0 + s;
     int64_t pa = 0, pb = 0;
@@ -165,6 +166,12 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product_wide(Prod p) {
       t -= pair * (t1 - t0);
       pa = ((0x011020 >> (20 - 4 * pair)) & 15) * p.a_plane * 2;
       pb = ((0x101002 >> (20 - 4 * pair)) & 15) * p.b_plane * 2;
+    }
+    if constexpr (LOW) {   // the lo plane first
+      if (s < t1 - t0)
+        pa = p.a_plane * 2, pb = p.b_plane * 2;
+      else
+        t -= t1 - t0;
     }
     a.load(t, pa, lds_at + buf * STAGE, wave);
     b.load(t, pb, lds_at + buf * STAGE + OpA::BYTES, wave);
@@ -202,18 +209,30 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product_wide(Prod p) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   read(0, 0);
-  for (int s = 0; s < stages; ++s) {
-    read(s, 1);
-    multiply(0);
-    interleave();
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();   // the next stage is in LDS, and this one's readers are done
-    if (s + 2 < stages) load(s + 2, s & 1);
-    read(s + 1, 0);    // (behind the last stage: read, not used)
-    multiply(1);
-    interleave();
-    __builtin_amdgcn_sched_barrier(0);
+  auto run = [&](int first, int last) {
+    for (int s = first; s < last; ++s) {
+      read(s, 1);
+      multiply(0);
+      interleave();
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();   // the next stage is in LDS, and this one's readers are done
+      if (s + 2 < stages) load(s + 2, s & 1);
+      read(s + 1, 0);    // (behind the last stage: read, not used)
+      multiply(1);
+      interleave();
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  if constexpr (LOW) {
+    run(0, t1 - t0);
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) scale_low<T>(acc[i][j]);
+    run(t1 - t0, stages);
+  } else {
+    run(0, stages);
   }
   // The outputs leave through LDS, up to 64 rows of a wave at a time, so that a row's columns are written together; the
   // sixteen groups of four columns are exchanged by the row, which spreads the rows over the banks.
@@ -303,19 +322,19 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product_wide(Prod p) {
   }
 }
 
-template <typename T, typename TO, bool AKC, bool BKC, int EPI, bool SPLIT>
+template <typename T, typename TO, bool AKC, bool BKC, int EPI, bool SPLIT, bool LOW = false>
 int launch(const Prod& p, bool big, int splits, hipStream_t stream) {
   const dim3 grid(p.tiles_m * p.tiles_n, 1, splits);
   if (big)
-    k_product_wide<T, TO, 256, 256, 2, 4, AKC, BKC, EPI, SPLIT><<<grid, dim3(512), 0, stream>>>(p);
+    k_product_wide<T, TO, 256, 256, 2, 4, AKC, BKC, EPI, SPLIT, LOW><<<grid, dim3(512), 0, stream>>>(p);
   else if constexpr (AKC && !SPLIT)
     // Eight waves of 32 x 64: a compute unit with one tile hides more of its latencies than with four of 64 x 64, whose
     // fewer LDS reads win where both operands take transposing reads (dkernel) and over float32's long reductions:
     // 2048 x 512 x 512 bfloat16 y 10.6 / 13.3 us, dx 7.5 / 8.5, but dkernel of 4096 x 2048 x 2048 55.5 / 50.8 and float32
     // y of 4096 x 1024 x 1024 91 / 79
-    k_product_wide<T, TO, 128, 128, 4, 2, AKC, BKC, EPI, SPLIT><<<grid, dim3(512), 0, stream>>>(p);
+    k_product_wide<T, TO, 128, 128, 4, 2, AKC, BKC, EPI, SPLIT, LOW><<<grid, dim3(512), 0, stream>>>(p);
   else
-    k_product_wide<T, TO, 128, 128, 2, 2, AKC, BKC, EPI, SPLIT><<<grid, dim3(256), 0, stream>>>(p);
+    k_product_wide<T, TO, 128, 128, 2, 2, AKC, BKC, EPI, SPLIT, LOW><<<grid, dim3(256), 0, stream>>>(p);
   AZ_LAUNCH_CHECK();
   return AZ_OK;
 }
@@ -327,6 +346,15 @@ int az_product_wide(int dtype, int pass, bool split_k, bool big, const Prod* p, 
     if (pass == PASS_Y)
       return split_k ? launch<T, TO, true, false, EPI_PARTIAL, SPLIT>(*p, big, splits, stream)
                      : launch<T, TO, true, false, EPI_FORWARD, SPLIT>(*p, big, splits, stream);
+    if constexpr (!SPLIT) {
+      if (p->planes > 1) {
+        if (pass == PASS_DX)
+          return split_k ? launch<T, TO, true, true, EPI_PARTIAL, SPLIT, true>(*p, big, splits, stream)
+                         : launch<T, TO, true, true, EPI_STORE, SPLIT, true>(*p, big, splits, stream);
+        return split_k ? launch<T, TO, false, false, EPI_PARTIAL, SPLIT, true>(*p, big, splits, stream)
+                       : launch<T, TO, false, false, EPI_STORE, SPLIT, true>(*p, big, splits, stream);
+      }
+    }
     if (pass == PASS_DX)
       return split_k ? launch<T, TO, true, true, EPI_PARTIAL, SPLIT>(*p, big, splits, stream)
                      : launch<T, TO, true, true, EPI_STORE, SPLIT>(*p, big, splits, stream);

@@ -46,9 +46,9 @@ int az_dense_forward(int32_t dtype, int32_t act, int32_t rows, int32_t fan_in, i
                      const void* x, const void* kernel, const void* bias, const void* residual, void* y,
                      void* z, void* workspace, int64_t workspace_bytes, void* stream);
 
-/* The gradients of az_dense_forward for dy[rows, fan_out]: with dz = dy act'(z) (rounded to `dtype`
- * for the 16-bit types, whose matrix instructions take it, except where rows x fan_out is a few hundred),
- *   dx = dz kernel^T,  dkernel = x^T dz,  dbias = column sums of dz before that rounding.
+/* The gradients of az_dense_forward for dy[rows, fan_out]: with dz = dy act'(z) (for the 16-bit types, whose
+ * matrix instructions take it, as the sum of two values of that type: to 2^-16 of itself, AZ_TYPE_F16 2^-22),
+ *   dx = dz kernel^T,  dkernel = x^T dz,  dbias = column sums of dz in float32.
  * (the residual's gradient is dy).  Any of dx, dkernel, dbias may be NULL.  x is read for dkernel,
  * kernel for dx, z with an activation.  Sums have a fixed order: results do not depend on timing.
  * rows = 0 sets dkernel and dbias to zero.

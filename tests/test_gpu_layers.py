@@ -811,3 +811,37 @@ def test_dense_of_nothing_but_nan():
     assert bool(torch.isnan(y).all()) and bool(torch.isnan(dx).all()) and bool(torch.isnan(dw).all())
     # three products of 4.3e9 multiply-adds: milliseconds; a term-by-term fallback would take tens of seconds
     assert start.elapsed_time(end) < 1000
+
+
+@pytest.mark.parametrize("T", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("M,K,N", [(64, 256, 256), (300, 520, 264), (1003, 401, 517), (700, 2048, 40), (1024, 1024, 1024),
+                                   (1100, 1032, 1100), (4100, 1032, 4104), (64, 4096, 4096)])
+@pytest.mark.parametrize("act", ["swish", "gelu"])
+def test_dense_gradients_of_16_bits_are_as_exact_as_their_rounding(T, M, K, N, act):
+    """The gradients' errors against those of their last rounding alone, by their norms.  What is added before it: z
+    is kept in float16, off by half a step (at most 2^-11 |z|, of which the root mean square is 0.58 or less, as of any value spread
+    evenly over a step), which moves dz by |dy z act''(z)| as much; dz is kept to 2^-16 of itself at least; float32 sums
+    of n terms are off by less than n 2^-24 of their norm, here 2^-12 of 16-bit steps.  Errors of separate terms have
+    signs of their own, so their squares add up.  1.02 for the scatter of the norms themselves: each has 10^4
+    values or more, whose squares' mean scatters by 1 percent."""
+    x, w = rand((M, K), T, 1).requires_grad_(), rand((K, N), T, 2, K ** -0.5).requires_grad_()
+    b, dy = rand((N,), T, 3), rand((M, N), T, 4)
+    dx, dw = torch.autograd.grad(mctx.dense(x, w, b, act), (x, w), dy)
+    x, w, dy = x.detach().double(), w.detach().double(), dy.double()
+    z = x @ w + b.double()
+    slope = act64(z, act)[1]
+    if act == "swish":
+        p = torch.sigmoid(z)
+        bend = p * (1 - p) * (2 + z * (1 - 2 * p))
+    else:
+        bend = (2 - z * z) * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    dz = dy * slope
+    off = 0.58 * 2.0 ** -11 * (dy * z * bend).abs() + 2.0 ** -16 * dz.abs()
+    sq = off * off
+    for got, want, added in ((dx, dz @ w.t().contiguous(), sq.sum(0) @ (w * w).t().contiguous().sum(1)),
+                             (dw, x.t().contiguous() @ dz, (x * x).sum(1) @ sq.sum(1))):
+        rounding = (want.to(T).double() - want).square().sum()
+        err = (got.double() - want).square().sum()
+        if float(rounding) == 0:
+            continue
+        assert float(err.sqrt()) <= 1.02 * float((rounding + added).sqrt()), (float(err.sqrt()), float(rounding.sqrt()))
