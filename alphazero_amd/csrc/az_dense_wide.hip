@@ -119,6 +119,21 @@ __device__ __forceinline__ uint4 fragment(const char* lds, int r0, int sub, int 
   }
 }
 
+// The pairs of planes of float32 operands, a hexadecimal digit each from the left: (0,2) (2,0) (1,1) (0,1) (1,0) (0,0), so
+// that what is small has been added up before the accumulator has its full size.
+constexpr int PAIRS = 6, A_PLANES = 0x021010, B_PLANES = 0x201100;
+constexpr int plane_of(int planes, int pair) { return (planes >> (4 * (PAIRS - 1 - pair))) & 15; }
+constexpr bool small_first() {
+  int seen = 0;   // a bit for each pair
+  for (int i = 0; i < PAIRS; ++i) {
+    const int a = plane_of(A_PLANES, i), b = plane_of(B_PLANES, i);
+    if (a + b > 2 || (i > 0 && a + b > plane_of(A_PLANES, i - 1) + plane_of(B_PLANES, i - 1))) return false;
+    seen |= 1 << (3 * a + b);
+  }
+  return seen == 0b1011111;
+}
+static_assert(small_first());
+
 template <typename T>
 __device__ __forceinline__ az_f32x4 mma16(uint4 a, uint4 b, az_f32x4 c) {
   return mma(__builtin_bit_cast(AzPack<T>, a), __builtin_bit_cast(AzPack<T>, b), c);
@@ -157,15 +172,15 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void k_product_wide(Prod p) {
   b.init(p.b, p.ldb, p.N, p.K, n0, wave, lane);
   // stages of this split; float32 operands go through them once for each pair of planes, dz for each of its two
   const int t0 = blockIdx.z * (p.k_chunk / STEP), t1 = min((p.K + STEP - 1) / STEP, t0 + p.k_chunk / STEP);
-  const int stages = (t1 - t0) * (SPLIT ? 6 : LOW ? 2 : 1);
+  const int stages = (t1 - t0) * (SPLIT ? PAIRS : LOW ? 2 : 1);
   auto load = [&](int s, int buf) {
     int t = t0 + s;
     int64_t pa = 0, pb = 0;
     if constexpr (SPLIT) {
-      const int pair = s / (t1 - t0);          // (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
+      const int pair = s / (t1 - t0);
       t -= pair * (t1 - t0);
-      pa = ((0x011020 >> (20 - 4 * pair)) & 15) * p.a_plane * 2;
-      pb = ((0x101002 >> (20 - 4 * pair)) & 15) * p.b_plane * 2;
+      pa = plane_of(A_PLANES, pair) * p.a_plane * 2;
+      pb = plane_of(B_PLANES, pair) * p.b_plane * 2;
     }
     if constexpr (LOW) {   // the lo plane first
       if (s < t1 - t0)

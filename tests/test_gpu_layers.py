@@ -845,3 +845,29 @@ def test_dense_gradients_of_16_bits_are_as_exact_as_their_rounding(T, M, K, N, a
         if float(rounding) == 0:
             continue
         assert float(err.sqrt()) <= 1.02 * float((rounding + added).sqrt()), (float(err.sqrt()), float(rounding.sqrt()))
+
+
+@pytest.mark.parametrize("M,N", [(2900, 3000), (4096, 4096)], ids=["tiles of 128", "tiles of 256"])
+def test_dense_float32_planes_are_added_the_small_ones_first(M, N):
+    """Large float32 products on planes of 8 bits, x = x0 + x1 + x2: one term of 2^12, all others +-(1 + 2^-9) + 2^-18,
+    whose first two planes cancel in pairs, times 1.  The third planes' 2046 x 2^-18 are 16 steps of the sum: added up before
+    the first planes they are exact (11 bits) and the sum is rounded once; an accumulator of 2^12 (steps of 2^-11)
+    would swallow 32 x 2^-18 at a time."""
+    K = 2048
+    terms = torch.empty(K, device="cuda")
+    terms[0::2], terms[1::2] = 1 + 2.0 ** -9 + 2.0 ** -18, -(1 + 2.0 ** -9) + 2.0 ** -18
+    terms[0], terms[1] = 2.0 ** 12, 0.0
+    want = 2.0 ** 12 + (K - 2) * 2.0 ** -18
+    one = torch.ones((), device="cuda")
+    a = terms.expand(M, K).contiguous()
+    y = mctx.dense(a, one.expand(K, N).contiguous())
+    assert float((y.double() - want).abs().max()) <= 2.0 ** -11
+    y = mctx.dense(one.expand(M, K).contiguous(), terms.unsqueeze(1).expand(K, N).contiguous())
+    assert float((y.double() - want).abs().max()) <= 2.0 ** -11
+    # the gradients' products: dx of [M, N] over K, dkernel of [M, N] over K
+    x = torch.zeros((M, N), device="cuda", requires_grad=True)
+    (dx,) = torch.autograd.grad(mctx.dense(x, one.expand(N, K).contiguous()), x, a)
+    assert float((dx.double() - want).abs().max()) <= 2.0 ** -11
+    w = torch.zeros((M, N), device="cuda", requires_grad=True)
+    (dw,) = torch.autograd.grad(mctx.dense(a.t().contiguous(), w), w, one.expand(K, N).contiguous())
+    assert float((dw.double() - want).abs().max()) <= 2.0 ** -11
