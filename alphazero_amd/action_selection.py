@@ -125,7 +125,8 @@ def sample_actions(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     probability among the kept ones exceeds `uniform`; log_prob is its log probability among them.  temperature
     divides the logits; 0 takes the largest one.  The four parameters are numbers or [B] tensors (in which a
     negative or NaN temperature counts as 0, top_k <= 0 as all, and top_p, min_p beyond [0, 1] as the nearer end).
-    -inf and NaN logits are illegal; a row without a legal action gives action 0 and log_prob -inf.
+    -inf and NaN logits are illegal; a row without a legal action gives action 0 and log_prob -inf.  Neither output
+    carries a derivative.
     """
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"sample_actions: logits {tuple(logits.shape)} must be [B, A] with A >= 1")

@@ -6,6 +6,8 @@ residual network puts around them, as HIP kernels of libaz_mcts.so (include/az_l
 bfloat16 and float16; sums are held in float32 and an output is rounded once.  There is no CPU path.
 """
 import torch
+from torch.autograd import forward_ad
+from torch.fx.experimental import proxy_tensor
 
 from . import _native as nat
 
@@ -32,8 +34,23 @@ def _native(device, fn, *args):
         nat.check(rc)
 
 
+# Whether torch.jit.trace or, by a dispatch mode, make_fx records the calls: they would see the outputs' allocation alone, and
+# the recorded program would return memory that nothing has written.  (The quick forms of the public questions where there are
+# such: a call costs ten microseconds.)
+_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+_modes = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 1)
+
+
+def _no_tangents(op, *tensors):
+    """Refuses the dual tensors of forward-mode differentiation, whose tangents a native call would drop."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{op}: no forward-mode derivatives")
+
+
 def _checked(op, x, others, same_type=False):
-    """Refuses tensors of other types or devices than the kernels take."""
+    """Refuses tensors of other types or devices than the kernels take, and calls that are being recorded."""
+    if _tracing() or (_modes() and proxy_tensor.get_proxy_mode() is not None):
+        raise NotImplementedError(f"{op}: a native call cannot be traced")
     if x.dtype not in DTYPES:
         raise TypeError(f"{op}: float32, bfloat16 or float16 tensors, got {x.dtype}")
     at = x.get_device()
@@ -75,6 +92,8 @@ def _dense_forward(x, kernel, bias, residual, act, keep_z):
 
 
 def _dense_backward(ctx, dy):
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        _no_tangents("dense", dy)
     x, kernel, z = ctx.saved_tensors
     M, K = x.shape
     N = kernel.shape[1]
@@ -110,7 +129,7 @@ class _Dense(torch.autograd.Function):
 
 
 def dense(x, kernel, bias=None, activation=None, residual=None):
-    """act(x @ kernel + bias) + residual, differentiable in every tensor.
+    """act(x @ kernel + bias) + residual, differentiable (backwards, once) in every tensor.
 
     x [..., fan_in], kernel [fan_in, fan_out], bias [fan_out], residual [..., fan_out] of one type
     (float32, bfloat16 or float16) on one GPU; strided tensors are copied first.
@@ -122,6 +141,8 @@ def dense(x, kernel, bias=None, activation=None, residual=None):
             (bias is not None and bias.shape != (N,)) or \
             (residual is not None and (residual.shape[-1:] != (N,) or residual.shape[:-1] != x.shape[:-1])):
         _refuse_dense(x, kernel, bias, activation, residual)
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        _no_tangents("dense", x, kernel, bias, residual)
     _checked("dense", x, (("kernel", kernel), ("bias", bias), ("residual", residual)), True)
     x2, r2 = _rows(x), None if residual is None else _rows(residual)
     kernel = kernel.contiguous()
@@ -164,6 +185,8 @@ def _norm_forward(x, scale, bias, eps, keep):
 
 
 def _norm_backward(ctx, dy):
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        _no_tangents("layer_norm", dy)
     x, scale, mean, rstd = ctx.saved_tensors
     M, D = x.shape
     need = ctx.needs_input_grad
@@ -197,7 +220,8 @@ class _LayerNorm(torch.autograd.Function):
 
 
 def layer_norm(x, scale=None, bias=None, eps=1e-6):
-    """(x - mean) / sqrt(variance + eps) * scale + bias over the last axis, differentiable in every tensor.
+    """(x - mean) / sqrt(variance + eps) * scale + bias over the last axis, differentiable (backwards, once) in
+    every tensor.
 
     x [..., width] in float32, bfloat16 or float16; scale and bias [width], both of x's type or
     both float32; strided tensors are copied first.
@@ -217,6 +241,8 @@ def layer_norm(x, scale=None, bias=None, eps=1e-6):
     eps = float(eps)
     if not 0.0 <= eps < float("inf"):
         raise ValueError(f"layer_norm: eps {eps}")
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        _no_tangents("layer_norm", x, scale, bias)
     _checked("layer_norm", x, (("scale", scale), ("bias", bias)))
     x2 = _rows(x)
     scale = None if scale is None else scale.contiguous()

@@ -177,3 +177,53 @@ def test_sizes_beyond_the_abi_are_refused():
     assert lib.az_dense_forward(1, 0, 2 ** 31 - 2 ** 16, 1, 2 ** 20, some, some, None, None, some, None, some, 1 << 62, None) == -2
     d = nat.SampleDesc(dtype=0, rows=2 ** 31 - 1, actions=2, logits=4096, uniform=4096)
     assert lib.az_sample_actions(C.byref(d), some, some, None) == -2
+
+
+def test_dual_tensors_are_refused():
+    """Forward-mode differentiation: the tangent is not dropped silently, whichever tensor carries it."""
+    import torch.autograd.forward_ad as forward_ad
+    x, w, b = torch.ones(3, 4), torch.ones(4, 2), torch.ones(2)
+    with forward_ad.dual_level():
+        def dual(v):
+            return forward_ad.make_dual(v, torch.ones_like(v))
+        for args, kw in (((dual(x), w), {}), ((x, dual(w)), {}), ((x, w, dual(b)), {}), ((x, w), dict(residual=dual(t(3, 2)))),
+                         ((dual(x).reshape(1, 3, 4), w), {})):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                mctx.dense(*args, **kw)
+        for args in ((dual(x),), (x, dual(t(4))), (x, t(4), dual(t(4)))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                mctx.layer_norm(*args)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            mctx.dense(dual(x), w)
+        with pytest.raises(NotImplementedError, match="on the GPU"):      # none of them is dual
+            mctx.dense(x, w, b)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(lambda v: mctx.dense(v, w), (x,), (x,))
+
+
+@pytest.mark.parametrize("call", [lambda v: mctx.dense(v, t(4, 2)), lambda v: mctx.layer_norm(v),
+                                  lambda v: mctx.sample_actions(v, t(3))[0]], ids=["dense", "layer_norm", "sample_actions"])
+def test_recorded_calls_are_refused(call):
+    """A trace would hold the outputs' allocation and nothing that writes them."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x = torch.ones(3, 4)
+    with pytest.raises(NotImplementedError, match="traced"):
+        torch.jit.trace(call, (x,))
+    for mode in ("real", "fake"):
+        with pytest.raises(NotImplementedError, match="traced"):
+            make_fx(call, tracing_mode=mode)(x)
+    with pytest.raises(NotImplementedError, match="on the GPU"):
+        call(x)
+
+
+def test_dual_output_gradients_are_refused(monkeypatch):
+    """The same for the backward passes (without their native calls, which this machine need not be able to make)."""
+    import torch.autograd.forward_ad as forward_ad
+    from alphazero_amd import layers
+    monkeypatch.setattr(layers, "_checked", lambda *args: None)
+    monkeypatch.setattr(layers, "_native", lambda *args: None)
+    x, w = torch.ones(3, 4, requires_grad=True), torch.ones(4, 4)
+    for y in (mctx.dense(x, w), mctx.layer_norm(x)):
+        torch.autograd.grad(y, x, torch.ones(3, 4), retain_graph=True)
+        with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(y, x, forward_ad.make_dual(torch.ones(3, 4), torch.ones(3, 4)))
