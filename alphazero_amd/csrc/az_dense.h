@@ -23,10 +23,13 @@ __device__ __forceinline__ float exp_minus(float z) {
 
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + exp_minus(z)); }
 
+// The normal distribution's integral up to z: 1 + erf(z / sqrt 2) would cancel for negative z, down to nothing below -5.6.
+__device__ __forceinline__ float normal_cdf(float z) { return 0.5f * erfcf(z * -0.70710678f); }
+
 __device__ __forceinline__ float act_value(float z, int act) {
   if (act == AZ_ACT_RELU) return z != z ? z : fmaxf(z, 0.0f);
   if (act == AZ_ACT_SWISH) return z * sigmoid(z);
-  if (act == AZ_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
+  if (act == AZ_ACT_GELU) return z * normal_cdf(z);
   return z;
 }
 
@@ -37,7 +40,7 @@ __device__ __forceinline__ float act_slope(float z, int act) {
     return p * (1.0f + z * (1.0f - p));
   }
   if (act == AZ_ACT_GELU)
-    return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * (0.39894228f * exp_minus(0.5f * z * z));
+    return normal_cdf(z) + z * (0.39894228f * exp_minus(0.5f * z * z));
   return 1.0f;
 }
 

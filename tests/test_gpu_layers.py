@@ -871,3 +871,27 @@ def test_dense_float32_planes_are_added_the_small_ones_first(M, N):
     w = torch.zeros((M, N), device="cuda", requires_grad=True)
     (dw,) = torch.autograd.grad(mctx.dense(a.t().contiguous(), w), w, one.expand(K, N).contiguous())
     assert float((dw.double() - want).abs().max()) <= 2.0 ** -11
+
+
+@pytest.mark.parametrize("T", TYPES, ids=str)
+@pytest.mark.parametrize("act,least", [("gelu", -9.0), ("swish", -80.0)])
+def test_dense_activation_tails(T, act, least):
+    """Value and slope keep their relative precision far down the negative side.  One input a row and a kernel of 1, so
+    that z is x itself.  In steps of U: gelu's argument z / sqrt 2 is off by two, which its integral magnifies (z^2 + 1) times;
+    erfc, exp and a reciprocal are off by less than five each, what surrounds them by less than six.  exp(-z^2 / 2) of the
+    slope: an argument of two roundings, z^2 steps.  swish: its exponent is held to less than a step of its result."""
+    x = torch.linspace(least, 0.0, 1009, device="cuda").to(T)
+    z = x.double()
+    xl = x.unsqueeze(1).contiguous().requires_grad_()
+    y = mctx.dense(xl, torch.ones((1, 1), dtype=T, device="cuda"), None, act)
+    (dx,) = torch.autograd.grad(y, xl, torch.ones_like(y))
+    if act == "gelu":
+        cdf = 0.5 * torch.special.erfc(-z / math.sqrt(2.0))
+        density = z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+        want, slope, size, grown = z * cdf, cdf + density, cdf + density.abs(), 2 * z * z
+    else:
+        p = 1 / (1 + torch.exp(-z))
+        want, slope, size, grown = z * p, p * (1 + z * (1 - p)), p * (1 + z.abs()), 0.0
+    close(y.detach()[:, 0], want, (grown + 16) * U * want.abs(), T, "y")
+    # (a 16-bit layer keeps z as float16, which holds x of either type here but for bfloat16's smallest)
+    close(dx[:, 0], slope, (grown + 24) * U * size + (2.0 ** -16 * slope.abs() + 2.0 ** -24 if T != torch.float32 else 0), T, "dx")
