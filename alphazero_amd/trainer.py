@@ -72,10 +72,11 @@ class Config:
     # not in the reference: with one process the minibatch update (loss, gradient, clip + Adam)
     # is captured once in a HIP graph and replayed (learner.GraphedMinibatchStep)
     graph_sgd: bool = True
-    # not in the reference: the learner's MLP layers run as layers.dense instead of library calls
+    # not in the reference: the learner's MLP layers run as layers.dense instead of library calls (the residual
+    # torso's always do; refused with the convolutional one, which has no such form)
     native_dense: bool = False
     # not in the reference: the shared torso for Breakout-MinAtar, "conv" (alphazero.py:246-267) or
-    # "residual" (networks.ResidualNetworks on the flattened observation)
+    # "residual" (networks.ResidualNetworks on the flattened observation, float32); other environments have none
     torso: str = "conv"
     residual_width: int = 256
     residual_blocks: int = 2
@@ -84,6 +85,13 @@ class Config:
 class Trainer:
     def __init__(self, cfg, device=None):
         self.cfg = cfg
+        self.atari = cfg.env_id == "Breakout-MinAtar"
+        if cfg.torso not in ("conv", "residual"):
+            raise ValueError(f"Config.torso {cfg.torso!r} is neither 'conv' nor 'residual'")
+        if cfg.torso != "conv" and not self.atari:
+            raise ValueError(f"Config.torso {cfg.torso!r}: {cfg.env_id} has no torso (Breakout-MinAtar has)")
+        if cfg.native_dense and self.atari and cfg.torso == "conv":
+            raise ValueError("Config.native_dense: the convolutional torso does not run on layers.dense")
         self.rank, self.world, local = parallel.trainer_ranks()
         self.device = torch.device("cuda", local) if device is None else torch.device(device)
         if self.device.type == "cuda":
@@ -95,7 +103,6 @@ class Trainer:
         self.lanes = shard.lanes
         self.key = shard.key
         self.env = envs_lib.make(cfg.env_id, episode_length=cfg.episode_length)
-        self.atari = cfg.env_id == "Breakout-MinAtar"
         # identical initial parameters on every rank (alphazero.py:1305-1326 replicates them)
         g = torch.Generator(device=self.device).manual_seed(cfg.seed)
         if self.atari:
@@ -106,11 +113,9 @@ class Trainer:
             if cfg.torso == "residual":
                 self.policy_layers = networks.ResidualNetworks(
                     obs, act, cfg.num_atoms, cfg.residual_width, cfg.residual_blocks, generator=g, device=self.device)
-            elif cfg.torso == "conv":
+            else:
                 self.policy_layers = minatar.AtariNetworks(act, cfg.num_atoms, tuple(cfg.atari_dense_layer_sizes),
                                                            generator=g, device=self.device)
-            else:
-                raise ValueError(f"Config.torso {cfg.torso!r} is neither 'conv' nor 'residual'")
             self.value_layers = None
             self.model = None
             self.recurrent_fn = minatar.recurrent_fn(self.env, self.policy_layers, cfg.n_step_gamma,

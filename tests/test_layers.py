@@ -227,3 +227,14 @@ def test_dual_output_gradients_are_refused(monkeypatch):
         torch.autograd.grad(y, x, torch.ones(3, 4), retain_graph=True)
         with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(y, x, forward_ad.make_dual(torch.ones(3, 4), torch.ones(3, 4)))
+
+
+@pytest.mark.parametrize("match,kw", [
+    ("native_dense", dict(env_id="Breakout-MinAtar", native_dense=True)),
+    ("has no torso", dict(env_id="CartPole-v1", torso="residual")),
+    ("neither", dict(env_id="CartPole-v1", torso="transformer")),
+])
+def test_trainer_refuses_settings_without_effect(match, kw):
+    from alphazero_amd import trainer
+    with pytest.raises(ValueError, match=match):
+        trainer.Trainer(trainer.Config(**kw), device="cpu")
