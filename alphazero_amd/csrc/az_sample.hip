@@ -284,6 +284,29 @@ __device__ __forceinline__ void count(Shared<NT, NB>& s, int bin, const Weights&
     atomicAdd(reinterpret_cast<uint32_t*>(&s.bins[bin]), 1u);
 }
 
+// Where a top_k cut falls into the last bin, whose actions are never drawn: the weight of those behind its first `kept`, which
+// are out of the weight that top_p is a share of.  Their weights are at most 33 units (2^51 e^-31.875), so the numbers
+// of actions of each weight tell it.  `over(f)` calls f for each legal logit.
+template <int NT, int NB, typename Over>
+__device__ __forceinline__ u64 beyond(Shared<NT, NB>& s, const Weights& w, u64 kept, Over&& over) {
+  const float scale = w.scale(NB);
+  clear(s);
+  over([&](float l) {
+    if (bin_of(w.top, l, scale, NB) == NB - 1) {
+      const u64 m = w.mass(l);
+      atomicAdd(reinterpret_cast<uint32_t*>(&s.bins[m < 63 ? m : 63]), 1u);
+    }
+  });
+  sync<NT>();
+  u64 less = 0;
+  for (int m = 63; m >= 0; --m) {
+    const u64 n = s.bins[m], in = n < kept ? n : kept;
+    kept -= in;
+    less += (n - in) * m;
+  }
+  return less;
+}
+
 // The shortest prefix of the descending order, among logits with a key >= `least`, whose counts (MASS: weights) sum up
 // to the goal; false if there is none (no cut).
 template <bool MASS, int NB, typename Row>
@@ -402,6 +425,7 @@ template <int NB, typename Row>
 __device__ __forceinline__ Result draw(const Row& row, Shared<Row::THREADS, NB>& s, const Weights& w, const Options& o) {
   constexpr int NT = Row::THREADS;
   Cut cut = {0, ~0ull};
+  u64 less = 0;
   auto ties_of = [&](uint32_t key) {
     u64 ties = 0, ahead;
     each(row, [&](float l, int) { ties += key_of(l) == key; });
@@ -409,11 +433,14 @@ __device__ __forceinline__ Result draw(const Row& row, Shared<Row::THREADS, NB>&
   };
   if (o.top_k > 0) {
     Cut c;
-    if (select<false>(row, s, w, (u64)o.top_k, 1.0, 0, 0, &c)) cut = c;
+    if (select<false>(row, s, w, (u64)o.top_k, 1.0, 0, 0, &c))
+      cut = c;
+    else if (s.found == NB - 1 && o.top_p < 1.0 && !o.goal)
+      less = beyond(s, w, (u64)o.top_k - s.found_before, [&](auto&& f) { each(row, [&](float l, int) { f(l); }); });
   }
   if (o.top_p < 1.0) {
     // the weight of the ties at the top_k cut that are out
-    const u64 less = cut.key && !o.goal ? (ties_of(cut.key) - cut.ties) * w.mass(logit_of(cut.key)) : 0;
+    if (cut.key && !o.goal) less = (ties_of(cut.key) - cut.ties) * w.mass(logit_of(cut.key));
     Cut c;
     if (select<true>(row, s, w, o.goal, o.goal ? 1.0 : o.top_p, cut.key, less, &c)) {
       if (c.key > cut.key)
@@ -605,19 +632,22 @@ __global__ __launch_bounds__(64 * WAVES) void k_sample_wave(az_sample_desc d, in
     // the bin that holds the first cut, and the actions up to it (k_sample_group has the same, over more threads)
     const float scale = w.scale(NB);
     int bound = NB;
+    u64 less = 0;
     if (o.top_k > 0) {
       clear(s);
       each(row, [&](float x, int) { count<false>(s, bin_of(top, x, scale, NB), w, x); });
       sync<64>();
       find(s, 0, (u64)o.top_k);
       bound = s.found;
+      if (bound == NB - 1 && o.top_p < 1.0)
+        less = beyond(s, w, (u64)o.top_k - s.found_before, [&](auto&& f) { each(row, [&](float x, int) { f(x); }); });
       if (bound >= NB - 1) bound = NB, o.top_k = 0;   // nothing that could be drawn is cut
     }
     if (bound == NB && o.top_p < 1.0) {
       clear(s);
       each(row, [&](float x, int) { count<true>(s, bin_of(top, x, scale, NB), w, x); });
       sync<64>();
-      o.goal = find(s, 0, 0, o.top_p);
+      o.goal = find(s, 0, 0, o.top_p, less);
       bound = s.found;
     }
     int n = FEW + 1;
@@ -743,6 +773,7 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
     const float scale = w.scale(BINS);
     // the bin that holds the first cut
     int bound = BINS;
+    u64 less = 0;
     if (o.top_k > 0 && o.top_k <= NT) {
       // top_k threads whose largest logits are at or above some logit hold top_k actions there: the histogram of
       // the threads' largest ones gives a bin that is low enough
@@ -764,6 +795,15 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
       __syncthreads();
       find(s, 0, (u64)o.top_k);
       bound = s.found;
+      if (bound == BINS - 1 && o.top_p < 1.0)
+        less = beyond(s, w, (u64)o.top_k - s.found_before, [&](auto&& f) {
+          const float none_ = anew(-INFINITY);
+          front.chunks(memory, [&](int, const float* l) {
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+              if (l[v] > none_) f(l[v]);
+          });
+        });
       if (bound >= BINS - 1) bound = BINS, o.top_k = 0;   // nothing that could be drawn is cut
     }
     if (bound == BINS && o.top_p < 1.0) {
@@ -775,7 +815,7 @@ __global__ __launch_bounds__(NT, 4) void k_sample_group(az_sample_desc d, int32_
           if (l[v] > none) count<true>(s, bin_of(top, l[v], scale_, BINS), w, l[v]);
       });
       __syncthreads();
-      o.goal = find(s, 0, 0, o.top_p);
+      o.goal = find(s, 0, 0, o.top_p, less);
       bound = s.found;
     }
     // the actions up to that bin, in index order, into the list

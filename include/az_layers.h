@@ -90,8 +90,8 @@ int64_t az_layer_norm_workspace_bytes(int32_t rows, int32_t width);
  *
  * Each parameter is a number or, if its pointer is not NULL, one value a row: temperature (0, negative, NaN or
  * below 1e-300: the likeliest action), top_k (<= 0: all), top_p (>= 1 or NaN: all), min_p (<= 0 or NaN: none; above 1 it is 1).
- * Weights are summed as 64-bit integers (unit: the largest weight / 2^41 or finer): draws do not depend on the order of
- * the additions. */
+ * Weights are summed as 64-bit integers (unit: the largest weight / 2^41 or finer; each is rounded to a whole one): draws
+ * do not depend on the order of the additions. */
 typedef struct az_sample_desc {
   int32_t dtype, rows, actions, top_k;
   double temperature, top_p, min_p;

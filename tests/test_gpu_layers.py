@@ -895,3 +895,31 @@ def test_dense_activation_tails(T, act, least):
     close(y.detach()[:, 0], want, (grown + 16) * U * want.abs(), T, "y")
     # (a 16-bit layer keeps z as float16, which holds x of either type here but for bfloat16's smallest)
     close(dx[:, 0], slope, (grown + 24) * U * size + (2.0 ** -16 * slope.abs() + 2.0 ** -24 if T != torch.float32 else 0), T, "dx")
+
+
+@pytest.mark.parametrize("A", [200, 300, 1000, 1500, 9000, 40000])
+def test_sample_actions_share_of_a_top_k_that_ends_far_down(A):
+    """top_p is a share of the top_k's probability also where the top_k ends 32 temperatures below the largest logit,
+    among actions that are never drawn.  They hold f = e^-32 = 1.27e-14 each, and n of them are in the top_k: a share
+    p = 1/2 - d keeps one of the two equal actions in front of them where p (2 + n f) <= 1, and a share of all A - 2 would keep
+    both where p (2 + (A - 2) f) > 1.  Weights are whole multiples of 2^-51 (above 1024 actions up to 2^-46), f of 28.5
+    (0.89, rounded to 1): sums of n of them are off by at most n / 2, so a border has to be that far away.  n = 1 and d = (A - 2) f / 8: 7
+    (0.2) times A - 2 to either side.  n = A / 2 - 2 and d = 3 A f / 16: 3.6 (0.08) times A below, the rounding being
+    in the share's favour by 0.05 A of it, 3.6 (0.16) times A above."""
+    far = math.exp(-32.0)
+    logits = torch.full((2, A), -32.0, device="cuda")
+    logits[:, 3], logits[:, A - 5] = 0.0, 0.0
+    u = torch.tensor([0.75, 0.25], device="cuda")
+    p = 0.5 - (A - 2) * far / 8
+    for T in (torch.float32, torch.float16):
+        check_sample(logits.to(T), u, top_k=3, top_p=p)
+        check_sample(logits.to(T), u, top_k=A // 2, top_p=0.5 - 3 * A * far / 16)
+        check_sample(logits.to(T), u, top_k=0, top_p=p)
+    if A == 40000:
+        # a row whose candidates are more than the list holds, 5000 equal ones: 2500 hold p (5000 + n f) for n = 1 (7000 units
+        # to spare) and do not for n = 35000 (8600, the rounding adding 1900 to them); 20000 would leave 350, less than the rounding
+        logits[:, :] = -32.0
+        logits[:, 100:5100] = 0.0
+        u = torch.tensor([0.9999, 0.5], device="cuda")
+        for k in (5001, 0):
+            check_sample(logits, u, top_k=k, top_p=0.5 - 2e-14)
