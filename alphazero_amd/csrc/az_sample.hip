@@ -78,8 +78,9 @@ struct Weights {
   __device__ __forceinline__ float scale(int bins) const { return (float)fmin(inv_t * (bins / 32), 1e30); }
 };
 
+// (halves, whose difference is finite for any two logits)
 __device__ __forceinline__ int bin_of(float top, float l, float scale, int bins) {
-  return (int)fminf((top - l) * scale, (float)(bins - 1));
+  return (int)fminf(fmaf(l, -0.5f, 0.5f * top) * (2.0f * scale), (float)(bins - 1));
 }
 
 // ---------------------------------------------------------------------------

@@ -923,3 +923,14 @@ def test_sample_actions_share_of_a_top_k_that_ends_far_down(A):
         u = torch.tensor([0.9999, 0.5], device="cuda")
         for k in (5001, 0):
             check_sample(logits, u, top_k=k, top_p=0.5 - 2e-14)
+
+
+@pytest.mark.parametrize("A", [18, 300, 1000, 1500, 9000, 40000])
+def test_sample_actions_logits_further_apart_than_a_float32(A):
+    """Logits whose difference is beyond float32, at temperatures of that size: far apart as numbers, near as weights."""
+    logits = rand((4, A), torch.float32, 1, 1e38).clamp(-3.4e38, 3.4e38)
+    logits[:, 1], logits[:, A - 2] = -3.4e38, 3.4e38
+    temperature = torch.tensor([math.inf, 3e38, 1e38, 2e37], device="cuda")
+    for i, kw in enumerate((dict(), dict(top_k=5), dict(top_k=A - 1), dict(top_p=0.5), dict(top_p=0.99, top_k=A - 2),
+                            dict(min_p=0.1), dict(top_k=A // 2 + 1, top_p=0.9))):
+        check_sample(logits, uniforms(4, 3 + i), temperature=temperature, **kw)
