@@ -474,19 +474,30 @@ int64_t splits_for(int64_t tiles, int64_t want, int64_t K, int64_t least) {
 // its dx 57 against 37 (128 tiles).  With fewer tiles they pay where the splits that fill the compute units stay long:
 // dkernel of 16384 x 2048 x 2048 in bfloat16 125 (4 splits of 4096) against 149, of 8192 x 2048 x 2048 83 (4 of 2048)
 // against 77; in float32, where every step is six, 389 against 436.
-// Few outputs, up to 1024 tiles of 16 x 16, as long as the reduction is not too long for the waves of one workgroup
-// (k_product_few / the best other form): 64 x 256 x 256 float32 3.2 / 7.1, bfloat16 3.0 / 7.0, 512 x 512 x 512 float32
-// 8.5 / 11.6, 8 x 2048 x 2048 float32 8.2 / 14.3, 8 x 4096 x 4096 bfloat16 dx 8.6 / 12.0 but y (whose second operand it
-// reads element by element) 22.5 / 12.1; up to 2560 tiles of 16-bit operands that the wide kernel would have to copy:
-// 1003 x 401 x 517 15 / 13-15, in fewer launches.
+// Few outputs, up to 1024 tiles of 16 x 16, as long as the reduction is not too long for the waves of one workgroup, and for
+// all of them together (k_product_few / the best other form; y reads its second operand element by element): 64 x 256 x 256
+// float32 3.2 / 7.1, bfloat16 3.0 / 7.0, 512 x 512 x 512 float32 9.6 / 11.6, 256 x 1024 x 1024 bfloat16 y 9.1 / 11.5, dx 9.5 /
+// 10.4, 200 x 1500 x 1100 y 13.8 / 19.3, float32 23.5 / 27.9, 8 x 4096 x 4096 bfloat16 dx 8.5 / 11.6 (two planes of dz 17.6 / 19.9,
+// with dz); but 32 x 4096 x 4096 bfloat16 dx 17.1 / 13.7, 128 x 2048 x 2048 y 21 / 11, dx 17 / 9.8 (float32 33 / 21, 31 / 21), 64 x
+// 4096 x 4096 dx 31 / 15 (two planes 64 / 25, float32 59 / 34).
+// Up to 2560 tiles of 16-bit operands that the wide kernel would have to copy, if dx and dkernel are both so small: they then
+// share one launch.  A backward pass that way / on 64 x 64 tiles, relu: 1003 x 401 x 517 32 / 39, 700 x 391 x 900 28 / 37,
+// 1001 x 257 x 600 21 / 35, 2003 x 129 x 301 28 / 30, 611 x 333 x 999 32 / 42; swish 56 / 61, 46 / 58, 35 / 54, 42 / 46, 58 / 73.  With one
+// product alone it does not pay: 1003 x 1003 x 403 50 / 40, 901 x 901 x 450 47 / 38, 515 x 515 x 1111 49 / 45, 1025 x 517 x 401
+// 40 / 35, and for y 16.1 / 13.0 (1001 x 257 x 600), 20.3 / 16.8 (901 x 901 x 450), 12.4 / 10.3 (2003 x 129 x 301), 12.9 / 17.1 (1025 x 517 x 401).
+bool small_pair(int dtype, int64_t M, int64_t N, int64_t K, bool in_place) {
+  return dtype != AZ_TYPE_F32 && !in_place && az_ceil(M, 16) * az_ceil(N, 16) <= 2560 && K <= 1024;
+}
+
 // in_place: a 16-bit operand need not be copied for the wide kernel.  contiguous: operands with a contiguous reduction.
-Plan plan_of(int dtype, int64_t M, int64_t N, int64_t K, bool in_place, int contiguous) {
+// pair: dx and dkernel are both small enough for the launch that they share.
+Plan plan_of(int dtype, int64_t M, int64_t N, int64_t K, bool in_place, int contiguous, bool pair = false) {
   Plan p = {};
   const double work = (double)M * N * K;
   const bool f32 = dtype == AZ_TYPE_F32;
   const int64_t pieces = az_ceil(M, 16) * az_ceil(N, 16);
-  p.few = pieces <= 1024 ? K <= (contiguous == 2 ? 4096 : contiguous == 1 ? (f32 ? 4096 : 2048) : 1024)
-                         : pieces <= 2560 && K <= 1024 && !f32 && !in_place;
+  p.few = pair || (pieces <= 1024 && pieces * K <= 0x180000 &&
+                   K <= (contiguous == 2 ? 4096 : contiguous == 1 ? (f32 ? 4096 : 2048) : 1024));
   p.wide = !p.few && work >= (f32 ? 0x1p31 : in_place ? 0x1p25 : 0x1p29);
   int64_t s = 1;
   if (!p.few && !p.wide) {
@@ -590,7 +601,11 @@ Layout layout_of(int dtype, int64_t M, int64_t K, int64_t N, int pass) {
     if (l.y.wide) l.x = room(M * Kp * each), l.kernel = room(K * Np * each);
     if (l.y.splits > 1) l.partial = room(l.y.splits * M * N * 4);
   } else {
-    l.dx = plan_of(dtype, M, K, N, N % 64 == 0, 2), l.dw = plan_of(dtype, K, N, M, K % 8 == 0 && N % 8 == 0, 0);
+    const bool dx_in_place = N % 64 == 0, dw_in_place = K % 8 == 0 && N % 8 == 0;
+    l.dx = plan_of(dtype, M, K, N, dx_in_place, 2), l.dw = plan_of(dtype, K, N, M, dw_in_place, 0);
+    const bool small_dx = small_pair(dtype, M, K, N, dx_in_place), small_dw = small_pair(dtype, K, N, M, dw_in_place);
+    if ((l.dx.few || small_dx) && (l.dw.few || small_dw))
+      l.dx = plan_of(dtype, M, K, N, dx_in_place, 2, true), l.dw = plan_of(dtype, K, N, M, dw_in_place, 0, true);
     l.chunks = slope_chunks(M, az_ceil(N, 256));
     l.dz = room(M * Np * 4);   // float32, or two planes of 16 bits
     if (dtype == AZ_TYPE_F32 && (l.dx.wide || l.dw.wide)) l.dz_planes = room(M * Np * 6);
