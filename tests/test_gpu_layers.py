@@ -934,3 +934,108 @@ def test_sample_actions_logits_further_apart_than_a_float32(A):
     for i, kw in enumerate((dict(), dict(top_k=5), dict(top_k=A - 1), dict(top_p=0.5), dict(top_p=0.99, top_k=A - 2),
                             dict(min_p=0.1), dict(top_k=A // 2 + 1, top_p=0.9))):
         check_sample(logits, uniforms(4, 3 + i), temperature=temperature, **kw)
+
+
+# ---------------------------------------------------------------- the forms of large layers
+def check_dense_large(x, w, b, r, dy, act, y, grads):
+    """check_dense with 64-bit products on the GPU, and with dz as the kernels keep it: to 2^-16 of itself in a 16-bit layer."""
+    T = x.dtype
+    x, w, dy = (v.detach().double() for v in (x, w, dy))
+    b = torch.zeros(w.shape[1], dtype=torch.float64, device="cuda") if b is None else b.detach().double()
+    (M, K), N = x.shape, w.shape[1]
+    wt, xt = w.t().contiguous(), x.t().contiguous()
+    z = x @ w + b
+    ez = (K + 4) * U * (x.abs() @ w.abs() + b.abs())
+    value, slope, curve = act64(z, act)
+    want = value if r is None else value + r.detach().double()
+    close(y, want, 1.2 * ez + 8 * U * (value.abs() + want.abs()), T, "y")
+    kept = ez + (2.0 ** -11 * z.abs() + 2.0 ** -25 if T != torch.float32 else 0)
+    eslope = (z.abs() <= kept).double() if act == "relu" else curve * kept + 16 * U
+    dz = dy * slope
+    exact = dy.abs() * eslope + 2 * U * dz.abs()
+    edz = exact if act in (None, "relu") or T == torch.float32 else exact + 2.0 ** -16 * (dz.abs() + exact) + TINY[T]
+    dx, dw, db, dr = grads
+    close(dx, dz @ wt, edz @ wt.abs() + (N + 4) * U * (dz.abs() + edz) @ wt.abs(), T, "dx")
+    close(dw, xt @ dz, xt.abs() @ edz + (M + 4) * U * xt.abs() @ (dz.abs() + edz), T, "dw")
+    if db is not None:
+        close(db, dz.sum(0), exact.sum(0) + (M + 4) * U * (dz.abs() + exact).sum(0), T, "db")
+    if dr is not None:
+        assert torch.equal(dr.double(), dy)
+
+
+def step_and_check(T, M, K, N, act, bias=True, res=True, offset=0):
+    """One training step of a layer whose tensors begin `offset` elements behind an aligned address."""
+    def tensor(shape, seed, scale=1.0):
+        n = math.prod(shape)
+        return rand((n + offset,), T, seed, scale)[offset:].view(shape)
+    x, w = tensor((M, K), 1).requires_grad_(), tensor((K, N), 2, K ** -0.5).requires_grad_()
+    b = tensor((N,), 3).requires_grad_() if bias else None
+    r = tensor((M, N), 4).requires_grad_() if res else None
+    dy = tensor((M, N), 5)
+    y = mctx.dense(x, w, b, act, r)
+    g = torch.autograd.grad(y, [t for t in (x, w, b, r) if t is not None], dy)
+    check_dense_large(x, w, b, r, dy, act, y.detach(), (g[0], g[1], g[2] if bias else None, g[-1] if res else None))
+
+
+@pytest.mark.parametrize("T", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("M,K,N,act", [
+    (4200, 328, 4100, "swish"),     # y in tiles of 256 with every edge ragged, operands copied
+    (4200, 320, 4104, "gelu"),      # y in tiles of 256, operands in place
+    (4100, 256, 4104, None),
+    (4200, 4100, 328, "swish"),     # dx
+    (4200, 4104, 320, "relu"),      # dx over one plane of dz
+    (328, 4100, 4200, "swish"),     # dkernel
+    (320, 4104, 4160, None),
+    (16400, 2040, 2000, "gelu"),    # dkernel with its reduction split
+    (16400, 2040, 2000, None),
+])
+def test_dense_of_16_bits_in_large_tiles(T, M, K, N, act):
+    step_and_check(T, M, K, N, act)
+
+
+@pytest.mark.parametrize("M,K,N,act", [(2100, 1032, 1100, "swish"), (2101, 1033, 1101, "gelu"), (2100, 1032, 1100, "relu"),
+                                       (4100, 264, 4104, "swish"), (4104, 4100, 260, "gelu"), (12288, 1000, 1024, "swish")])
+def test_dense_of_float32_planes_with_activations(M, K, N, act):
+    """The large float32 products' epilogue, dz as planes behind a slope, rows of dz padded to whole steps."""
+    step_and_check(torch.float32, M, K, N, act)
+
+
+@pytest.mark.parametrize("T", TYPES, ids=str)
+@pytest.mark.parametrize("M,K,N,act", [(1000, 1024, 768, "swish"), (2100, 1088, 1152, "relu"), (4200, 320, 4160, None),
+                                       (700, 392, 904, "gelu")])
+def test_dense_large_and_not_aligned(T, M, K, N, act):
+    """Sizes whose operands the wide kernel would read in place, one element off."""
+    step_and_check(T, M, K, N, act, offset=1)
+
+
+def test_dense_one_row_is_a_row_of_many():
+    """Another form may serve one row than many: the same sums in another order."""
+    for T in TYPES:
+        x, w, b, r = rand((24, 40), T, 1), rand((40, 24), T, 2, 0.2), rand((24,), T, 3), rand((24, 24), T, 4)
+        many, one = mctx.dense(x, w, b, "swish", r), mctx.dense(x[15], w, b, "swish", r[15])
+        size = x[15].abs().double() @ w.abs().double() + b.abs().double() + r[15].abs().double()
+        # (a slope of swish is at most 1.1; the rounding of either side)
+        close(one, many[15].double(), 2 * 1.2 * 44 * U * size + 8 * U * size + HALF[T] * many[15].double().abs(), T, "row")
+
+
+@pytest.mark.parametrize("B", [2049, 4100, 8195])
+def test_sample_actions_many_rows_left_to_the_second_kernel(B):
+    """Rows that one kernel leaves to the other, of which a workgroup takes several: rows without a cut by their parameters,
+    and equal logits, in turn with rows that are not left; against the same rows in calls of few, and some by the definition."""
+    A = 4500
+    logits = rand((B, A), torch.float32, 1, 2.5)
+    logits[::3] = 1.5
+    u = uniforms(B, 2)
+    at = torch.arange(B, device="cuda")
+    top_p = torch.where(at % 2 == 0, 0.9, 1.0).float()
+    top_k = torch.where(at % 5 == 0, 7, 0).int()
+    logits[B - 2] = -math.inf
+    for kw in (dict(top_p=top_p, top_k=top_k), dict(top_p=0.5), dict(temperature=torch.full((B,), 0.8, device="cuda"))):
+        action, lp = mctx.sample_actions(logits, u, **kw)
+        for first in range(0, B, 500):
+            part = slice(first, first + 500)
+            few = {k: v[part] if torch.is_tensor(v) else v for k, v in kw.items()}
+            a, l = mctx.sample_actions(logits[part], u[part], **few)
+            assert torch.equal(a, action[part]) and torch.equal(l, lp[part])
+        rows = torch.cat([at[:8], at[-8:]])
+        check_sample(logits[rows], u[rows], **{k: v[rows] if torch.is_tensor(v) else v for k, v in kw.items()})
