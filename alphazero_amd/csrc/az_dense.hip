@@ -97,7 +97,8 @@ struct Stage {
   }
 };
 
-template <typename T, bool AKC, bool BKC, int EPI>
+// PLANES: of dz.
+template <typename T, bool AKC, bool BKC, int EPI, int PLANES>
 __global__ __launch_bounds__(256) void k_product_tile(Prod p) {
   typedef Stage<T, AKC> StageA;
   typedef Stage<T, BKC> StageB;
@@ -111,9 +112,7 @@ __global__ __launch_bounds__(256) void k_product_tile(Prod p) {
   StageB sb;
   az_f32x4 acc[2][2] = {};
   int buf = 0;
-  for (int plane = p.planes - 1; plane >= 0; --plane) {
-    const T* a = (const T*)p.a + plane * p.a_plane;
-    const T* b = (const T*)p.b + plane * p.b_plane;
+  auto run = [&](const T* a, const T* b) {
     sa.load(a, p.lda, p.M, m0, k_begin, k_end);
     sb.load(b, p.ldb, p.N, n0, k_begin, k_end);
     for (int k = k_begin; k < k_end; k += BK, buf ^= 1) {
@@ -142,10 +141,13 @@ __global__ __launch_bounds__(256) void k_product_tile(Prod p) {
           for (int j = 0; j < 2; ++j) acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
       }
     }
-    if (plane > 0)
-      for (int i = 0; i < 2; ++i)
-        for (int j = 0; j < 2; ++j) scale_low<T>(acc[i][j]);
+  };
+  if constexpr (PLANES > 1) {
+    run((const T*)p.a + p.a_plane, (const T*)p.b + p.b_plane);
+    for (int i = 0; i < 2; ++i)
+      for (int j = 0; j < 2; ++j) scale_low<T>(acc[i][j]);
   }
+  run((const T*)p.a, (const T*)p.b);
   for (int i = 0; i < 2; ++i)
     for (int j = 0; j < 2; ++j) {
       const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
@@ -175,16 +177,14 @@ __device__ __forceinline__ AzPack<T> piece(const T* p, int64_t ld, int K, int r,
 }
 
 // One workgroup's 16 x 16 outputs.  Rows and columns beyond the edge read the last one's operands and are not stored.
-template <typename T, bool AKC, bool BKC, int EPI>
+template <typename T, bool AKC, bool BKC, int EPI, int PLANES>
 __device__ __forceinline__ void few_outputs(const Prod& p, int block, az_f32x4 (*sums)[64]) {
   constexpr int E = AzPack<T>::N;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int m0 = (block % p.tiles_m) * 16, n0 = (block / p.tiles_m) * 16;
   const int m = min(m0 + (lane & 15), p.M - 1), n = min(n0 + (lane & 15), p.N - 1);
   az_f32x4 acc = {};
-  for (int plane = p.planes - 1; plane >= 0; --plane) {
-    const T* pa = (const T*)p.a + plane * p.a_plane;
-    const T* pb = (const T*)p.b + plane * p.b_plane;
+  auto run = [&](const T* pa, const T* pb) {
     int k = wave * 4 * E;
 #pragma unroll 4
     for (; k + 4 * E <= p.K; k += WAVES * 4 * E) {
@@ -199,8 +199,12 @@ __device__ __forceinline__ void few_outputs(const Prod& p, int block, az_f32x4 (
       const AzPack<T> b = piece<T, BKC, false>(pb, p.ldb, p.K, n, at);
       acc = mma(b, a, acc);
     }
-    if (plane > 0) scale_low<T>(acc);
+  };
+  if constexpr (PLANES > 1) {
+    run((const T*)p.a + p.a_plane, (const T*)p.b + p.b_plane);
+    scale_low<T>(acc);
   }
+  run((const T*)p.a, (const T*)p.b);
   sums[wave][lane] = acc;
   __syncthreads();
   if (wave > 0) return;
@@ -209,10 +213,10 @@ __device__ __forceinline__ void few_outputs(const Prod& p, int block, az_f32x4 (
   finish<T, EPI>(p, m0 + (lane & 15), n0 + (lane >> 4) * 4, v);
 }
 
-template <typename T, bool AKC, bool BKC, int EPI>
+template <typename T, bool AKC, bool BKC, int EPI, int PLANES>
 __global__ __launch_bounds__(WAVES * 64) void k_product_few(Prod p) {
   __shared__ az_f32x4 sums[WAVES][64];
-  few_outputs<T, AKC, BKC, EPI>(p, blockIdx.x, sums);
+  few_outputs<T, AKC, BKC, EPI, PLANES>(p, blockIdx.x, sums);
 }
 
 // The bias' gradient from `chunks` rows of partial column sums, added in k_join's order: 64 columns a workgroup.
@@ -233,15 +237,15 @@ __device__ __forceinline__ void join_columns(const float* part, int N, int chunk
 
 // All of a small layer's backward pass behind dz in one launch (each launch costs the host three microseconds): dx,
 // then dkernel, then the bias' gradient.
-template <typename T>
+template <typename T, int PLANES>
 __global__ __launch_bounds__(WAVES * 64) void k_gradients_few(Prod dx, Prod dw, int dx_blocks, int dw_blocks,
                                                               const float* part, int chunks, T* dbias) {
   __shared__ az_f32x4 sums[WAVES][64];
   const int block = blockIdx.x;
   if (block < dx_blocks)
-    few_outputs<T, true, true, EPI_STORE>(dx, block, sums);
+    few_outputs<T, true, true, EPI_STORE, PLANES>(dx, block, sums);
   else if (block < dx_blocks + dw_blocks)
-    few_outputs<T, false, false, EPI_STORE>(dw, block - dx_blocks, sums);
+    few_outputs<T, false, false, EPI_STORE, PLANES>(dw, block - dx_blocks, sums);
   else
     join_columns(part, dw.N, chunks, dbias, block - dx_blocks - dw_blocks, reinterpret_cast<float(*)[64]>(sums));
 }
@@ -553,17 +557,26 @@ int product(Prod p, const Plan& plan, float* partial, const Join* extra, hipStre
   const int splits = (int)az_ceil(p.K, p.k_chunk);
   Prod q = p;
   if (splits > 1) q.partial = partial;
+  auto run = [&]<int PLANES>() {
+    if (plan.few) {
+      k_product_few<T, AKC, BKC, EPI, PLANES><<<dim3((unsigned)tiles), dim3(WAVES * 64), 0, stream>>>(q);
+    } else {
+      const dim3 grid((unsigned)tiles, 1, splits), block(256);
+      if (splits == 1)
+        k_product_tile<T, AKC, BKC, EPI, PLANES><<<grid, block, 0, stream>>>(q);
+      else
+        k_product_tile<T, AKC, BKC, EPI_PARTIAL, PLANES><<<grid, block, 0, stream>>>(q);
+    }
+  };
   if (plan.wide) {
     if (int rc = az_product_wide(dtype, pass, splits > 1, plan.big, &q, splits, stream)) return rc;
-  } else if (plan.few) {
-    k_product_few<T, AKC, BKC, EPI><<<dim3((unsigned)tiles), dim3(WAVES * 64), 0, stream>>>(q);
-    AZ_LAUNCH_CHECK();
   } else {
-    const dim3 grid((unsigned)tiles, 1, splits), block(256);
-    if (splits == 1)
-      k_product_tile<T, AKC, BKC, EPI><<<grid, block, 0, stream>>>(q);
-    else
-      k_product_tile<T, AKC, BKC, EPI_PARTIAL><<<grid, block, 0, stream>>>(q);
+    bool two = false;
+    if constexpr (sizeof(T) == 2 && EPI == EPI_STORE) {
+      two = p.planes > 1;
+      if (two) run.template operator()<2>();
+    }
+    if (!two) run.template operator()<1>();
     AZ_LAUNCH_CHECK();
   }
   if (splits > 1 || extra) {
@@ -737,15 +750,23 @@ extern "C" int az_dense_backward(int32_t dtype, int32_t act, int32_t rows, int32
       Prod px = {}, pw = {};
       operand_a(px, sdz, nullptr, 0);
       operand_b(px, Source{kernel, fan_out, 0}, nullptr, 0);
-      px.M = rows, px.N = fan_in, px.K = fan_out, px.out = dx, px.planes = 1 + low;
+      px.M = rows, px.N = fan_in, px.K = fan_out, px.out = dx;
       operand_a(pw, Source{x, fan_in, 0}, nullptr, 0);
       operand_b(pw, sdz, nullptr, 0);
-      pw.M = fan_in, pw.N = fan_out, pw.K = rows, pw.out = dkernel, pw.planes = 1 + low;
+      pw.M = fan_in, pw.N = fan_out, pw.K = rows, pw.out = dkernel;
       const int64_t nx = prepare(px, 16), nw = prepare(pw, 16);
       const int64_t nb = dbias ? az_ceil(fan_out, 64) : 0;
       if (!az_grid_fits(nx + nw + nb, WAVES * 64)) return az_fail(AZ_ERR_UNSUPPORTED, "dense: too many outputs");
-      k_gradients_few<T><<<dim3((unsigned)(nx + nw + nb)), dim3(WAVES * 64), 0, stream>>>(
-          px, pw, (int)nx, (int)nw, (const float*)(ws + l.bias), l.chunks, (T*)dbias);
+      auto run = [&]<int PLANES>() {
+        k_gradients_few<T, PLANES><<<dim3((unsigned)(nx + nw + nb)), dim3(WAVES * 64), 0, stream>>>(
+            px, pw, (int)nx, (int)nw, (const float*)(ws + l.bias), l.chunks, (T*)dbias);
+      };
+      if constexpr (F32)
+        run.template operator()<1>();
+      else if (low)
+        run.template operator()<2>();
+      else
+        run.template operator()<1>();
       AZ_LAUNCH_CHECK();
       return AZ_OK;
     }
