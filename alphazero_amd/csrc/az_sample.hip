@@ -79,8 +79,12 @@ struct Weights {
 };
 
 // (halves, whose difference is finite for any two logits)
+__device__ __forceinline__ float place_of(float top, float l, float scale) {
+  return fmaf(l, -0.5f, 0.5f * top) * (2.0f * scale);
+}
+
 __device__ __forceinline__ int bin_of(float top, float l, float scale, int bins) {
-  return (int)fminf(fmaf(l, -0.5f, 0.5f * top) * (2.0f * scale), (float)(bins - 1));
+  return (int)fminf(place_of(top, l, scale), (float)(bins - 1));
 }
 
 // ---------------------------------------------------------------------------
@@ -287,15 +291,17 @@ __device__ __forceinline__ void count(Shared<NT, NB>& s, int bin, const Weights&
 
 // Where a top_k cut falls into the last bin, whose actions are never drawn: the weight of those behind its first `kept`, which
 // are out of the weight that top_p is a share of.  Their weights are at most 33 units (2^51 e^-31.875), so the numbers
-// of actions of each weight tell it.  `over(f)` calls f for each legal logit.
+// of actions of each weight tell it; from 38 temperatures on they are none (2^51 e^-38 < 1 / 2).  `over(f)` calls f for
+// each legal logit.
 template <int NT, int NB, typename Over>
 __device__ __forceinline__ u64 beyond(Shared<NT, NB>& s, const Weights& w, u64 kept, Over&& over) {
   const float scale = w.scale(NB);
   clear(s);
   over([&](float l) {
-    if (bin_of(w.top, l, scale, NB) == NB - 1) {
+    const float at = place_of(w.top, l, scale);
+    if (at >= NB - 1 && at < 38.0f * (NB / 32)) {
       const u64 m = w.mass(l);
-      atomicAdd(reinterpret_cast<uint32_t*>(&s.bins[m < 63 ? m : 63]), 1u);
+      if (m > 0) atomicAdd(reinterpret_cast<uint32_t*>(&s.bins[m < 63 ? m : 63]), 1u);
     }
   });
   sync<NT>();
