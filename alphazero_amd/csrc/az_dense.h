@@ -69,7 +69,7 @@ __device__ __forceinline__ void keep(az_f16* p, float z) {
 // significant bits: to 2^-16 of itself at least (bfloat16; float16: 2^-22), where rounding it to the type alone would add as much
 // to the gradients' errors as their own last rounding does (1.41 to 1.46 times that rounding's error in all, measured from
 // 300 x 520 x 264 on; 1.00 with two planes, float16 1.05 by its z).  The products run over the lo plane, scale, and go on over the
-// hi plane: twice the matrix instructions, dx and dkernel of 16384 x 4096 x 4096 bfloat16 866 and 824 us (432 and 411 over one
+// hi plane: twice the matrix instructions, dx and dkernel of 16384 x 4096 x 4096 bfloat16 830 and 791 us (418 and 398 over one
 // plane, as a layer without an activation or with relu has it).
 template <typename T>
 struct Low {

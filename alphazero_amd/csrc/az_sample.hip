@@ -14,10 +14,11 @@
 // other: that gives each its place in the descending order and the weight ahead of it at once.  A row whose list would
 // not fit (ties, a flat distribution) is left to a second kernel that works over the row in memory.
 //
-// 4096 x 32768 float32, top_k 100 and top_p 0.9: 166 us, of which reading the 537 MB takes 126-139 in this form (104 at a
+// 4096 x 32768 float32, top_k 100 and top_p 0.9: 164 us, of which reading the 537 MB takes 126-139 in this form (104 at a
 // large copy's rate: two rows a compute unit are in flight, as many as the registers hold); 4096 x 362 with a mask and
 // top_p: 15 us, the latency of a wave's steps; 64 x 18: 5 us.  Bound by the weights' exponentials in 64 bits instead:
-// top_p alone over 4096 x 32768, 840 us for normal logits of deviation 2.5, 1.9 ms for flat ones.
+// top_p alone over 4096 x 32768, for normal logits of deviation 2.5 0.48 ms at 0.8 (all rows end in the list), 0.88 at 0.9, 1.6
+// at 0.95, 1.9 for equal logits; no cut 0.29.  2048 x 65536, whose rows are read again for each pass, 296 us (as above).
 #include <hip/hip_runtime.h>
 
 #include <cfloat>
@@ -916,7 +917,7 @@ void launch_group(const az_sample_desc& d, int32_t* action, float* log_prob, dou
     k_sample_group<T, 512, CHUNKS, true><<<dim3(d.rows), dim3(512), 0, stream>>>(d, action, log_prob, unit);
   } else {
     // (the rows left are often all or none: a workgroup a row up to 1024, so that all of them share the work; 4096 x
-    // 32768 with top_p alone 842 us against 988 with eight rows a workgroup at every size)
+    // 32768 with top_p 0.9 alone 842 us against 988 with eight rows a workgroup at every size)
     const int per = d.rows >= 8192 ? 8 : d.rows >= 1024 ? d.rows / 1024 : 1;
     k_sample_group<T, 512, CHUNKS, false><<<dim3(d.rows), dim3(512), 0, stream>>>(d, action, log_prob, unit);
     k_sample_rest<T, 512><<<dim3((unsigned)az_ceil(d.rows, per)), dim3(512), 0, stream>>>(d, action, log_prob, unit, per);
@@ -944,6 +945,9 @@ extern "C" int az_sample_actions(const az_sample_desc* d, int32_t* action, float
     constexpr int V = 16 / sizeof(T);
     const int n = d->actions;
     const dim3 rows(d->rows);
+    // In microseconds, no cut / top_p 0.9 / top_k 100 too.  A wave a row against a workgroup: 4096 x 300 13 / 16 / 20 against 58 / 83 /
+    // 119, 4096 x 1000 27 / 48 / 23 against 69 / 142 / 124, 64 x 1000 15 / 18 / 13 against 10 / 20 / 16.  The row in registers against read
+    // again for each pass: 4096 x 32768 246 / 864 / 163 against 279 / 971 / 311, 4096 x 20000 238 / 444 / 167 against 185 / 442 / 232.
     if (n <= 256)
       k_sample_wave<T, 256, 1><<<rows, dim3(64), 0, stream>>>(*d, action, log_prob, unit);
     else if (n <= 512)

@@ -84,8 +84,8 @@ def mse_value_loss(values, targets):
 
 def mlp_apply(layers, x, native=False):
     """networks/networks.py:25-48: Dense + swish on all but the last layer.
-    native: every layer is one layers.dense (one launch forward, four backward) instead of library
-    calls; the same sums in another order."""
+    native: every layer is one layers.dense (a small one's forward pass is one launch, its backward pass two)
+    instead of library calls; the same sums in another order."""
     if native:
         for i, (w, b) in enumerate(layers):
             x = layers_lib.dense(x, w, b, "swish" if i + 1 < len(layers) else None)
