@@ -63,7 +63,8 @@ int64_t az_dense_workspace_bytes(int32_t dtype, int32_t rows, int32_t fan_in, in
 /* y = (x - mean) * rstd * scale + bias over the last axis of x[rows, width], with the biased variance
  * and rstd = 1 / sqrt(variance + eps).  scale and bias [width] may each be NULL (1 and 0); they have the type
  * `param_dtype`, which is `dtype` or AZ_TYPE_F32.  mean and rstd [rows] float32 (both or neither NULL) are
- * kept for az_layer_norm_backward. */
+ * kept for az_layer_norm_backward.  Sums are float32: a row whose values or squared differences add up to more than
+ * that holds (deviations around 1e19) has an infinite variance. */
 int az_layer_norm_forward(int32_t dtype, int32_t param_dtype, int32_t rows, int32_t width, const void* x,
                           const void* scale, const void* bias, float eps, void* y, float* mean, float* rstd,
                           void* stream);
