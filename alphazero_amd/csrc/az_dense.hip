@@ -486,9 +486,10 @@ int64_t splits_for(int64_t tiles, int64_t want, int64_t K, int64_t least) {
 // 4096 x 4096 dx 31 / 15 (two planes 64 / 25, float32 59 / 34).
 // Up to 2560 tiles of 16-bit operands that the wide kernel would have to copy, if dx and dkernel are both so small: they then
 // share one launch.  A backward pass that way / on 64 x 64 tiles, relu: 1003 x 401 x 517 32 / 39, 700 x 391 x 900 28 / 37,
-// 1001 x 257 x 600 21 / 35, 2003 x 129 x 301 28 / 30, 611 x 333 x 999 32 / 42; swish 56 / 61, 46 / 58, 35 / 54, 42 / 46, 58 / 73.  With one
-// product alone it does not pay: 1003 x 1003 x 403 50 / 40, 901 x 901 x 450 47 / 38, 515 x 515 x 1111 49 / 45, 1025 x 517 x 401
-// 40 / 35, and for y 16.1 / 13.0 (1001 x 257 x 600), 20.3 / 16.8 (901 x 901 x 450), 12.4 / 10.3 (2003 x 129 x 301), 12.9 / 17.1 (1025 x 517 x 401).
+// 1001 x 257 x 600 21 / 35, 2003 x 129 x 301 28 / 30, 611 x 333 x 999 32 / 42; swish 56 / 61, 46 / 58, 35 / 54, 42 / 46,
+// 58 / 73.  With one product alone it does not pay: 1003 x 1003 x 403 50 / 40, 901 x 901 x 450 47 / 38, 515 x 515 x 1111 49 / 45,
+// 1025 x 517 x 401 40 / 35, and for y 1001 x 257 x 600 16.1 / 13.0, 901 x 901 x 450 20.3 / 16.8, 2003 x 129 x 301 12.4 / 10.3,
+// 1025 x 517 x 401 12.9 / 17.1.
 bool small_pair(int dtype, int64_t M, int64_t N, int64_t K, bool in_place) {
   return dtype != AZ_TYPE_F32 && !in_place && az_ceil(M, 16) * az_ceil(N, 16) <= 2560 && K <= 1024;
 }

@@ -15,16 +15,16 @@
 // PFLOP/s; a library product of that size reaches 1.2), at which the matrix pipes are busy 0.69 and 0.63 of the cycles of a
 // clock that the power limit holds near 2 GHz; over dz's two planes 791 and 850, 830 and 887 us.  The forward pass takes
 // 522-552 us at best, 563-584 on average, its pipes busy 0.5 of the cycles: its epilogue moves another 400 MB that nothing
-// overlaps (one workgroup a compute unit: two stages are 128 KB).  LDS is busy a quarter of the cycles, without bank conflicts.  Measured and not kept: four
-// waves of 128 x 128 (fewer LDS reads, but one wave a SIMD: 1.83 ms a step instead of 1.52), three to five stages for the
+// overlaps (one workgroup a compute unit: two stages are 128 KB).  LDS is busy a quarter of the cycles, without bank
+// conflicts.  Measured and not kept: four waves of 128 x 128 (fewer LDS reads, but one wave a SIMD: 1.83 ms a step instead of 1.52), three to five stages for the
 // 128 x 128 tiles (8192 x 1024 x 1024: 44 us instead of 28: their loads already fill the way from L2, 64 bytes a cycle).
 //
 // float32 products run on the same instructions: an operand is split into three bfloat16 planes x = x0 + x1 + x2
 // (each the rounding of what the planes before it left, so the three hold all 24 bits), and of the nine products the
 // six that matter, x0 y0, x0 y1, x1 y0, x1 y1, x0 y2, x2 y0, are added in one float32 accumulator, the small ones
 // first.  What is left out is below 2^-26 of the terms' magnitudes; operands below 2^-110 lose bits of their last plane
-// (products of values around 2^-114 are off by 6e-7 instead of 1.2e-7 at 1400 x 1300 x 1400, around 2^-118 by 9e-6).  Six bfloat16 products cost 6 / 16 of
-// the float32 instruction's time.  An infinity or an overflow turns into NaN on the way (inf - inf, inf * 0): an output
+// (products of values around 2^-114 are off by 6e-7 instead of 1.2e-7 at 1400 x 1300 x 1400, around 2^-118 by 9e-6).  Six
+// bfloat16 products cost 6 / 16 of the float32 instruction's time.  An infinity or an overflow turns into NaN on the way (inf - inf, inf * 0): an output
 // that is not finite is worked out again from the float32 operands by the float32 instruction, 16 rows of a wave at a time.
 #include <hip/hip_runtime.h>
 

@@ -1039,3 +1039,33 @@ def test_sample_actions_many_rows_left_to_the_second_kernel(B):
             assert torch.equal(a, action[part]) and torch.equal(l, lp[part])
         rows = torch.cat([at[:8], at[-8:]])
         check_sample(logits[rows], u[rows], **{k: v[rows] if torch.is_tensor(v) else v for k, v in kw.items()})
+
+
+@pytest.mark.parametrize("T", TYPES, ids=str)
+@pytest.mark.parametrize("M,K,N", [(70, 96, 80), (300, 520, 264), (901, 901, 450), (1300, 1304, 1300)])
+def test_dense_gradients_of_infinite_operands(T, M, K, N):
+    """C ABI: an infinity of x reaches its row of dkernel and one of the kernel its column of dx, as infinities, over either
+    plane of dz too; nothing else changes."""
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[T]
+    x, w, dy = rand((M, K), T, 1), rand((K, N), T, 2, K ** -0.5), rand((M, N), T, 3)
+    z = rand((M, N), torch.float32 if T == torch.float32 else torch.float16, 4)
+    lib = nat.lib()
+    n = lib.az_dense_workspace_bytes(code, M, K, N, 1)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+
+    def gradients(x, w):
+        dx, dw = torch.empty_like(x), torch.empty_like(w)
+        nat.check(lib.az_dense_backward(code, nat.ACT_SWISH, M, K, N, nat.ptr(x), nat.ptr(w), nat.ptr(z), nat.ptr(dy), nat.ptr(dx),
+                                        nat.ptr(dw), None, nat.ptr(ws), n, nat.stream_ptr()))
+        return dx, dw
+    dx, dw = gradients(x, w)
+    x2, w2 = x.clone(), w.clone()
+    x2[3, 5], w2[7, 9] = math.inf, -math.inf
+    dx2, dw2 = gradients(x2, w2)
+    # (a slope's sign: swish falls below z = -1.278; values around it and of dy around 0 are left out)
+    dz = dy.double() * act64(z.double(), "swish")[1]
+    clear = dz.abs() > 1e-3
+    rows, cols = [i for i in range(K) if i != 5], [i for i in range(K) if i != 7]
+    assert torch.equal(dw2[rows], dw[rows]) and torch.equal(dx2[:, cols], dx[:, cols])
+    assert torch.equal(dw2[5].double()[clear[3]], (dz[3] * math.inf)[clear[3]])
+    assert torch.equal(dx2[:, 7].double()[clear[:, 9]], (dz[:, 9] * -math.inf)[clear[:, 9]])
